@@ -281,6 +281,58 @@ int tw4_gemv_f16_configs(int* out, int max_configs);
  * runs (python/tandem/layers/attention.py). */
 int tw4_attend_one(const uint16_t* qkv, uint16_t* y, int M, int heads, int kv_heads, int head_dim, void* stream);
 
+/* RMS norm of each query and key head, rotation by position, and the write of keys and values into a paged cache, in one pass.
+ * qkv [tokens, (heads + 2 kv_heads) head_dim] = [q | k | v] of fp16 (bf16 = 1: bfloat16), rows row_stride values apart; positions
+ * int32 [tokens]; table float32 [table_rows, head_dim] = cos | sin; q_weight, k_weight [head_dim] or NULL (no norm). q_out
+ * [tokens, heads, head_dim]. slots NULL: k_out [tokens, kv_heads, head_dim], v_out unused. Otherwise k_out and v_out are caches of
+ * num_pages pages with these strides (in values) of pages, heads and tokens, and token t goes to page slots[t] / page_size,
+ * offset slots[t] % page_size; a slot outside of the cache is not written. A position outside of the table gives NaN.
+ * head_dim 64 or 128, page_size 16, 32, 64, 128 or 256, every operand 16-byte aligned, strides multiples of 8.
+ * Replaces _qkv_prologue_kernel (python/tandem/layers/triton_ops.py:22-99). */
+int tw4_norm_rope(const uint16_t* qkv, int64_t row_stride, const int32_t* positions, const float* table, int table_rows,
+                  const uint16_t* q_weight, const uint16_t* k_weight, float eps, uint16_t* q_out, uint16_t* k_out,
+                  uint16_t* v_out, const int32_t* slots, int num_pages, int page_size, int64_t page_stride,
+                  int64_t head_stride, int64_t token_stride, int tokens, int heads, int kv_heads, int head_dim, int bf16,
+                  void* stream);
+
+/* The pages, positions and slots of a step's new tokens. Request i of `batch` (1 .. 4096) has context[i] tokens in the pages
+ * table[i * table_stride ..] (width entries) and brings fresh[i] more; the first *taken of n_free free_pages are in use. Writes the new
+ * pages into table, *taken_out, starts [batch + 1] (first row of each request), lens [batch] = context + fresh, positions and
+ * slots [tokens] (0 and -1 behind the last request; -1 where there is no page), and counts [4]: new tokens, pages given, pages
+ * the list lacked, new tokens past `tokens`. lens may be context, taken_out taken. page_size as in tw4_norm_rope.
+ * Replaces the host's block allocator and slot maps (python/tandem/cache/, executor/model_runner.py). */
+int tw4_plan_pages(const int32_t* context, const int32_t* fresh, int32_t* table, int64_t table_stride, int width,
+                   const int32_t* free_pages, int n_free, const int32_t* taken, int32_t* taken_out, int page_size,
+                   int32_t* starts, int32_t* lens, int32_t* positions, int32_t* slots, int32_t* counts, int batch,
+                   int tokens, void* stream);
+
+/* The pages of requests ended[0 .. count) back to the list, in place: *taken falls by their number, their rows of the table become
+ * -1 and their lengths 0. Indices outside of 0 .. batch - 1 are passed over. */
+int tw4_release_pages(const int32_t* ended, int count, int32_t* table, int64_t table_stride, int width, int32_t* lens,
+                      int batch, int32_t* free_pages, int n_free, int32_t* taken, int page_size, void* stream);
+
+/* Causal attention of new tokens over a paged cache: q [tokens, heads, head_dim] (strides q_token, q_head), caches as
+ * tw4_norm_rope writes them, table [batch, width] int32 (row stride table_stride), lens [batch] keys of each request (its new tokens
+ * among them), starts [batch + 1] first row of each request, or NULL: one row per request (tokens == batch). out [tokens, heads,
+ * head_dim], fp16 (bf16 = 1: bfloat16). Row t of a request's n sees keys j <= len - n + t. Entries of the table that are no page,
+ * and keys behind its width, are left out; a row that sees no key is zero; rows from starts[batch] on are not written. No
+ * content of table, lens or starts makes it touch anything outside of the operands. rows, splits: from tw4_paged_attention_plan
+ * (any of its values is valid for any call); splits > 1 takes ws and locks (zero before the first call, and after each; calls
+ * that share them must not overlap), TW4_ESPACE if they are too small.
+ * Replaces the reference's attention backends (python/tandem/layers/flashinfer_attention.py, triton_decode_attn.py). */
+int tw4_paged_attention(const uint16_t* q, int64_t q_token, int64_t q_head, const uint16_t* k, const uint16_t* v,
+                        int64_t page_stride, int64_t head_stride, int64_t token_stride, int num_pages, int page_size,
+                        const int32_t* table, int64_t table_stride, int width, const int32_t* lens, const int32_t* starts,
+                        uint16_t* out, float* ws, int64_t ws_floats, int32_t* locks, int64_t n_locks, int tokens,
+                        int batch, int heads, int kv_heads, int head_dim, float scale, int rows, int splits, int bf16,
+                        void* stream);
+
+/* How tw4_paged_attention divides a call of these sizes on a device of `cus` CUs (max_query, max_keys: the most new tokens and
+ * keys a request can have; single: starts is NULL): writes rows of a tile, splits, and the floats and counters that takes to
+ * out[0 .. 4). Splits stay within TW4_AUTO_SPLIT_FLOATS and TW4_AUTO_SPLIT_COUNTERS. Host code. */
+int tw4_paged_attention_plan(int tokens, int batch, int heads, int kv_heads, int head_dim, int max_query, int max_keys,
+                             int single, int cus, int* out);
+
 /* RMSNorm of the decoder layer around the projections, fp16 rows [M, K], fp32 math, K % 512 == 0,
  * K <= 8192, rows 16-byte aligned. y = fp16(x * rsqrt(mean(x^2) + eps) * weight).
  * Replaces ops.rms_norm of the GPU path (python/tandem/layers/ops.py:107-109, FlashInfer's

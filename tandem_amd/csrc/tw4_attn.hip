@@ -1,0 +1,464 @@
+// Causal attention of new tokens over a paged cache, grouped-query heads. Request i of the batch has len_i keys in its pages, the
+// last n_i of them those of its new tokens (rows start_i .. start_i + n_i - 1 of q); new token t sees the keys
+// j <= len_i - n_i + t:
+//
+//   o = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale (q . k_j) - max)
+//
+// in one pass over the keys with a running maximum and sum in fp32 (the online softmax: when a block of keys raises the maximum,
+// what was summed so far is scaled by exp(old - new)).
+//
+// The G = heads / kv_heads query heads of a KV head are rows of one tile, row r = t G + g, so a KV head's keys are read once for
+// all of them. Scores are computed transposed, S^T = K Q^T: a lane of the matrix instruction's result then holds one row's scores
+// of several keys, its limit, maximum and sum are one register each, and its probabilities are already where the second
+// product O^T = V^T P^T wants them (the order of keys inside a product is free: K's rows and V^T's columns only have to agree).
+// Probabilities are rounded to the cache's type for that product (at most half a step of the type, relative, each: the same size
+// as the rounding of the result); their sum is of the unrounded values.
+//
+// Rows kernel: a workgroup has one tile of 16 MT rows and a range of keys; its four wavefronts take blocks of 32 keys in turn, each
+// with a softmax of its own, joined at the end. K comes straight into registers (a lane has 16 bytes of a key), V through a
+// wavefront's own LDS, read back transposed. With few rows in flight the keys are split over `splits` workgroups; the last to arrive
+// joins their results in order.
+#include <algorithm>
+
+#include "tw4_attn.h"
+
+namespace tw4 {
+
+struct AttnArgs {
+    const uint16_t* q;
+    const uint16_t* k;
+    const uint16_t* v;
+    const int32_t* table;
+    const int32_t* lens;
+    const int32_t* starts;  // null: one row per request
+    uint16_t* out;          // [tokens, heads, D]
+    float* ws;
+    int32_t* locks;
+    int64_t q_token, q_head, page_stride, head_stride, token_stride, table_stride;
+    float scale;  // times log2(e)
+    int tokens, batch, heads, kv_heads, group, num_pages, width, shift, splits, slots;
+};
+
+constexpr int kTileFloats = 2;  // per row beside its D sums: maximum and sum
+
+// A tile of rows: its request, first row, and the keys it can see.
+struct Tile {
+    int request, first, rows;  // rows of the request from `first` on, at least 1
+    int start, len, fresh;     // the request's first token, keys, new tokens
+};
+
+// Slot s of the grid is a tile of request i, the last i with base_i = floor(start_i G / B) + i <= s: the base of the next request
+// is at least ceil(n_i G / B) further on, so no scan of the lengths is needed; slots past a request's rows have none. Each wavefront
+// looks at 64 requests at a time.
+template <int B>
+__device__ __forceinline__ bool find_tile(const AttnArgs& a, int slot, int lane, Tile& t) {
+    int start, fresh;
+    if (a.starts) {
+        int lo = 0, step = 64;
+        while (step < a.batch) step *= 64;
+        for (; step > 1;) {
+            step /= 64;
+            const int64_t i = lo + static_cast<int64_t>(lane) * step;
+            bool before = false;
+            if (i < a.batch) {
+                const int s = min(max(a.starts[i], 0), a.tokens);
+                before = static_cast<int64_t>(s) * a.group / B + i <= slot;
+            }
+            lo += step * max(__popcll(__ballot(before)) - 1, 0);
+        }
+        t.request = __builtin_amdgcn_readfirstlane(lo);
+        start = min(max(a.starts[t.request], 0), a.tokens);
+        fresh = min(max(a.starts[t.request + 1], start), a.tokens) - start;
+        t.first = (slot - static_cast<int>(static_cast<int64_t>(start) * a.group / B) - t.request) * B;
+    } else {
+        const int per = (a.group + B - 1) / B;
+        t.request = slot / per;
+        start = t.request;
+        fresh = 1;
+        t.first = (slot - t.request * per) * B;
+    }
+    t.start = start;
+    t.fresh = fresh;
+    t.len = a.lens[t.request];
+    t.rows = fresh * a.group - t.first;
+    return t.first >= 0 && t.rows > 0;
+}
+
+// Where the 16 bytes of chunk c of row r lie in a wavefront's V tile of D-value rows: the chunks of a row change places with
+// the row in pairs of 32 bytes, so that a transposed read (4 rows of 32 bytes for each 16 lanes) meets every bank once.
+template <int D>
+__device__ __forceinline__ int v_chunk(int r, int c) {
+    return D == 128 ? r * 16 + (c ^ ((r & 7) << 1)) : r * 8 + (c ^ (((r >> 1) & 3) << 1));
+}
+
+__device__ __forceinline__ u2 read_tr(const u4* lds, int byte) {
+    typedef __attribute__((address_space(3))) s4 lds_s4;
+    return bitcast<u2>(__builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds_s4*)(reinterpret_cast<const char*>(lds) + byte)));
+}
+
+// Largest of the four values a column has in lanes c, c + 16, c + 32, c + 48. A NaN is passed over.
+__device__ __forceinline__ float max_rows(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    const float s = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(s), __float_as_uint(s), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+__device__ __forceinline__ bool odd16(uint32_t v, uint32_t exponent) {  // either half infinite or NaN
+    return (v & exponent) == exponent || ((v >> 16) & exponent) == exponent;
+}
+
+constexpr float kNone = -__builtin_inff();
+
+template <typename T, int D, int MT>
+__global__ void __launch_bounds__(256) rows_kernel(AttnArgs a) {
+    constexpr int B = 16 * MT, KS = D / 32, DT = D / 16, C = D / 8, VJ = C / 2;  // VJ: 1 KB loads of 32 keys
+    constexpr uint32_t kExponent = __is_same(T, h1) ? 0x7C00u : 0x7F80u;
+    static_assert(32 * D * 2 * 4 >= 4 * 16 * D * 4, "the join of 16 rows uses the V tiles' LDS");
+    __shared__ u4 lds[4 * 32 * C];
+    __shared__ float stat[2][4][B];
+    __shared__ int last_flag;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c16 = lane & 15, g4 = lane >> 4;
+    const int slot = blockIdx.x / a.kv_heads, head = blockIdx.x - slot * a.kv_heads, split = blockIdx.y;
+    Tile t;
+    if (!find_tile<B>(a, slot, lane, t)) return;
+
+    // this lane's rows: limits (last key seen), queries
+    int limit[MT], low = 0x7FFFFFFF, high = -1;
+    u4 q[MT][KS];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const int r = t.first + 16 * m + c16;
+        const bool there = 16 * m + c16 < t.rows;
+        const int tok = r / a.group, g = r - tok * a.group;
+        limit[m] = there ? t.len - t.fresh + tok : -1;
+        if (there) low = min(low, limit[m]), high = max(high, limit[m]);
+        const uint16_t* src = a.q + (t.start + tok) * a.q_token + (head * a.group + g) * a.q_head + 8 * g4;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) q[m][s] = there ? *reinterpret_cast<const u4*>(src + 32 * s) : u4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) low = min(low, __shfl_xor(low, d)), high = max(high, __shfl_xor(high, d));
+    low = __builtin_amdgcn_readfirstlane(low), high = __builtin_amdgcn_readfirstlane(high);
+
+    // keys [0, end), this workgroup's share [begin, stop) of them
+    const int end = static_cast<int>(min(static_cast<int64_t>(high) + 1, static_cast<int64_t>(a.width) << a.shift));
+    int begin = 0, stop = max(end, 0), parts = 1;
+    if (a.splits > 1 && end > 0) {
+        const int share = max((end + a.splits - 1) / a.splits, 128);
+        const int whole = (share + 127) & ~127;
+        parts = (end + whole - 1) / whole;
+        if (split >= parts) return;
+        begin = split * whole;
+        stop = min(end, begin + whole);
+    } else if (split > 0) {
+        return;
+    }
+
+    f4 o[MT][DT];
+    float top[MT], sum[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        top[m] = kNone, sum[m] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[m][d] = f4{0, 0, 0, 0};
+    }
+    u4* vt = lds + wave * 32 * C;
+    const int32_t* table = a.table + t.request * a.table_stride;
+    const uint16_t* kh = a.k + head * a.head_stride;
+    const uint16_t* vh = a.v + head * a.head_stride;
+    const int final16 = (stop - 1) & ~15;  // the last 16 keys that are there
+
+    for (int base = begin + 32 * wave; base < stop; base += 128) {
+        // the pages of the block's two halves; a page the table does not have is page 0, read and left out
+        int64_t at[2];
+        int absent = 0, first[2], lastrow[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            first[h] = min(base + 16 * h, final16);
+            const int page = table[first[h] >> a.shift];
+            const bool there = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.num_pages);
+            absent |= there ? 0 : 1 << h;
+            at[h] = (there ? page : 0) * a.page_stride + (first[h] & ((1 << a.shift) - 1)) * a.token_stride;
+            lastrow[h] = min(stop - 1 - first[h], 15);
+        }
+        u4 kf[2][KS], vf[VJ];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint16_t* src = kh + at[h] + min(c16, lastrow[h]) * a.token_stride + 8 * g4;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) kf[h][s] = *reinterpret_cast<const u4*>(src + 32 * s);
+        }
+#pragma unroll
+        for (int j = 0; j < VJ; ++j) {  // chunk lane % C of row lane / C + j (64 / C)
+            const int row = lane / C + j * (64 / C), h = j * 2 / VJ;
+            vf[j] = *reinterpret_cast<const u4*>(vh + at[h] + min(row & 15, lastrow[h]) * a.token_stride + 8 * (lane % C));
+        }
+#pragma unroll
+        for (int j = 0; j < VJ; ++j) vt[v_chunk<D>(lane / C + j * (64 / C), lane % C)] = vf[j];
+
+        const bool masked = absent || base + 32 > min(low + 1, stop);
+        u4 p[MT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            f4 s[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                s[0] = mma16<T>(kf[0][i], q[m][i], s[0]);
+                s[1] = mma16<T>(kf[1][i], q[m][i], s[1]);
+            }
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = s[i >> 2][i & 3] * a.scale;
+            if (masked) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int key = base + 16 * (i >> 2) + 4 * g4 + (i & 3);
+                    if (key > min(limit[m], stop - 1) || (absent >> (i >> 2) & 1)) x[i] = kNone;
+                }
+            }
+            float high8 = x[0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) high8 = fmaxf(high8, x[i]);
+            const float now = fmaxf(top[m], max_rows(high8));
+            const float zero = now == kNone ? 0.0f : now;  // a row that has seen nothing yet
+            const float keep = __builtin_amdgcn_exp2f(top[m] - zero);
+            top[m] = now;
+            sum[m] *= keep;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[i] = __builtin_amdgcn_exp2f(x[i] - zero);
+                sum[m] += x[i];
+            }
+            p[m] = from_f32<T>(x);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[m][d] *= keep;
+        }
+        // V back, transposed: 4 rows x 16 columns for each 16 lanes
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            const int r = 4 * g4 + (c16 >> 2), c = 2 * d + ((c16 & 3) >> 1), half = (c16 & 1) * 8;
+            const u2 lo = read_tr(vt, v_chunk<D>(r, c) * 16 + half), hi = read_tr(vt, v_chunk<D>(r + 16, c) * 16 + half);
+            u4 w = u4{lo.x, lo.y, hi.x, hi.y};
+            if (masked) {
+                // A probability of zero does not take an infinity or NaN away: where some row does not see a key, such values
+                // are taken out of the product and added to the rows that see them.
+                bool odd = false;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) odd |= odd16(w[i], kExponent);
+                if (__ballot(odd)) {
+#pragma unroll
+                    for (int m = 0; m < MT; ++m)
+#pragma unroll 1
+                        for (int key = 0; key < 32; ++key) {
+                            if (base + key > min(limit[m], stop - 1) || (absent >> (key >> 4) & 1)) continue;
+                            const uint16_t* row = reinterpret_cast<const uint16_t*>(vt);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const int col = 16 * d + 4 * g4 + i;
+                                const uint16_t bits = row[v_chunk<D>(key, col >> 3) * 8 + (col & 7)];
+                                if ((bits & kExponent) == kExponent) o[m][d][i] += static_cast<float>(bitcast<T>(bits));
+                            }
+                        }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if ((w[i] & kExponent) == kExponent) w[i] &= 0xFFFF0000u;
+                        if (((w[i] >> 16) & kExponent) == kExponent) w[i] &= 0xFFFFu;
+                    }
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < MT; ++m) o[m][d] = mma16<T>(w, p[m], o[m][d]);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+
+    // the four wavefronts' results become one, 16 rows at a time through LDS
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const float l = sum_rows(sum[m]);
+        if (g4 == 0) stat[0][wave][16 * m + c16] = top[m], stat[1][wave][16 * m + c16] = l;
+    }
+    float* od = reinterpret_cast<float*>(lds);  // [wave][row][D]
+    constexpr int PER = D / 16;                 // values of a row per thread: row threadIdx / 16
+    const int row = threadIdx.x >> 4, col = (threadIdx.x & 15) * PER;
+    const int unit = slot * a.kv_heads + head;
+    constexpr int kRowFloats = D + kTileFloats;
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(a.ws, 0, 0x7FFFFFFF, kBufferFlags);
+    float res[MT][PER], rtop[MT], rsum[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        __syncthreads();
+#pragma unroll
+        for (int d = 0; d < DT; ++d) *reinterpret_cast<f4*>(od + (wave * 16 + c16) * D + 16 * d + 4 * g4) = o[m][d];
+        __syncthreads();
+        rtop[m] = kNone;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) rtop[m] = fmaxf(rtop[m], stat[0][w][16 * m + row]);
+        const float zero = rtop[m] == kNone ? 0.0f : rtop[m];
+        rsum[m] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) res[m][i] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            // a wavefront without keys has sums of zero
+            const float f = __builtin_amdgcn_exp2f(stat[0][w][16 * m + row] - zero);
+            rsum[m] += f * stat[1][w][16 * m + row];
+#pragma unroll
+            for (int i = 0; i < PER; ++i) res[m][i] += f * od[(w * 16 + row) * D + col + i];
+        }
+    }
+    if (parts > 1) {
+        // [unit][split][row][D + 2]: the sums, then maximum and sum
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            const int to = static_cast<int>(((static_cast<int64_t>(unit) * a.splits + split) * B + 16 * m + row) * kRowFloats * 4);
+#pragma unroll
+            for (int i = 0; i < PER; i += 2)
+                __builtin_amdgcn_raw_buffer_store_b64(u2{__float_as_uint(res[m][i]), __float_as_uint(res[m][i + 1])}, rs, to,
+                                                      (col + i) * 4, kCoherentAux);
+            if (col == 0)
+                __builtin_amdgcn_raw_buffer_store_b64(u2{__float_as_uint(rtop[m]), __float_as_uint(rsum[m])}, rs, to, D * 4,
+                                                      kCoherentAux);
+        }
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (threadIdx.x == 0)
+            last_flag = __hip_atomic_fetch_add(a.locks + unit, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
+        __syncthreads();
+        if (!last_flag) return;
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            rtop[m] = kNone, rsum[m] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) res[m][i] = 0.0f;
+            for (int s = 0; s < parts; ++s) {
+                const int from =
+                    static_cast<int>(((static_cast<int64_t>(unit) * a.splits + s) * B + 16 * m + row) * kRowFloats * 4);
+                const u2 ms = bitcast<u2>(__builtin_amdgcn_raw_buffer_load_b64(rs, from, D * 4, kCoherentAux));
+                const float mt = __uint_as_float(ms.x), now = fmaxf(rtop[m], mt), zero = now == kNone ? 0.0f : now;
+                const float keep = __builtin_amdgcn_exp2f(rtop[m] - zero), f = __builtin_amdgcn_exp2f(mt - zero);
+                rtop[m] = now;
+                rsum[m] = rsum[m] * keep + f * __uint_as_float(ms.y);
+#pragma unroll
+                for (int i = 0; i < PER; i += 2) {
+                    const u2 x = bitcast<u2>(__builtin_amdgcn_raw_buffer_load_b64(rs, from, (col + i) * 4, kCoherentAux));
+                    res[m][i] = res[m][i] * keep + f * __uint_as_float(x.x);
+                    res[m][i + 1] = res[m][i + 1] * keep + f * __uint_as_float(x.y);
+                }
+            }
+        }
+        if (threadIdx.x == 0) __hip_atomic_store(a.locks + unit, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        if (16 * m + row >= t.rows) continue;
+        const int r = t.first + 16 * m + row, tok = r / a.group, g = r - tok * a.group;
+        const bool nothing = rsum[m] == 0.0f;  // no key, or none with a score above -inf: zero (the largest adds 1)
+        const float inv = 1.0f / rsum[m];
+        uint16_t* dst = a.out + (static_cast<int64_t>(t.start + tok) * a.heads + head * a.group + g) * D + col;
+        T y[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) y[i] = static_cast<T>(nothing ? 0.0f : res[m][i] * inv);
+        if constexpr (PER == 8) {
+            *reinterpret_cast<u4*>(dst) = *reinterpret_cast<const u4*>(y);
+        } else {
+            *reinterpret_cast<u2*>(dst) = *reinterpret_cast<const u2*>(y);
+        }
+    }
+}
+
+constexpr int64_t kWorkspaceFloats = TW4_AUTO_SPLIT_FLOATS;
+
+int64_t tile_slots(int tokens, int batch, int group, int rows, bool single) {
+    if (single) return static_cast<int64_t>(batch) * ((group + rows - 1) / rows);
+    return static_cast<int64_t>(tokens) * group / rows + batch;
+}
+
+template <typename T, int D>
+int attn_launch(const AttnArgs& a, int rows, hipStream_t st) {
+    const dim3 grid(static_cast<unsigned>(a.slots) * a.kv_heads, a.splits);
+    if (rows == 16)
+        rows_kernel<T, D, 1><<<grid, 256, 0, st>>>(a);
+    else
+        rows_kernel<T, D, 2><<<grid, 256, 0, st>>>(a);
+    TW4_LAUNCH_CHECK("paged_attention: launch");
+    return TW4_OK;
+}
+
+}  // namespace tw4
+
+using namespace tw4;
+
+// out: rows of a tile, splits, workspace floats, counters
+extern "C" int tw4_paged_attention_plan(int tokens, int batch, int heads, int kv_heads, int head_dim, int max_query, int max_keys,
+                                        int single, int cus, int* out) {
+    TW4_REQUIRE(out && tokens >= 0 && batch >= 0 && kv_heads >= 1 && heads >= 1 && heads % kv_heads == 0 && head_dim >= 1 && cus >= 1,
+                TW4_EINVAL, "paged_attention_plan: bad sizes");
+    const int group = heads / kv_heads;
+    const int rows = static_cast<int64_t>(max_query) * group > 16 ? 32 : 16;
+    const int64_t units = tile_slots(tokens, batch, group, rows, single) * kv_heads;
+    int64_t splits = 1;
+    if (units > 0 && units < 2 * cus) {
+        splits = (2 * cus + units - 1) / units;
+        splits = std::min<int64_t>(splits, (static_cast<int64_t>(max_keys) + 127) / 128);
+        splits = std::min<int64_t>(splits, kWorkspaceFloats / (units * rows * (head_dim + kTileFloats)));
+        splits = std::max<int64_t>(splits, 1);
+    }
+    out[0] = rows;
+    out[1] = static_cast<int>(splits);
+    out[2] = splits > 1 ? static_cast<int>(units * splits * rows * (head_dim + kTileFloats)) : 0;
+    out[3] = splits > 1 ? static_cast<int>(units) : 0;
+    return TW4_OK;
+}
+
+extern "C" int tw4_paged_attention(const uint16_t* q, int64_t q_token, int64_t q_head, const uint16_t* k, const uint16_t* v,
+                                   int64_t page_stride, int64_t head_stride, int64_t token_stride, int num_pages, int page_size,
+                                   const int32_t* table, int64_t table_stride, int width, const int32_t* lens,
+                                   const int32_t* starts, uint16_t* out, float* ws, int64_t ws_floats, int32_t* locks,
+                                   int64_t n_locks, int tokens, int batch, int heads, int kv_heads, int head_dim, float scale,
+                                   int rows, int splits, int bf16, void* stream) {
+    TW4_REQUIRE(tokens >= 0 && batch >= 0 && heads >= 1 && kv_heads >= 1 && heads % kv_heads == 0, TW4_EINVAL,
+                "paged_attention: heads a multiple of kv_heads (%d, %d)", heads, kv_heads);
+    TW4_REQUIRE(head_dim == 64 || head_dim == 128, TW4_EINVAL, "paged_attention: head_dim 64 or 128 (%d)", head_dim);
+    const int shift = page_shift(page_size);
+    TW4_REQUIRE(shift >= 0, TW4_EINVAL, "paged_attention: page_size 16, 32, 64, 128 or 256 (%d)", page_size);
+    TW4_REQUIRE(scale > 0.0f && scale < 1e30f, TW4_EINVAL, "paged_attention: a positive scale (%g)", scale);
+    TW4_REQUIRE(rows == 16 || rows == 32, TW4_ECONFIG, "paged_attention: tiles of 16 or 32 rows (%d)", rows);
+    TW4_REQUIRE(width >= 0 && num_pages >= 0 && static_cast<int64_t>(num_pages) * page_size < 1LL << 31 &&
+                    static_cast<int64_t>(width) * page_size < 1LL << 31,
+                TW4_EINVAL, "paged_attention: fewer than 2^31 slots (%d pages of %d, %d per request)", num_pages, page_size, width);
+    TW4_REQUIRE(static_cast<int64_t>(tokens) * heads < 1LL << 31, TW4_EINVAL, "paged_attention: too many rows (%d tokens)", tokens);
+    TW4_REQUIRE(starts || tokens == batch, TW4_EINVAL, "paged_attention: without query starts one token per request (%d, %d)",
+                tokens, batch);
+    if (tokens == 0 || batch == 0) return TW4_OK;
+    TW4_REQUIRE(q && out && lens && (!width || table) && (!num_pages || (k && v)), TW4_EINVAL, "paged_attention: null pointer");
+    TW4_REQUIRE(num_pages > 0 || width == 0, TW4_EINVAL, "paged_attention: a cache without pages");
+    for (const void* p : {static_cast<const void*>(q), static_cast<const void*>(k), static_cast<const void*>(v),
+                          static_cast<const void*>(out)})
+        TW4_REQUIRE(reinterpret_cast<uintptr_t>(p) % 16 == 0, TW4_EINVAL, "paged_attention: operands must be 16-byte aligned");
+    TW4_REQUIRE(q_token % 8 == 0 && q_head % 8 == 0 && page_stride % 8 == 0 && head_stride % 8 == 0 && token_stride % 8 == 0,
+                TW4_EINVAL, "paged_attention: strides must be multiples of 8");
+    const int group = heads / kv_heads;
+    const int64_t slots = tile_slots(tokens, batch, group, rows, !starts), units = slots * kv_heads;
+    TW4_REQUIRE(units < 1LL << 31 && splits >= 1 && splits <= 65535, TW4_EINVAL, "paged_attention: grid (%lld tiles, %d splits)",
+                static_cast<long long>(units), splits);
+    if (splits > 1) {
+        const int64_t need = units * splits * rows * (head_dim + kTileFloats);
+        TW4_REQUIRE(ws && locks && need <= ws_floats && need < kMaxPartialFloats && units <= n_locks, TW4_ESPACE,
+                    "paged_attention: %d splits need %lld floats and %lld counters (got %lld, %lld)", splits,
+                    static_cast<long long>(need), static_cast<long long>(units), static_cast<long long>(ws_floats),
+                    static_cast<long long>(n_locks));
+    }
+    const AttnArgs a{q, k, v, table, lens, starts, out, ws, locks, q_token, q_head, page_stride, head_stride, token_stride,
+                     table_stride, scale * 1.44269504088896340736f, tokens, batch, heads, kv_heads, group, num_pages, width, shift,
+                     splits, static_cast<int>(slots)};
+    auto st = static_cast<hipStream_t>(stream);
+    if (bf16) return head_dim == 64 ? attn_launch<bf1, 64>(a, rows, st) : attn_launch<bf1, 128>(a, rows, st);
+    return head_dim == 64 ? attn_launch<h1, 64>(a, rows, st) : attn_launch<h1, 128>(a, rows, st);
+}

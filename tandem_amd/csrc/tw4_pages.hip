@@ -1,0 +1,224 @@
+// The bookkeeping of a step over a paged cache, on the GPU, from the lengths of the batch's requests: request i has c_i
+// tokens in the cache and brings n_i more. With page size P, pages_i(x) = min(ceil(x / P), W) and W the width of the table,
+//
+//   start_i = n_0 + .. + n_(i-1)                      the request's first row among the step's tokens
+//   len_i   = c_i + n_i
+//   first_i = taken + sum over j < i of (pages_j(len_j) - pages_j(c_j))
+//   table[i][pages_i(c_i) + j] = free[first_i + j]    for its j-th new page (-1 past the end of the list)
+//   position of row t of request i = c_i + t - start_i
+//   slot = table[i][position / P] P + position % P    (-1: no page, or a row behind the last request)
+//   taken <- min(first_last, length of the list)
+//
+// It moves a few KB and is bound by a launch and two or three dependent round trips to memory. One workgroup does the scan
+// and the tables, and for up to kInline rows the rows too: one launch for a decode step. Past that a second launch spreads
+// the rows over the GPU, finding each row's request by bisection in the starts.
+#include "tw4_attn.h"
+
+namespace tw4 {
+
+constexpr int kThreads = 1024, kPerThread = 4, kMaxBatch = kThreads * kPerThread, kInline = 8192;
+
+struct PageArgs {
+    const int32_t* context;
+    const int32_t* fresh;
+    int32_t* table;
+    int64_t table_stride;
+    const int32_t* free_pages;
+    const int32_t* taken;
+    int32_t* taken_out;
+    int32_t* starts;
+    int32_t* lens;
+    int32_t* positions;
+    int32_t* slots;
+    int32_t* counts;
+    int batch, tokens, width, n_free, shift;
+};
+
+// The last i with starts[i] <= at, starts[0] = 0 (requests without tokens come before the one that has the row).
+__device__ __forceinline__ int request_of(const int32_t* starts, int batch, int at) {
+    int lo = 0, hi = batch;  // starts[lo] <= at, starts[hi] > at or hi = batch
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (starts[mid] <= at) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ int pages_of(int64_t tokens, const PageArgs& a) {
+    return static_cast<int>(min((tokens + (1 << a.shift) - 1) >> a.shift, static_cast<int64_t>(a.width)));
+}
+
+// Row t's position and slot; context(i): the tokens request i had.
+template <typename F>
+__device__ __forceinline__ void place_row(const PageArgs& a, const int32_t* starts, F context, int t) {
+    int pos = 0, slot = -1;
+    if (t < starts[a.batch]) {
+        const int i = request_of(starts, a.batch, t);
+        pos = context(i) + (t - starts[i]);
+        const int page = pos >> a.shift;
+        const int id = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.width) ? a.table[i * a.table_stride + page] : -1;
+        if (id >= 0) slot = (id << a.shift) + (pos & ((1 << a.shift) - 1));
+    }
+    a.positions[t] = pos;
+    a.slots[t] = slot;
+}
+
+// Sums over the workgroup of two values per thread, exclusive prefixes in `x`, `y`, totals in `tx`, `ty`.
+__device__ __forceinline__ void scan2(int& x, int& y, int& tx, int& ty, int (*part)[2]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int sx = x, sy = y;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int ox = __shfl_up(sx, d), oy = __shfl_up(sy, d);
+        if (lane >= d) sx += ox, sy += oy;
+    }
+    if (lane == 63) part[wave][0] = sx, part[wave][1] = sy;
+    __syncthreads();
+    int bx = 0, by = 0;
+    tx = ty = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; ++w) {
+        if (w == wave) bx = tx, by = ty;
+        tx += part[w][0], ty += part[w][1];
+    }
+    x = bx + sx - x;
+    y = by + sy - y;
+}
+
+__global__ void __launch_bounds__(kThreads) pages_kernel(PageArgs a, int rows) {
+    __shared__ int part[kThreads / 64][2];
+    __shared__ int32_t starts[kMaxBatch + 1], first[kMaxBatch + 1], context[kMaxBatch];
+    const int tid = threadIdx.x, base = tid * kPerThread;
+    int n[kPerThread], need[kPerThread], sum_n = 0, sum_need = 0;
+    const int taken = min(max(*a.taken, 0), a.n_free);
+#pragma unroll
+    for (int j = 0; j < kPerThread; ++j) {
+        const int i = base + j;
+        n[j] = need[j] = 0;
+        if (i < a.batch) {
+            const int c = max(a.context[i], 0);
+            n[j] = max(a.fresh[i], 0);
+            need[j] = pages_of(static_cast<int64_t>(c) + n[j], a) - pages_of(c, a);
+            context[i] = c;
+            sum_n += n[j], sum_need += need[j];
+        }
+    }
+    int total, pages;
+    scan2(sum_n, sum_need, total, pages, part);
+#pragma unroll
+    for (int j = 0; j < kPerThread; ++j) {
+        const int i = base + j;
+        if (i < a.batch) {
+            starts[i] = sum_n, first[i] = sum_need;
+            a.starts[i] = sum_n;
+            a.lens[i] = context[i] + n[j];  // the lengths' arrays may be one: read above, written here
+            sum_n += n[j], sum_need += need[j];
+        }
+    }
+    if (tid == 0) {
+        starts[a.batch] = total, first[a.batch] = pages;
+        a.starts[a.batch] = total;
+        const int given = min(pages, a.n_free - taken);
+        *a.taken_out = taken + given;
+        a.counts[0] = total, a.counts[1] = given, a.counts[2] = pages - given;
+        a.counts[3] = max(total - a.tokens, 0);
+    }
+    __syncthreads();
+    for (int p = tid; p < pages; p += kThreads) {
+        const int i = request_of(first, a.batch, p);
+        const int from = taken + p;
+        a.table[i * a.table_stride + pages_of(context[i], a) + (p - first[i])] = from < a.n_free ? a.free_pages[from] : -1;
+    }
+    if (rows == 0) return;
+    __threadfence_block();
+    __syncthreads();
+    for (int t = tid; t < rows; t += kThreads) place_row(a, starts, [&](int i) { return context[i]; }, t);
+}
+
+__global__ void __launch_bounds__(256) rows_kernel(PageArgs a) {
+    const int t = blockIdx.x * 256 + threadIdx.x;
+    // what a request had is its length less its rows: the context's array may be the lengths'
+    if (t < a.tokens) place_row(a, a.starts, [&](int i) { return a.lens[i] - (a.starts[i + 1] - a.starts[i]); }, t);
+}
+
+// The pages of the listed requests go back to the front of what is left of the free list, in order of request and page;
+// their rows of the table become -1 and their lengths 0. One workgroup: it runs when requests end.
+__global__ void __launch_bounds__(kThreads) release_kernel(const int32_t* ended, int count, int32_t* table, int64_t table_stride,
+                                                           int width, int32_t* lens, int batch, int32_t* free_pages, int n_free,
+                                                           int32_t* taken, int shift) {
+    __shared__ int part[kThreads / 64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int left = min(max(*taken, 0), n_free);
+    for (int e = 0; e < count; ++e) {
+        const int i = ended[e];
+        if (i < 0 || i >= batch) continue;  // uniform
+        const int held = static_cast<int>(min((static_cast<int64_t>(max(lens[i], 0)) + (1 << shift) - 1) >> shift,
+                                              static_cast<int64_t>(width)));
+        for (int p0 = 0; p0 < width; p0 += kThreads) {
+            const int p = p0 + static_cast<int>(threadIdx.x);
+            const int id = p < held ? table[i * table_stride + p] : -1;
+            if (p < width) table[i * table_stride + p] = -1;
+            const uint64_t have = __ballot(id >= 0);
+            if (lane == 0) part[wave] = __popcll(have);
+            __syncthreads();
+            int before = 0, sum = 0;
+            for (int w = 0; w < kThreads / 64; ++w) {
+                if (w < wave) before += part[w];
+                sum += part[w];
+            }
+            before += __popcll(have & ((1ULL << lane) - 1));
+            if (id >= 0 && left - sum + before >= 0) free_pages[left - sum + before] = id;
+            left = max(left - sum, 0);
+            __syncthreads();
+        }
+        if (threadIdx.x == 0) lens[i] = 0;
+        __syncthreads();  // the same request again: nothing is left of it
+    }
+    if (threadIdx.x == 0) *taken = left;
+}
+
+}  // namespace tw4
+
+using namespace tw4;
+
+extern "C" int tw4_plan_pages(const int32_t* context, const int32_t* fresh, int32_t* table, int64_t table_stride, int width,
+                              const int32_t* free_pages, int n_free, const int32_t* taken, int32_t* taken_out, int page_size,
+                              int32_t* starts, int32_t* lens, int32_t* positions, int32_t* slots, int32_t* counts, int batch,
+                              int tokens, void* stream) {
+    const int shift = page_shift(page_size);
+    TW4_REQUIRE(shift >= 0, TW4_EINVAL, "plan_pages: page_size 16, 32, 64, 128 or 256 (%d)", page_size);
+    TW4_REQUIRE(batch >= 1 && batch <= kMaxBatch, TW4_EINVAL, "plan_pages: 1 to %d requests (%d)", kMaxBatch, batch);
+    TW4_REQUIRE(tokens >= 0 && tokens < 1 << 30, TW4_EINVAL, "plan_pages: 0 <= tokens < 2^30 (%d)", tokens);
+    TW4_REQUIRE(width >= 0 && n_free >= 0 && table_stride >= width && static_cast<int64_t>(batch) * width < 1LL << 31,
+                TW4_EINVAL, "plan_pages: a table of fewer than 2^31 entries whose rows do not overlap (width %d, stride %lld)",
+                width, static_cast<long long>(table_stride));
+    TW4_REQUIRE(context && fresh && taken && taken_out && starts && lens && counts && (table || !width) &&
+                    (free_pages || !n_free) && ((positions && slots) || !tokens),
+                TW4_EINVAL, "plan_pages: null pointer");
+    PageArgs a{context, fresh, table, table_stride, free_pages, taken, taken_out, starts, lens, positions, slots, counts,
+               batch, tokens, width, n_free, shift};
+    auto st = static_cast<hipStream_t>(stream);
+    const bool one = tokens <= kInline;
+    pages_kernel<<<1, kThreads, 0, st>>>(a, one ? tokens : 0);
+    TW4_LAUNCH_CHECK("plan_pages: launch");
+    if (!one) {
+        rows_kernel<<<(tokens + 255) / 256, 256, 0, st>>>(a);
+        TW4_LAUNCH_CHECK("plan_pages: launch");
+    }
+    return TW4_OK;
+}
+
+extern "C" int tw4_release_pages(const int32_t* ended, int count, int32_t* table, int64_t table_stride, int width,
+                                 int32_t* lens, int batch, int32_t* free_pages, int n_free, int32_t* taken, int page_size,
+                                 void* stream) {
+    const int shift = page_shift(page_size);
+    TW4_REQUIRE(shift >= 0, TW4_EINVAL, "release_pages: page_size 16, 32, 64, 128 or 256 (%d)", page_size);
+    TW4_REQUIRE(count >= 0 && batch >= 1 && width >= 0 && n_free >= 0 && table_stride >= width, TW4_EINVAL,
+                "release_pages: bad sizes (%d of %d requests, width %d)", count, batch, width);
+    if (count == 0 || width == 0) return TW4_OK;
+    TW4_REQUIRE(ended && table && lens && taken && (free_pages || !n_free), TW4_EINVAL, "release_pages: null pointer");
+    release_kernel<<<1, kThreads, 0, static_cast<hipStream_t>(stream)>>>(ended, count, table, table_stride, width, lens, batch,
+                                                                         free_pages, n_free, taken, shift);
+    TW4_LAUNCH_CHECK("release_pages: launch");
+    return TW4_OK;
+}

@@ -1,0 +1,184 @@
+"""The paged KV cache of a decoder and its bookkeeping on the GPU (python/tandem/cache/): pages of a fixed number of tokens, a
+list of the free ones, a table of each request's pages, and the positions and slots of a step's tokens from the requests' lengths
+alone. Nothing is read back: a step, with its pages, can be captured in a HIP graph and replayed.
+
+    plan_pages         pages, positions and slots of one step (tw4_plan_pages)
+    release_pages      pages of ended requests back to the list (tw4_release_pages)
+    PagedKVCache       keys and values of every layer, the table and the lists
+    PagedBatch         one step over a cache, as tandem_amd.model's attention takes it
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import TYPE_CHECKING, NamedTuple, Sequence
+
+import torch
+
+from tandem_amd.layers import rotary, w4_hip
+from tandem_amd.layers.rotary import PAGE_SIZES, check_int32
+
+if TYPE_CHECKING:
+    from tandem_amd.model import DecoderConfig
+
+MAX_REQUESTS = 4096  # of one plan_pages call
+
+
+class PagePlan(NamedTuple):
+    """int32 tensors of plan_pages. counts: new tokens, pages given, pages the list did not have, tokens past num_tokens."""
+
+    query_start: torch.Tensor  # [B + 1]
+    seq_lens: torch.Tensor     # [B]
+    positions: torch.Tensor    # [num_tokens]
+    slots: torch.Tensor        # [num_tokens]
+    taken: torch.Tensor        # [1]
+    counts: torch.Tensor       # [4]
+
+
+def _check_table(who: str, page_table: torch.Tensor, free_pages: torch.Tensor, page_size: int) -> None:
+    if not (page_table.is_cuda and page_table.dim() == 2 and page_table.dtype == torch.int32) or (
+            page_table.shape[1] > 1 and page_table.stride(1) != 1) or (
+            page_table.shape[0] > 1 and page_table.stride(0) < page_table.shape[1]):
+        raise RuntimeError(f"{who}: page_table must be an int32 GPU tensor [requests, pages per request] of separate contiguous rows "
+                           f"(got {page_table.dtype} {tuple(page_table.shape)} on {page_table.device})")
+    if page_size not in PAGE_SIZES:
+        raise RuntimeError(f"{who}: a page size of {PAGE_SIZES} (got {page_size})")
+    check_int32(who, "free_pages", free_pages, (free_pages.numel(),), page_table)
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return max(t.stride(0), t.shape[1])
+
+
+def plan_pages(context_lens: torch.Tensor, query_lens: torch.Tensor, page_table: torch.Tensor, free_pages: torch.Tensor,
+               taken: torch.Tensor, page_size: int, num_tokens: int, *, seq_lens_out: torch.Tensor | None = None,
+               taken_out: torch.Tensor | None = None) -> PagePlan:
+    """Room in the cache for the new tokens of a step. Request i of B has context_lens[i] tokens in its pages page_table[i] and
+    brings query_lens[i] more (0: it sits this step out); free_pages [F] lists free pages, of which the first taken[0] are
+    in use. New pages are entered into page_table, in order of request; num_tokens rows get their positions and slots, those
+    behind the last request's position 0 and slot -1. Where the list has no page left, or a request outgrows its row of the
+    table, the entry and the slots there are -1.
+
+    int32 GPU tensors; lengths below zero count as zero, and the new tokens are fewer than 2^31 in all. seq_lens_out (context_lens
+    itself, to advance it) and taken_out (taken itself) are written instead of new tensors. Nothing is read back; the caller that
+    wants to know whether the pages sufficed reads counts[2]."""
+    who = "plan_pages"
+    _check_table(who, page_table, free_pages, page_size)
+    batch, width = page_table.shape
+    if not 1 <= batch <= MAX_REQUESTS:
+        raise RuntimeError(f"{who}: 1 to {MAX_REQUESTS} requests (got {batch})")
+    if not 0 <= num_tokens < 1 << 30:
+        raise RuntimeError(f"{who}: 0 <= num_tokens < 2^30 (got {num_tokens})")
+    dev = page_table.device
+    for name, t, shape in (("context_lens", context_lens, (batch,)), ("query_lens", query_lens, (batch,)), ("taken", taken, (1,)),
+                           ("seq_lens_out", seq_lens_out, (batch,)), ("taken_out", taken_out, (1,))):
+        if t is not None:
+            check_int32(who, name, t, shape, page_table)
+    # one allocation for what is new: each starts a 16-byte line
+    sizes = [batch + 1, 0 if seq_lens_out is not None else batch, num_tokens, num_tokens, 0 if taken_out is not None else 1, 4]
+    starts = [0]
+    for n in sizes:
+        starts.append(starts[-1] + (n + 3) // 4 * 4)
+    flat = torch.empty(starts[-1], dtype=torch.int32, device=dev)
+    query_start, lens, positions, slots, left, counts = (flat[s:s + n] for s, n in zip(starts, sizes))
+    plan = PagePlan(query_start, lens if seq_lens_out is None else seq_lens_out, positions, slots,
+                    left if taken_out is None else taken_out, counts)
+    index = page_table.get_device()
+    with w4_hip.on_device(index):
+        w4_hip.check(w4_hip.library().tw4_plan_pages(
+            context_lens.data_ptr(), query_lens.data_ptr(), page_table.data_ptr(), _row_stride(page_table), width,
+            free_pages.data_ptr(), free_pages.numel(), taken.data_ptr(), plan.taken.data_ptr(), page_size,
+            plan.query_start.data_ptr(), plan.seq_lens.data_ptr(), plan.positions.data_ptr(), plan.slots.data_ptr(),
+            plan.counts.data_ptr(), batch, num_tokens, w4_hip.raw_stream(index)))
+    return plan
+
+
+def release_pages(ended: torch.Tensor, context_lens: torch.Tensor, page_table: torch.Tensor, free_pages: torch.Tensor,
+                  taken: torch.Tensor, page_size: int) -> None:
+    """The pages of the requests ``ended`` (int32 [n], indices into page_table's rows; others are passed over) go back to the
+    list: taken[0] falls by their number and they are the next to be given. Their rows become -1 and their lengths 0, all in place."""
+    who = "release_pages"
+    _check_table(who, page_table, free_pages, page_size)
+    batch, width = page_table.shape
+    check_int32(who, "ended", ended, (ended.numel(),), page_table)
+    check_int32(who, "context_lens", context_lens, (batch,), page_table)
+    check_int32(who, "taken", taken, (1,), page_table)
+    if ended.numel() == 0 or batch == 0:
+        return
+    index = page_table.get_device()
+    with w4_hip.on_device(index):
+        w4_hip.check(w4_hip.library().tw4_release_pages(
+            ended.data_ptr(), ended.numel(), page_table.data_ptr(), _row_stride(page_table), width, context_lens.data_ptr(), batch,
+            free_pages.data_ptr(), free_pages.numel(), taken.data_ptr(), page_size, w4_hip.raw_stream(index)))
+
+
+@dataclass(frozen=True)
+class PagedBatch:
+    """One step over a PagedKVCache: which tokens, where they go, and what they may see."""
+
+    cache: "PagedKVCache"
+    page_table: torch.Tensor
+    seq_lens: torch.Tensor
+    query_start: torch.Tensor
+    positions: torch.Tensor
+    slots: torch.Tensor
+    counts: torch.Tensor
+    max_query_len: int
+    max_seq_len: int
+
+
+class PagedKVCache:
+    """Keys and values [layers, pages, KV heads, page size, head_dim] for up to max_requests requests of up to max_seq_len tokens.
+    A request has a lane (a row of the table) from its first token until release. Lanes 0 .. B - 1 take part in a step of B;
+    those with no new token sit it out. One stream at a time works on a cache, as on any tensor it writes."""
+
+    def __init__(self, layers: int, kv_heads: int, head_dim: int, num_pages: int, max_requests: int, max_seq_len: int,
+                 page_size: int = 16, rope_theta: float = 1e6, dtype: torch.dtype = torch.float16,
+                 device: torch.device | str = "cuda") -> None:
+        if page_size not in PAGE_SIZES or head_dim not in (64, 128) or dtype not in rotary.TYPES:
+            raise ValueError(f"PagedKVCache: page size of {PAGE_SIZES}, head_dim 64 or 128, float16 or bfloat16 (got {page_size}, "
+                             f"{head_dim}, {dtype})")
+        if min(layers, kv_heads, num_pages, max_seq_len) < 1 or not 1 <= max_requests <= MAX_REQUESTS:
+            raise ValueError(f"PagedKVCache: at least one layer, head, page and token, 1 to {MAX_REQUESTS} requests (got {layers}, "
+                             f"{kv_heads}, {num_pages}, {max_seq_len}, {max_requests})")
+        if num_pages * page_size >= 1 << 31:
+            raise ValueError(f"PagedKVCache: fewer than 2^31 slots (got {num_pages} pages of {page_size})")
+        self.page_size, self.max_seq_len, self.max_requests = page_size, max_seq_len, max_requests
+        width = -(-max_seq_len // page_size)
+        shape = (layers, num_pages, kv_heads, page_size, head_dim)
+        self.keys, self.values = (torch.empty(shape, dtype=dtype, device=device) for _ in range(2))
+        dev = self.keys.device
+        self.page_table = torch.full((max_requests, width), -1, dtype=torch.int32, device=dev)
+        self.context_lens = torch.zeros(max_requests, dtype=torch.int32, device=dev)
+        self.free_pages = torch.arange(num_pages, dtype=torch.int32, device=dev)
+        self.taken = torch.zeros(1, dtype=torch.int32, device=dev)
+        self.rotary = rotary.rotary_table(max_seq_len, head_dim, rope_theta, dev)
+
+    @classmethod
+    def for_model(cls, config: "DecoderConfig", num_pages: int, max_requests: int, max_seq_len: int, page_size: int = 16,
+                  device: torch.device | str = "cuda") -> "PagedKVCache":
+        """A cache of float16 for a DecoderModel of this configuration."""
+        if config.rope_type != "default":
+            raise NotImplementedError(f"rope_scaling of type {config.rope_type!r}: only plain rotary positions are supported")
+        return cls(config.num_layers, config.num_kv_heads, config.head_dim, num_pages, max_requests, max_seq_len, page_size,
+                   config.rope_theta, torch.float16, device)
+
+    def plan(self, query_lens: torch.Tensor, num_tokens: int, max_query_len: int | None = None,
+             max_seq_len: int | None = None) -> PagedBatch:
+        """Takes pages for query_lens[i] new tokens of lane i (int32 [B], B <= max_requests) and advances the lanes' lengths; the
+        step's tokens are num_tokens rows, lane by lane (rows behind the last are computed for nothing). max_query_len,
+        max_seq_len: bounds the host knows, for the division of the work."""
+        if query_lens.dim() != 1 or not 1 <= query_lens.numel() <= self.max_requests:
+            raise RuntimeError(f"PagedKVCache.plan: query_lens [1 .. {self.max_requests}] expected (got {tuple(query_lens.shape)})")
+        b = query_lens.numel()
+        lens = self.context_lens[:b]
+        plan = plan_pages(lens, query_lens, self.page_table[:b], self.free_pages, self.taken, self.page_size, num_tokens,
+                          seq_lens_out=lens, taken_out=self.taken)
+        return PagedBatch(self, self.page_table[:b], lens, plan.query_start, plan.positions, plan.slots, plan.counts,
+                          num_tokens if max_query_len is None else max_query_len,
+                          self.max_seq_len if max_seq_len is None else max_seq_len)
+
+    def release(self, lanes: Sequence[int] | torch.Tensor) -> None:
+        """The lanes' requests have ended: their pages are free again."""
+        ended = torch.as_tensor(lanes, dtype=torch.int32).to(self.page_table.device)
+        release_pages(ended, self.context_lens, self.page_table, self.free_pages, self.taken, self.page_size)
