@@ -9,19 +9,23 @@ token ids are copied into the static input buffer (padding rows take token 0 and
 never returned); then the bucket's graph replays and the first b rows of its output are returned.
 
 Every W4Linear picks its kernel from the bucket's M at capture time, so each bucket replays the
-kernels its table names for that batch size. The KV-cache plumbing of the reference runner (paged
-layout, FlashInfer wrappers, the KV-split variants) belongs to the attention path, which this build
-leaves out (see tandem_amd.model).
+kernels its table names for that batch size.
+
+With a cache (tandem_amd.kv_cache.PagedKVCache) the graphs decode: a replay takes pages for each lane's token, writes its keys and
+values, attends over the lane's context and advances its length, all on the GPU (the reference plans on the host and keeps
+KV-split variants of its graphs, python/tandem/executor/cuda_graph.py; here the split follows the lengths inside the kernel).
+Without one, ``model(input_ids)`` runs on its one-token context.
 """
 
 from __future__ import annotations
 
 import logging
-from typing import Callable, Sequence
+from typing import Callable, Optional, Sequence
 
 import torch
 from torch import nn
 
+from tandem_amd.kv_cache import PagedKVCache
 from tandem_amd.layers import w4_hip
 
 logger = logging.getLogger(__name__)
@@ -38,22 +42,32 @@ def bucket_sizes(max_bs: int) -> list[int]:
 
 
 class DecodeGraphRunner:
-    """Bucketed HIP graphs of ``model(input_ids)`` (and ``model.compute_logits`` when ``logits``)."""
+    """Bucketed HIP graphs of ``model(input_ids)`` (and ``model.compute_logits`` when ``logits``), or of a decode step over
+    ``cache``."""
 
-    def __init__(self, model: nn.Module, max_bs: int, device: torch.device, logits: bool = True) -> None:
+    def __init__(self, model: nn.Module, max_bs: int, device: torch.device, logits: bool = True,
+                 cache: Optional[PagedKVCache] = None) -> None:
+        if cache is not None and max_bs > cache.max_requests:
+            raise ValueError(f"max_bs {max_bs} is more than the cache's {cache.max_requests} lanes")
         self.model = model
+        self.cache = cache
         self.device = device
         self.logits = logits
         self.sizes = bucket_sizes(max_bs)
         self.max_bs = self.sizes[-1]
         self.input_ids = torch.zeros(self.max_bs, dtype=torch.long, device=device)
+        # no lane has a token while graphs are captured: the cache stays as it is
+        self.query_lens = torch.zeros(self.max_bs, dtype=torch.int32, device=device)
         self.graphs: dict[int, torch.cuda.CUDAGraph] = {}
         self.outputs: dict[int, torch.Tensor] = {}
         self._capture_all()
 
     def _fn(self, bs: int) -> Callable[[], torch.Tensor]:
         def run() -> torch.Tensor:
-            hidden = self.model(self.input_ids[:bs])
+            if self.cache is None:
+                hidden = self.model(self.input_ids[:bs])
+            else:
+                hidden = self.model(self.input_ids[:bs], self.cache.plan(self.query_lens[:bs], bs, max_query_len=1))
             return self.model.compute_logits(hidden) if self.logits else hidden
         return run
 
@@ -85,12 +99,20 @@ class DecodeGraphRunner:
     @torch.inference_mode()
     def run(self, input_ids: Sequence[int] | torch.Tensor) -> torch.Tensor:
         """Token ids of b <= max_bs sequences -> the first b rows of the bucket's output (a view of a
-        static buffer, overwritten by the next replay of that bucket)."""
+        static buffer, overwritten by the next replay of that bucket). With a cache sequence i is lane i; a lane with an id below
+        zero sits the step out, and the rows are those of the others in order."""
         ids = torch.as_tensor(input_ids, dtype=torch.long)
         b = int(ids.numel())
         if not self.can_run(b):
             raise ValueError(f"decode batch {b} outside 1..{self.max_bs}")
         bs = self.bucket(b)
+        if self.cache is not None:
+            ids = ids.reshape(-1).cpu()
+            lens = torch.zeros(bs, dtype=torch.int32)
+            lens[:b] = ids >= 0
+            self.query_lens[:bs].copy_(lens)
+            ids = ids[ids >= 0]
+            b = int(ids.numel())
         padded = torch.zeros(bs, dtype=torch.long)
         padded[:b] = ids.reshape(-1).cpu()
         self.input_ids[:bs].copy_(padded.to(self.device, non_blocking=False))

@@ -6,15 +6,22 @@ step runs besides attention:
     DecoderConfig     the fields of config.json the step needs     python/tandem/model_config.py
     GatedMLP          gate_up (SwiGLU epilogue) + down             python/tandem/layers/mlp.py:16-45
     Attention         qkv_proj + o_proj around the attention       python/tandem/layers/attention.py
+                      (over a paged cache: head norms, rotary positions, attention of the new tokens)
     DecoderLayer      add+norm, attention, add+norm, MLP with the  python/tandem/models/llama_family.py:35-67
                       residual stream carried between layers
     DecoderModel      embedding, layers, final add+norm, lm_head   python/tandem/models/llama_family.py:70-116
 
-Attention over a KV cache (paged cache, FlashInfer, RoPE, QK-norm) is another path of tandem and is
-not part of this build. ``Attention.attend`` computes attention over a one-token context, the
-first decode position: softmax over a single key is 1, so each query head's output is the value row
-of its KV head (grouped-query attention). That is exact for that position and costs one small copy
-kernel, so a captured step has the real launch sequence of a decoder layer around the projections.
+A model is called with token ids alone, or with a step over a paged cache (tandem_amd.kv_cache.PagedBatch):
+
+    cache = PagedKVCache.for_model(cfg, num_pages=4096, max_requests=32, max_seq_len=8192)
+    batch = cache.plan(query_lens, num_tokens)          # lanes' new tokens: prompts, chunks, single tokens, any mix
+    hidden = model(input_ids, batch)                    # [num_tokens] ids, lane by lane
+    logits = model.compute_logits(hidden[batch.query_start[1:].long() - 1])   # each lane's last token
+
+With it, each layer normalises (Qwen3) and rotates queries and keys into the cache in one kernel and attends over the lane's
+pages (python/tandem/layers/attention.py, triton_ops.py, flashinfer_attention.py). Without it, ``Attention.attend`` computes
+attention over a one-token context, the first decode position: softmax over a single key is 1, so each query head's output is the
+value row of its KV head (grouped-query attention), one small copy kernel. At position 0 that is what the cached form gives.
 
 Projections are W4Linear (AutoAWQ checkpoints) or nn.Linear (fp16 checkpoints); ``prepare`` moves
 the model to the GPU, repacks the W4 layers and routes the fp16 projections and the logits head
@@ -32,8 +39,10 @@ from typing import Any, Optional
 import torch
 from torch import nn
 
-from tandem_amd.layers import gemv16, norm, w4_hip
+from tandem_amd.kv_cache import PagedBatch
+from tandem_amd.layers import gemv16, norm, rotary, w4_hip
 from tandem_amd.layers.linear import finalize_quantized, make_linear
+from tandem_amd.layers.paged_attention import paged_attention
 
 
 @dataclass(frozen=True)
@@ -47,21 +56,29 @@ class DecoderConfig:
     vocab_size: int
     rms_norm_eps: float = 1e-6
     tie_word_embeddings: bool = False
+    rope_theta: float = 1e6
+    qk_norm: bool = False
+    rope_type: str = "default"
 
     @classmethod
     def from_hf(cls, d: dict[str, Any]) -> "DecoderConfig":
-        """The fields of a Hugging Face config.json (python/tandem/model_config.py)."""
+        """The fields of a Hugging Face config.json (python/tandem/model_config.py). Without a model_type: Qwen3, whose
+        queries and keys are normalised head by head."""
         heads = int(d["num_attention_heads"])
+        qwen3 = d.get("model_type", "qwen3") == "qwen3"
+        rope = d.get("rope_parameters") or d.get("rope_scaling") or {}
         return cls(hidden_size=int(d["hidden_size"]), intermediate_size=int(d["intermediate_size"]),
                    num_heads=heads, num_kv_heads=int(d.get("num_key_value_heads", heads)),
                    head_dim=int(d.get("head_dim") or d["hidden_size"] // heads),
                    num_layers=int(d["num_hidden_layers"]), vocab_size=int(d["vocab_size"]),
                    rms_norm_eps=float(d.get("rms_norm_eps", 1e-6)),
-                   tie_word_embeddings=bool(d.get("tie_word_embeddings", False)))
+                   tie_word_embeddings=bool(d.get("tie_word_embeddings", False)),
+                   rope_theta=float(d.get("rope_theta") or rope.get("rope_theta") or (1e6 if qwen3 else 1e4)), qk_norm=qwen3,
+                   rope_type=str(rope.get("rope_type") or rope.get("type") or "default"))
 
 
-QWEN3_8B = DecoderConfig(4096, 12288, 32, 8, 128, 36, 151936)
-QWEN3_1_7B = DecoderConfig(2048, 6144, 16, 8, 128, 28, 151936, tie_word_embeddings=True)
+QWEN3_8B = DecoderConfig(4096, 12288, 32, 8, 128, 36, 151936, qk_norm=True)
+QWEN3_1_7B = DecoderConfig(2048, 6144, 16, 8, 128, 28, 151936, tie_word_embeddings=True, qk_norm=True)
 
 
 def silu_and_mul(y: torch.Tensor) -> torch.Tensor:
@@ -90,8 +107,8 @@ class GatedMLP(nn.Module):
 
 
 class Attention(nn.Module):
-    """The projections of grouped-query attention; ``attend`` is the one-token-context attention
-    described in the module docstring."""
+    """The projections of grouped-query attention and, between them, attention over a paged cache or (``attend`` without a batch)
+    over a one-token context, as the module docstring describes."""
 
     def __init__(self, cfg: DecoderConfig, quant: Optional[Any] = None) -> None:
         super().__init__()
@@ -100,6 +117,10 @@ class Attention(nn.Module):
         self.kv_size = cfg.num_kv_heads * cfg.head_dim
         self.qkv_proj = make_linear(cfg.hidden_size, self.q_size + 2 * self.kv_size, False, quant)
         self.o_proj = make_linear(self.q_size, cfg.hidden_size, False, quant)
+        self.eps = cfg.rms_norm_eps
+        # weights of the head norms: the norms themselves run inside norm_rope_cache
+        self.q_norm = norm.RMSNorm(cfg.head_dim, cfg.rms_norm_eps) if cfg.qk_norm else None
+        self.k_norm = norm.RMSNorm(cfg.head_dim, cfg.rms_norm_eps) if cfg.qk_norm else None
 
     def _hip_attend(self, qkv: torch.Tensor) -> bool:
         """Plain contiguous 16-byte aligned fp16 GPU rows [q | k | v] that no gradient, transform, mode or compiler follows, whole
@@ -112,10 +133,18 @@ class Attention(nn.Module):
                 and self.num_heads % self.num_kv_heads == 0 and qkv.data_ptr() % 16 == 0
                 and 8 * (1 << 31) > qkv.numel())
 
-    def attend(self, qkv: torch.Tensor) -> torch.Tensor:
-        """[M, q | k | v] -> [M, num_heads * head_dim]: query head h takes the value row of KV head
-        h // (num_heads / num_kv_heads)."""
+    def attend(self, qkv: torch.Tensor, batch: Optional[PagedBatch] = None, layer: int = 0) -> torch.Tensor:
+        """[M, q | k | v] -> [M, num_heads * head_dim]: with a batch, attention of its tokens over the cache's ``layer``, which
+        takes their keys and values; without, query head h takes the value row of KV head h // (num_heads / num_kv_heads)."""
         m = qkv.shape[0]
+        if batch is not None:
+            cache = batch.cache
+            keys, values = cache.keys[layer], cache.values[layer]
+            q = rotary.norm_rope_cache(qkv, batch.positions, cache.rotary, self.num_heads, self.num_kv_heads, keys, values,
+                                       batch.slots, None if self.q_norm is None else self.q_norm.weight,
+                                       None if self.k_norm is None else self.k_norm.weight, self.eps)
+            return paged_attention(q, keys, values, batch.page_table, batch.seq_lens, batch.query_start,
+                                   max_query_len=batch.max_query_len, max_seq_len=batch.max_seq_len).view(m, self.q_size)
         if self._hip_attend(qkv):
             y = torch.empty((m, self.q_size), dtype=torch.float16, device=qkv.device)
             with w4_hip.on_device(qkv.get_device()):
@@ -127,8 +156,9 @@ class Attention(nn.Module):
         group = self.num_heads // self.num_kv_heads
         return v.expand(m, self.num_kv_heads, group, self.head_dim).reshape(m, self.q_size).contiguous()
 
-    def forward(self, hidden: torch.Tensor) -> torch.Tensor:
-        return self.o_proj(self.attend(self.qkv_proj(hidden)))
+    def forward(self, hidden: torch.Tensor, batch: Optional[PagedBatch] = None, layer: int = 0) -> torch.Tensor:
+        step = () if batch is None else (batch, layer)
+        return self.o_proj(self.attend(self.qkv_proj(hidden), *step))
 
 
 class DecoderLayer(nn.Module):
@@ -139,21 +169,23 @@ class DecoderLayer(nn.Module):
         self.input_layernorm = norm.RMSNorm(cfg.hidden_size, cfg.rms_norm_eps)
         self.post_attention_layernorm = norm.RMSNorm(cfg.hidden_size, cfg.rms_norm_eps)
 
-    def forward(self, hidden: torch.Tensor, residual: Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor]:
+    def forward(self, hidden: torch.Tensor, residual: Optional[torch.Tensor], batch: Optional[PagedBatch] = None,
+                layer: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
         """The residual stream is carried between layers, so every "add residual, then normalise"
         pair is one kernel (python/tandem/models/llama_family.py:47-67)."""
+        step = () if batch is None else (batch, layer)
         n1, n2 = self.input_layernorm, self.post_attention_layernorm
         attn, mlp = self.self_attn, self.mlp
         if hasattr(attn.qkv_proj, "forward_norm"):  # W4: the norm goes into the projection's prologue
             qkv, residual = attn.qkv_proj.forward_norm(hidden, residual, n1.weight, n1.eps)
-            hidden = attn.o_proj(attn.attend(qkv))
+            hidden = attn.o_proj(attn.attend(qkv, *step))
         else:
             if residual is None:
                 residual = hidden
                 hidden = norm.rms_norm(hidden, n1.weight, n1.eps)
             else:
                 hidden, residual = norm.fused_add_rms_norm(hidden, residual, n1.weight, n1.eps)
-            hidden = attn(hidden)
+            hidden = attn(hidden, *step)
         if hasattr(mlp.gate_up_proj, "forward_norm"):
             act, residual = mlp.gate_up_proj.forward_norm(hidden, residual, n2.weight, n2.eps)
             return mlp.down_proj(act if mlp.fused_act else silu_and_mul(act)), residual
@@ -176,13 +208,14 @@ class DecoderModel(nn.Module):
         self.lm_head = None if cfg.tie_word_embeddings else nn.Linear(cfg.hidden_size, cfg.vocab_size, bias=False)
         self.gemv_table: dict = {}
 
-    def forward(self, input_ids: torch.Tensor) -> torch.Tensor:
-        """input_ids [M] -> final hidden states [M, hidden] (python/tandem/models/llama_family.py:90-109)."""
+    def forward(self, input_ids: torch.Tensor, batch: Optional[PagedBatch] = None) -> torch.Tensor:
+        """input_ids [M] -> final hidden states [M, hidden] (python/tandem/models/llama_family.py:90-109). With a batch the ids are
+        its tokens, lane by lane; rows behind its last token hold no result."""
         emb = self.model.embed_tokens
         hidden = emb.weight[input_ids]
         residual = None
-        for layer in self.model.layers:
-            hidden, residual = layer(hidden, residual)
+        for i, layer in enumerate(self.model.layers):
+            hidden, residual = layer(hidden, residual, *(() if batch is None else (batch, i)))
         n = self.model.norm
         hidden, _ = norm.fused_add_rms_norm(hidden, residual, n.weight, n.eps)
         return hidden
@@ -210,9 +243,11 @@ def prepare(model: DecoderModel, device: torch.device, device_name: Optional[str
 def init_random(model: DecoderModel, seed: int = 0) -> DecoderModel:
     """Synthetic weights of the architecture, generated on the model's device: AutoAWQ tensors with
     uniform int4 q and z and fp16 scales U[0.001, 0.02] (the reference tests' recipe), fp16
-    projections N(0, 0.02), embeddings N(0, 1), norm weights 1 + U(-0.1, 0.1)."""
+    projections N(0, 0.02), embeddings N(0, 1), norm weights 1 + U(-0.1, 0.1). Head norms are drawn from a generator of their
+    own: the other weights of a seed are the same with and without them."""
     dev = next(model.parameters()).device
     g = torch.Generator(device=dev).manual_seed(seed)
+    heads = torch.Generator(device=dev).manual_seed(seed + 1)
     for mod in model.modules():
         if getattr(mod, "awq_layout", False):
             for t in (mod.qweight, mod.qzeros):
@@ -222,7 +257,8 @@ def init_random(model: DecoderModel, seed: int = 0) -> DecoderModel:
         if name.endswith("embed_tokens.weight"):
             p.copy_(torch.randn(p.shape, device=dev, generator=g))
         elif "norm" in name:
-            p.copy_(1.0 + (torch.rand(p.shape, device=dev, generator=g) - 0.5) * 0.2)
+            own = heads if name.endswith(("q_norm.weight", "k_norm.weight")) else g
+            p.copy_(1.0 + (torch.rand(p.shape, device=dev, generator=own) - 0.5) * 0.2)
         else:
             p.copy_(torch.randn(p.shape, device=dev, generator=g) * 0.02)
     return model
