@@ -19,6 +19,7 @@
 // wavefront's own LDS, read back transposed. With few rows in flight the keys are split over `splits` workgroups; the last to arrive
 // joins their results in order.
 #include <algorithm>
+#include <type_traits>
 
 #include "tw4_attn.h"
 
@@ -36,10 +37,11 @@ struct AttnArgs {
     int32_t* locks;
     int64_t q_token, q_head, page_stride, head_stride, token_stride, table_stride;
     float scale;  // times log2(e)
-    int tokens, batch, heads, kv_heads, group, num_pages, width, shift, splits, slots;
+    int tokens, batch, heads, kv_heads, group, num_pages, width, shift, splits, part_rows;
 };
 
 constexpr int kTileFloats = 2;  // per row beside its D sums: maximum and sum
+constexpr int kMinKeys = 128, kPerCu = 8;
 
 // A tile of rows: its request, first row, and the keys it can see.
 struct Tile {
@@ -112,7 +114,7 @@ __device__ __forceinline__ bool odd16(uint32_t v, uint32_t exponent) {  // eithe
 constexpr float kNone = -__builtin_inff();
 
 template <typename T, int D, int MT>
-__global__ void __launch_bounds__(256) rows_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(256, 2) rows_kernel(AttnArgs a) {
     constexpr int B = 16 * MT, KS = D / 32, DT = D / 16, C = D / 8, VJ = C / 2;  // VJ: 1 KB loads of 32 keys
     constexpr uint32_t kExponent = __is_same(T, h1) ? 0x7C00u : 0x7F80u;
     static_assert(32 * D * 2 * 4 >= 4 * 16 * D * 4, "the join of 16 rows uses the V tiles' LDS");
@@ -146,7 +148,7 @@ __global__ void __launch_bounds__(256) rows_kernel(AttnArgs a) {
     const int end = static_cast<int>(min(static_cast<int64_t>(high) + 1, static_cast<int64_t>(a.width) << a.shift));
     int begin = 0, stop = max(end, 0), parts = 1;
     if (a.splits > 1 && end > 0) {
-        const int share = max((end + a.splits - 1) / a.splits, 128);
+        const int share = max((end + a.splits - 1) / a.splits, kMinKeys);
         const int whole = (share + 127) & ~127;
         parts = (end + whole - 1) / whole;
         if (split >= parts) return;
@@ -166,51 +168,80 @@ __global__ void __launch_bounds__(256) rows_kernel(AttnArgs a) {
     }
     u4* vt = lds + wave * 32 * C;
     const int32_t* table = a.table + t.request * a.table_stride;
-    const uint16_t* kh = a.k + head * a.head_stride;
-    const uint16_t* vh = a.v + head * a.head_stride;
+    const char* kh = reinterpret_cast<const char*>(a.k + head * a.head_stride);
+    const char* vh = reinterpret_cast<const char*>(a.v + head * a.head_stride);
     const int final16 = (stop - 1) & ~15;  // the last 16 keys that are there
+    const uint32_t token_bytes = static_cast<uint32_t>(a.token_stride) * 2;
 
-    for (int base = begin + 32 * wave; base < stop; base += 128) {
-        // the pages of the block's two halves; a page the table does not have is page 0, read and left out
-        int64_t at[2];
-        int absent = 0, first[2], lastrow[2];
+    // A block of 32 keys is two halves of 16, each in one page. Table entries are fetched a block before the keys they lead to,
+    // K a block before its product, V a block before it goes to LDS: each load has a block's arithmetic to arrive in.
+    u4 kf[2][KS], vf[VJ];
+    auto pages = [&](int base, int (&page)[2]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) page[h] = table[min(base + 16 * h, final16) >> a.shift];
+    };
+    auto there = [&](int page) { return static_cast<uint32_t>(page) < static_cast<uint32_t>(a.num_pages); };
+    // byte offset of half h's first key; a page the table does not have is page 0, read and left out
+    auto offset = [&](int base, int h, int page) {
+        const int first = min(base + 16 * h, final16);
+        return ((there(page) ? page : 0) * a.page_stride + (first & ((1 << a.shift) - 1)) * a.token_stride) * 2;
+    };
+    auto last_row = [&](int base, int h) { return min(stop - 1 - min(base + 16 * h, final16), 15); };
+    auto load_k = [&](int base, const int (&page)[2]) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            first[h] = min(base + 16 * h, final16);
-            const int page = table[first[h] >> a.shift];
-            const bool there = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.num_pages);
-            absent |= there ? 0 : 1 << h;
-            at[h] = (there ? page : 0) * a.page_stride + (first[h] & ((1 << a.shift) - 1)) * a.token_stride;
-            lastrow[h] = min(stop - 1 - first[h], 15);
+            const char* src = kh + offset(base, h, page[h]);
+            const uint32_t lane_off = min(c16, last_row(base, h)) * token_bytes + 16 * g4;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) kf[h][s] = *reinterpret_cast<const u4*>(src + (lane_off + 64 * s));
         }
-        u4 kf[2][KS], vf[VJ];
+    };
+    auto load_v = [&](int base, const int (&page)[2]) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const uint16_t* src = kh + at[h] + min(c16, lastrow[h]) * a.token_stride + 8 * g4;
+            const char* src = vh + offset(base, h, page[h]);
+            const int last = last_row(base, h);
 #pragma unroll
-            for (int s = 0; s < KS; ++s) kf[h][s] = *reinterpret_cast<const u4*>(src + 32 * s);
+            for (int j = 0; j < VJ / 2; ++j)  // chunk lane % C of row lane / C + j (64 / C)
+                vf[h * (VJ / 2) + j] = *reinterpret_cast<const u4*>(
+                    src + (min(lane / C + j * (64 / C), last) * token_bytes + 16 * (lane % C)));
         }
+    };
+    auto block = [&](int base, const int (&now_page)[2], int (&next_page)[2], auto more) {
+        constexpr bool kMore = decltype(more)::value;
+        const int absent = (there(now_page[0]) ? 0 : 1) | (there(now_page[1]) ? 0 : 2);
+        const bool masked = absent || base + 32 > min(low + 1, stop);
+        f4 s[MT][2];
 #pragma unroll
-        for (int j = 0; j < VJ; ++j) {  // chunk lane % C of row lane / C + j (64 / C)
-            const int row = lane / C + j * (64 / C), h = j * 2 / VJ;
-            vf[j] = *reinterpret_cast<const u4*>(vh + at[h] + min(row & 15, lastrow[h]) * a.token_stride + 8 * (lane % C));
+        for (int m = 0; m < MT; ++m) s[m][0] = s[m][1] = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < KS; ++i)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                s[m][0] = mma16<T>(kf[0][i], q[m][i], s[m][0]);
+                s[m][1] = mma16<T>(kf[1][i], q[m][i], s[m][1]);
+            }
+        if constexpr (kMore) load_k(base + 128, next_page);
+        // A probability of zero does not take an infinity or NaN away: where some row does not see a key, such values are left out
+        // of the product and added to the rows that see them.
+        bool odd = false;
+        if (masked) {
+#pragma unroll
+            for (int j = 0; j < VJ; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) odd |= odd16(vf[j][i], kExponent);
+            odd = __ballot(odd) != 0;
         }
 #pragma unroll
         for (int j = 0; j < VJ; ++j) vt[v_chunk<D>(lane / C + j * (64 / C), lane % C)] = vf[j];
+        if constexpr (kMore) load_v(base + 128, next_page);
 
-        const bool masked = absent || base + 32 > min(low + 1, stop);
         u4 p[MT];
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-            f4 s[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
-#pragma unroll
-            for (int i = 0; i < KS; ++i) {
-                s[0] = mma16<T>(kf[0][i], q[m][i], s[0]);
-                s[1] = mma16<T>(kf[1][i], q[m][i], s[1]);
-            }
             float x[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = s[i >> 2][i & 3] * a.scale;
+            for (int i = 0; i < 8; ++i) x[i] = s[m][i >> 2][i & 3] * a.scale;
             if (masked) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -236,46 +267,61 @@ __global__ void __launch_bounds__(256) rows_kernel(AttnArgs a) {
             for (int d = 0; d < DT; ++d) o[m][d] *= keep;
         }
         // V back, transposed: 4 rows x 16 columns for each 16 lanes
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
         __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+        if (odd) {
+#pragma unroll 1
+            for (int key = 0; key < 32; ++key)
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    if (base + key > min(limit[m], stop - 1) || (absent >> (key >> 4) & 1)) continue;
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) {
+                        const u2 four = *reinterpret_cast<const u2*>(reinterpret_cast<const char*>(vt) +
+                                                                     v_chunk<D>(key, 2 * d + (g4 >> 1)) * 16 + (g4 & 1) * 8);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint16_t bits = static_cast<uint16_t>(four[i >> 1] >> (16 * (i & 1)));
+                            if ((bits & kExponent) == kExponent) o[m][d][i] += static_cast<float>(bitcast<T>(bits));
+                        }
+                        __builtin_amdgcn_sched_barrier(0);  // one at a time: the rare path is not to take registers
+                    }
+                }
+        }
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
             const int r = 4 * g4 + (c16 >> 2), c = 2 * d + ((c16 & 3) >> 1), half = (c16 & 1) * 8;
             const u2 lo = read_tr(vt, v_chunk<D>(r, c) * 16 + half), hi = read_tr(vt, v_chunk<D>(r + 16, c) * 16 + half);
             u4 w = u4{lo.x, lo.y, hi.x, hi.y};
-            if (masked) {
-                // A probability of zero does not take an infinity or NaN away: where some row does not see a key, such values
-                // are taken out of the product and added to the rows that see them.
-                bool odd = false;
+            if (odd) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) odd |= odd16(w[i], kExponent);
-                if (__ballot(odd)) {
-#pragma unroll
-                    for (int m = 0; m < MT; ++m)
-#pragma unroll 1
-                        for (int key = 0; key < 32; ++key) {
-                            if (base + key > min(limit[m], stop - 1) || (absent >> (key >> 4) & 1)) continue;
-                            const uint16_t* row = reinterpret_cast<const uint16_t*>(vt);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const int col = 16 * d + 4 * g4 + i;
-                                const uint16_t bits = row[v_chunk<D>(key, col >> 3) * 8 + (col & 7)];
-                                if ((bits & kExponent) == kExponent) o[m][d][i] += static_cast<float>(bitcast<T>(bits));
-                            }
-                        }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if ((w[i] & kExponent) == kExponent) w[i] &= 0xFFFF0000u;
-                        if (((w[i] >> 16) & kExponent) == kExponent) w[i] &= 0xFFFFu;
-                    }
+                for (int i = 0; i < 4; ++i) {
+                    if ((w[i] & kExponent) == kExponent) w[i] &= 0xFFFF0000u;
+                    if (((w[i] >> 16) & kExponent) == kExponent) w[i] &= 0xFFFFu;
                 }
             }
 #pragma unroll
             for (int m = 0; m < MT; ++m) o[m][d] = mma16<T>(w, p[m], o[m][d]);
         }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
         __builtin_amdgcn_wave_barrier();
+    };
+    int base = begin + 32 * wave;
+    if (base < stop) {
+        int now_page[2], next_page[2];
+        pages(base, now_page);
+        load_k(base, now_page);
+        load_v(base, now_page);
+        pages(min(base + 128, final16), next_page);
+        for (; base + 128 < stop; base += 128) {
+            int after[2];
+            pages(min(base + 256, final16), after);
+            block(base, now_page, next_page, std::true_type());
+#pragma unroll
+            for (int h = 0; h < 2; ++h) now_page[h] = next_page[h], next_page[h] = after[h];
+        }
+        block(base, now_page, next_page, std::false_type());
     }
 
     // the four wavefronts' results become one, 16 rows at a time through LDS
@@ -314,16 +360,18 @@ __global__ void __launch_bounds__(256) rows_kernel(AttnArgs a) {
         }
     }
     if (parts > 1) {
-        // [unit][split][row][D + 2]: the sums, then maximum and sum
+        // [unit][split][row][D + 2]: the sums, then maximum and sum; rows that are there only
+        const int64_t mine = (static_cast<int64_t>(unit) * a.splits + split) * a.part_rows;
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-            const int to = static_cast<int>(((static_cast<int64_t>(unit) * a.splits + split) * B + 16 * m + row) * kRowFloats * 4);
+            if (16 * m + row >= t.rows) continue;
+            const int to = static_cast<int>((mine + 16 * m + row) * kRowFloats * 4);
 #pragma unroll
             for (int i = 0; i < PER; i += 2)
-                __builtin_amdgcn_raw_buffer_store_b64(u2{__float_as_uint(res[m][i]), __float_as_uint(res[m][i + 1])}, rs, to,
-                                                      (col + i) * 4, kCoherentAux);
+                __builtin_amdgcn_raw_buffer_store_b64(u2{__float_as_uint(res[m][i]), __float_as_uint(res[m][i + 1])}, rs,
+                                                      to + (col + i) * 4, 0, kCoherentAux);
             if (col == 0)
-                __builtin_amdgcn_raw_buffer_store_b64(u2{__float_as_uint(rtop[m]), __float_as_uint(rsum[m])}, rs, to, D * 4,
+                __builtin_amdgcn_raw_buffer_store_b64(u2{__float_as_uint(rtop[m]), __float_as_uint(rsum[m])}, rs, to + D * 4, 0,
                                                       kCoherentAux);
         }
         __builtin_amdgcn_s_waitcnt(0);
@@ -334,22 +382,41 @@ __global__ void __launch_bounds__(256) rows_kernel(AttnArgs a) {
         if (!last_flag) return;
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
+            if (16 * m + row >= t.rows) continue;
             rtop[m] = kNone, rsum[m] = 0.0f;
 #pragma unroll
             for (int i = 0; i < PER; ++i) res[m][i] = 0.0f;
-            for (int s = 0; s < parts; ++s) {
-                const int from =
-                    static_cast<int>(((static_cast<int64_t>(unit) * a.splits + s) * B + 16 * m + row) * kRowFloats * 4);
-                const u2 ms = bitcast<u2>(__builtin_amdgcn_raw_buffer_load_b64(rs, from, D * 4, kCoherentAux));
-                const float mt = __uint_as_float(ms.x), now = fmaxf(rtop[m], mt), zero = now == kNone ? 0.0f : now;
-                const float keep = __builtin_amdgcn_exp2f(rtop[m] - zero), f = __builtin_amdgcn_exp2f(mt - zero);
-                rtop[m] = now;
-                rsum[m] = rsum[m] * keep + f * __uint_as_float(ms.y);
+            constexpr int VB = 8;  // parts in flight
+            for (int s0 = 0; s0 < parts; s0 += VB) {
+                u2 ms[VB], x[VB][PER / 2];
 #pragma unroll
-                for (int i = 0; i < PER; i += 2) {
-                    const u2 x = bitcast<u2>(__builtin_amdgcn_raw_buffer_load_b64(rs, from, (col + i) * 4, kCoherentAux));
-                    res[m][i] = res[m][i] * keep + f * __uint_as_float(x.x);
-                    res[m][i + 1] = res[m][i + 1] * keep + f * __uint_as_float(x.y);
+                for (int v = 0; v < VB; ++v) {
+                    const int s = min(s0 + v, parts - 1);  // past the last: read again, not added
+                    const int from = static_cast<int>(
+                        ((static_cast<int64_t>(unit) * a.splits + s) * a.part_rows + 16 * m + row) * kRowFloats * 4);
+                    ms[v] = bitcast<u2>(__builtin_amdgcn_raw_buffer_load_b64(rs, from + D * 4, 0, kCoherentAux));
+#pragma unroll
+                    for (int i = 0; i < PER / 2; ++i)
+                        x[v][i] = bitcast<u2>(__builtin_amdgcn_raw_buffer_load_b64(rs, from + (col + 2 * i) * 4, 0, kCoherentAux));
+                }
+                float now = rtop[m];
+#pragma unroll
+                for (int v = 0; v < VB; ++v) now = fmaxf(now, __uint_as_float(ms[v].x));
+                const float zero = now == kNone ? 0.0f : now, keep = __builtin_amdgcn_exp2f(rtop[m] - zero);
+                rtop[m] = now;
+                rsum[m] *= keep;
+#pragma unroll
+                for (int i = 0; i < PER; ++i) res[m][i] *= keep;
+#pragma unroll
+                for (int v = 0; v < VB; ++v) {
+                    if (s0 + v >= parts) break;
+                    const float f = __builtin_amdgcn_exp2f(__uint_as_float(ms[v].x) - zero);
+                    rsum[m] += f * __uint_as_float(ms[v].y);
+#pragma unroll
+                    for (int i = 0; i < PER / 2; ++i) {
+                        res[m][2 * i] += f * __uint_as_float(x[v][i].x);
+                        res[m][2 * i + 1] += f * __uint_as_float(x[v][i].y);
+                    }
                 }
             }
         }
@@ -381,8 +448,8 @@ int64_t tile_slots(int tokens, int batch, int group, int rows, bool single) {
 }
 
 template <typename T, int D>
-int attn_launch(const AttnArgs& a, int rows, hipStream_t st) {
-    const dim3 grid(static_cast<unsigned>(a.slots) * a.kv_heads, a.splits);
+int attn_launch(const AttnArgs& a, int rows, unsigned units, hipStream_t st) {
+    const dim3 grid(units, a.splits);
     if (rows == 16)
         rows_kernel<T, D, 1><<<grid, 256, 0, st>>>(a);
     else
@@ -403,16 +470,17 @@ extern "C" int tw4_paged_attention_plan(int tokens, int batch, int heads, int kv
     const int group = heads / kv_heads;
     const int rows = static_cast<int64_t>(max_query) * group > 16 ? 32 : 16;
     const int64_t units = tile_slots(tokens, batch, group, rows, single) * kv_heads;
+    const int64_t part = static_cast<int64_t>(single ? std::min(rows, group) : rows) * (head_dim + kTileFloats);
     int64_t splits = 1;
-    if (units > 0 && units < 2 * cus) {
-        splits = (2 * cus + units - 1) / units;
-        splits = std::min<int64_t>(splits, (static_cast<int64_t>(max_keys) + 127) / 128);
-        splits = std::min<int64_t>(splits, kWorkspaceFloats / (units * rows * (head_dim + kTileFloats)));
+    if (units > 0 && units < kPerCu * cus) {
+        splits = (kPerCu * cus + units - 1) / units;
+        splits = std::min<int64_t>(splits, (static_cast<int64_t>(max_keys) + kMinKeys - 1) / kMinKeys);
+        splits = std::min<int64_t>(splits, kWorkspaceFloats / (units * part));
         splits = std::max<int64_t>(splits, 1);
     }
     out[0] = rows;
     out[1] = static_cast<int>(splits);
-    out[2] = splits > 1 ? static_cast<int>(units * splits * rows * (head_dim + kTileFloats)) : 0;
+    out[2] = splits > 1 ? static_cast<int>(units * splits * part) : 0;
     out[3] = splits > 1 ? static_cast<int>(units) : 0;
     return TW4_OK;
 }
@@ -442,14 +510,17 @@ extern "C" int tw4_paged_attention(const uint16_t* q, int64_t q_token, int64_t q
     for (const void* p : {static_cast<const void*>(q), static_cast<const void*>(k), static_cast<const void*>(v),
                           static_cast<const void*>(out)})
         TW4_REQUIRE(reinterpret_cast<uintptr_t>(p) % 16 == 0, TW4_EINVAL, "paged_attention: operands must be 16-byte aligned");
+    TW4_REQUIRE(token_stride >= 0 && token_stride < 1LL << 26, TW4_EINVAL, "paged_attention: token stride (%lld)",
+                static_cast<long long>(token_stride));
     TW4_REQUIRE(q_token % 8 == 0 && q_head % 8 == 0 && page_stride % 8 == 0 && head_stride % 8 == 0 && token_stride % 8 == 0,
                 TW4_EINVAL, "paged_attention: strides must be multiples of 8");
     const int group = heads / kv_heads;
     const int64_t slots = tile_slots(tokens, batch, group, rows, !starts), units = slots * kv_heads;
     TW4_REQUIRE(units < 1LL << 31 && splits >= 1 && splits <= 65535, TW4_EINVAL, "paged_attention: grid (%lld tiles, %d splits)",
                 static_cast<long long>(units), splits);
+    const int part_rows = starts ? rows : std::min(rows, group);
     if (splits > 1) {
-        const int64_t need = units * splits * rows * (head_dim + kTileFloats);
+        const int64_t need = units * splits * part_rows * (head_dim + kTileFloats);
         TW4_REQUIRE(ws && locks && need <= ws_floats && need < kMaxPartialFloats && units <= n_locks, TW4_ESPACE,
                     "paged_attention: %d splits need %lld floats and %lld counters (got %lld, %lld)", splits,
                     static_cast<long long>(need), static_cast<long long>(units), static_cast<long long>(ws_floats),
@@ -457,8 +528,8 @@ extern "C" int tw4_paged_attention(const uint16_t* q, int64_t q_token, int64_t q
     }
     const AttnArgs a{q, k, v, table, lens, starts, out, ws, locks, q_token, q_head, page_stride, head_stride, token_stride,
                      table_stride, scale * 1.44269504088896340736f, tokens, batch, heads, kv_heads, group, num_pages, width, shift,
-                     splits, static_cast<int>(slots)};
+                     splits, part_rows};
     auto st = static_cast<hipStream_t>(stream);
-    if (bf16) return head_dim == 64 ? attn_launch<bf1, 64>(a, rows, st) : attn_launch<bf1, 128>(a, rows, st);
-    return head_dim == 64 ? attn_launch<h1, 64>(a, rows, st) : attn_launch<h1, 128>(a, rows, st);
+    if (bf16) return head_dim == 64 ? attn_launch<bf1, 64>(a, rows, static_cast<unsigned>(units), st) : attn_launch<bf1, 128>(a, rows, static_cast<unsigned>(units), st);
+    return head_dim == 64 ? attn_launch<h1, 64>(a, rows, static_cast<unsigned>(units), st) : attn_launch<h1, 128>(a, rows, static_cast<unsigned>(units), st);
 }
