@@ -22,6 +22,7 @@
 #include <type_traits>
 
 #include "tw4_attn.h"
+#include "tw4_lds.h"
 
 namespace tw4 {
 
@@ -440,6 +441,296 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(AttnArgs a) {
     }
 }
 
+typedef const __attribute__((address_space(4))) int32_t const_int;
+
+__device__ __forceinline__ u4 read_odd_free(u4 w, uint32_t exponent) {  // infinities and NaN of 16-bit halves as zero
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if ((w[i] & exponent) == exponent) w[i] &= 0xFFFF0000u;
+        if (((w[i] >> 16) & exponent) == exponent) w[i] &= 0xFFFFu;
+    }
+    return w;
+}
+
+template <typename T>
+__device__ __forceinline__ f16v mma32(const u4& a, const u4& b, const f16v& c) {
+    if constexpr (__is_same(T, h1))
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(bitcast<h8>(a), bitcast<h8>(b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(bitcast<bf8>(a), bitcast<bf8>(b), c, 0, 0, 0);
+}
+
+// Chunk kernel: a tile of 128 rows, 32 for each of four wavefronts; K and V in tiles of 64 keys through LDS by direct loads, two
+// stages: while a tile is computed the next one is on its way. A wavefront fetches 16 keys of each tile, which lie in one page.
+// Lane (c, h) = (lane % 32, lane / 32): scores S^T of row c, keys 8 (i / 4) + 4 h + i % 4 of 32.
+template <typename T, int D>
+__global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {
+    constexpr int B = 128, KEYS = 64, C = D / 8, KS = D / 16, DT = D / 32, ROWS = 64 / C, NJ = 16 / ROWS;  // ROWS of a 1 KB load
+    constexpr int TILE = KEYS * C;                                                                          // 16-byte chunks of a tile
+    constexpr uint32_t kExponent = __is_same(T, h1) ? 0x7C00u : 0x7F80u;
+    __shared__ u4 lds[2 * 2 * TILE];  // [stage][K, V][key][chunk]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c32 = lane & 31, h = lane >> 5;
+    // the last rows of a prompt see the most keys: they go first
+    const int slot = static_cast<int>(gridDim.x / a.kv_heads) - 1 - blockIdx.x / a.kv_heads, head = blockIdx.x % a.kv_heads;
+    const int split = blockIdx.y;
+    Tile t;
+    if (!find_tile<B>(a, slot, lane, t)) return;
+
+    const int r = t.first + 32 * wave + c32, tok = r / a.group;
+    const bool mine = 32 * wave + c32 < t.rows;
+    const int limit = mine ? t.len - t.fresh + tok : -1;
+    u4 q[KS];
+    {
+        const uint16_t* src = a.q + (t.start + tok) * a.q_token + (head * a.group + r - tok * a.group) * a.q_head + 8 * h;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) q[s] = mine ? *reinterpret_cast<const u4*>(src + 16 * s) : u4{0, 0, 0, 0};
+    }
+    // the wavefront's and the tile's bounds
+    int low = mine ? limit : 0x7FFFFFFF;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) low = min(low, __shfl_xor(low, d));
+    low = __builtin_amdgcn_readfirstlane(low);
+    const int rows_here = min(t.rows - 32 * wave, 32);  // <= 0: none
+    const int high = rows_here > 0 ? t.len - t.fresh + (t.first + 32 * wave + rows_here - 1) / a.group : -1;
+    const int tile_high = t.len - t.fresh + (t.first + min(t.rows, B) - 1) / a.group;
+    const int end = static_cast<int>(min(static_cast<int64_t>(tile_high) + 1, static_cast<int64_t>(a.width) << a.shift));
+    int begin = 0, stop = max(end, 0), parts = 1;
+    if (a.splits > 1 && end > 0) {
+        const int share = (max((end + a.splits - 1) / a.splits, kMinKeys) + KEYS - 1) & ~(KEYS - 1);
+        parts = (end + share - 1) / share;
+        if (split >= parts) return;
+        begin = split * share;
+        stop = min(end, begin + share);
+    } else if (split > 0) {
+        return;
+    }
+
+    f16v o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+    float top = kNone, sum = 0.0f;
+
+    const_int* table = (const_int*)(a.table + t.request * a.table_stride);
+    const uint16_t* kh = a.k + head * a.head_stride;
+    const uint16_t* vh = a.v + head * a.head_stride;
+    const int final16 = (stop - 1) & ~15;
+    const uint32_t token_bytes = static_cast<uint32_t>(a.token_stride) * 2;
+    const uint32_t lds_base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void*)lds));
+    auto entry = [&](int key) { return table[min(key + 16 * wave, final16) >> a.shift]; };  // page of this wavefront's 16 keys
+    // where chunk c of key r lies in a tile: places of 16 bytes such that the reads below meet every bank once
+    auto k_place = [](int row, int c) { return c ^ (D == 128 ? row & 15 : (row >> 1) & 7); };
+    auto v_place = [](int row, int c) { return c ^ (D == 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2); };
+    auto fetch = [&](int key, int page, int stage) {  // keys key + 16 wave .. + 15 into a stage
+        const int first = min(key + 16 * wave, final16), last = min(stop - 1 - first, 15);
+        const bool there = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.num_pages);
+        const int64_t at = (there ? page : 0) * a.page_stride + (first & ((1 << a.shift) - 1)) * a.token_stride;
+        const u4 kr = lds_rsrc(kh + at), vr = lds_rsrc(vh + at);
+        const uint32_t to = lds_base + stage * (2 * TILE * 16) + wave * (16 * C * 16);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int row = j * ROWS + lane / C;
+            const uint32_t from = min(row, last) * token_bytes;
+            lds_dma16<0>(kr, from + 16 * k_place(row, lane % C), 0, to + j * 1024);
+            lds_dma16<0>(vr, from + 16 * v_place(row, lane % C), 0, to + TILE * 16 + j * 1024);
+        }
+        return there;
+    };
+
+    // which of a tile's four sixteens are absent pages: every wavefront looks all four up
+    auto absent_of = [&](int key) {
+        int bits = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+            bits |= static_cast<uint32_t>(table[min(key + 16 * w, final16) >> a.shift]) < static_cast<uint32_t>(a.num_pages) ? 0 : 1 << w;
+        return bits;
+    };
+
+    int stage = 0, ahead = 0;
+    if (begin < stop) {
+        fetch(begin, entry(begin), 0);
+        ahead = entry(min(begin + KEYS, final16));
+    }
+    for (int base = begin; base < stop; base += KEYS, stage ^= 1) {
+        wait_stage<0>();
+        ring_barrier();
+        const int page = ahead;
+        ahead = entry(min(base + 2 * KEYS, final16));
+        if (base + KEYS < stop) fetch(base + KEYS, page, stage ^ 1);
+        const int absent = absent_of(base);
+        if (base > high) continue;  // none of this wavefront's rows sees the tile
+        const u4* kt = lds + stage * 2 * TILE;
+        const u4* vt = kt + TILE;
+        f16v s[2];
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[n][i] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < KS; ++i)
+#pragma unroll
+            for (int n = 0; n < 2; ++n) s[n] = mma32<T>(kt[(32 * n + c32) * C + k_place(c32, 2 * i + h)], q[i], s[n]);
+        const bool masked = absent || base + KEYS > min(low + 1, stop);
+        bool odd = false;
+        if (masked) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int key = 32 * n + 8 * (i >> 2) + 4 * h + (i & 3);
+                    if (base + key > min(limit, stop - 1) || (absent >> (key >> 4) & 1)) s[n][i] = kNone;
+                }
+            // A probability of zero does not take an infinity or NaN away: where some row does not see a key, such values are
+            // left out of the product and added to the rows that see them.
+#pragma unroll
+            for (int j = 0; j < TILE / 64; ++j) {
+                const u4 w = vt[64 * j + lane];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) odd |= odd16(w[i], kExponent);
+            }
+            odd = __ballot(odd) != 0;
+        }
+        float best = s[0][0];
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) best = fmaxf(best, s[n][i]);
+        {
+            const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(best), __float_as_uint(best), false, false);
+            best = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * a.scale;
+        }
+        // The sums are scaled to a new maximum only when it is more than 2^8 times the old: probabilities up to 256 instead of 1
+        // are as exact, and most tiles need no pass over the sums.
+        if (__ballot(best > top + 8.0f)) {
+            const float now = fmaxf(top, best), keep = __builtin_amdgcn_exp2f(top - (now == kNone ? 0.0f : now));
+            top = now;
+            sum *= keep;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] *= keep;
+        }
+        const float zero = top == kNone ? 0.0f : top;  // a row that has seen nothing yet
+        u4 p[4];
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][8 * u + i], a.scale, -zero));
+                    sum += x[i];
+                }
+                p[2 * n + u] = from_f32<T>(x);
+            }
+        if (odd) {
+#pragma unroll 1
+            for (int key = 0; key < KEYS; ++key) {
+                if (base + key > min(limit, stop - 1) || (absent >> (key >> 4) & 1)) continue;
+#pragma unroll
+                for (int i = 0; i < 4 * DT; ++i) {  // four values from 8 i + 4 h on
+                    const u2 four = *reinterpret_cast<const u2*>(reinterpret_cast<const char*>(vt) +
+                                                                 (key * C + v_place(key, i)) * 16 + h * 8);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint16_t bits = static_cast<uint16_t>(four[e >> 1] >> (16 * (e & 1)));
+                        if ((bits & kExponent) == kExponent)
+                            o[i >> 2][4 * (i & 3) + e] += static_cast<float>(bitcast<T>(bits));
+                    }
+                    __builtin_amdgcn_sched_barrier(0);  // one at a time: the rare path is not to take registers
+                }
+            }
+        }
+        const int g = (lane >> 4) & 1, i16 = lane & 15;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)  // 16 keys: 16 u + 8 (j / 4) + 4 h + j % 4 in place 8 h + j
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const int row = 16 * u + 4 * h + (i16 >> 2), at = (row * C + v_place(row, 4 * d + 2 * g + ((i16 & 3) >> 1))) * 16 + (i16 & 1) * 8;
+                const u2 lo = read_tr(vt, at), hi = read_tr(vt, at + 8 * C * 16);
+                u4 w = u4{lo.x, lo.y, hi.x, hi.y};
+                if (odd) w = read_odd_free(w, kExponent);
+                o[d] = mma32<T>(w, p[u], o[d]);
+            }
+    }
+
+    {
+        const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
+        sum = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+    }
+    if (parts > 1) {
+        // [unit][split][row][D + 2]: the sums, then maximum and sum
+        const int unit = slot * a.kv_heads + head;
+        constexpr int kRowFloats = D + kTileFloats;
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(a.ws, 0, 0x7FFFFFFF, kBufferFlags);
+        const int64_t first_row = static_cast<int64_t>(unit) * a.splits * a.part_rows + 32 * wave + c32;
+        if (mine) {
+            const int to = static_cast<int>((first_row + static_cast<int64_t>(split) * a.part_rows) * kRowFloats * 4);
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; i += 2)
+                    __builtin_amdgcn_raw_buffer_store_b64(u2{__float_as_uint(o[d][i]), __float_as_uint(o[d][i + 1])}, rs,
+                                                          to + (32 * d + 8 * (i >> 2) + 4 * h + (i & 3)) * 4, 0, kCoherentAux);
+            if (h == 0)
+                __builtin_amdgcn_raw_buffer_store_b64(u2{__float_as_uint(top), __float_as_uint(sum)}, rs, to + D * 4, 0, kCoherentAux);
+        }
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        int* flag = reinterpret_cast<int*>(lds);
+        if (threadIdx.x == 0)
+            *flag = __hip_atomic_fetch_add(a.locks + unit, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
+        __syncthreads();
+        if (!*flag) return;
+        if (mine) {
+            top = kNone, sum = 0.0f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+            for (int s = 0; s < parts; ++s) {
+                const int from = static_cast<int>((first_row + static_cast<int64_t>(s) * a.part_rows) * kRowFloats * 4);
+                const u2 ms = bitcast<u2>(__builtin_amdgcn_raw_buffer_load_b64(rs, from + D * 4, 0, kCoherentAux));
+                u2 x[8 * DT];
+#pragma unroll
+                for (int i = 0; i < 8 * DT; ++i)
+                    x[i] = bitcast<u2>(__builtin_amdgcn_raw_buffer_load_b64(
+                        rs, from + (8 * (i >> 1) + 4 * h + 2 * (i & 1)) * 4, 0, kCoherentAux));
+                const float other = __uint_as_float(ms.x), now = fmaxf(top, other), zero = now == kNone ? 0.0f : now;
+                const float keep = __builtin_amdgcn_exp2f(top - zero), f = __builtin_amdgcn_exp2f(other - zero);
+                top = now;
+                sum = sum * keep + f * __uint_as_float(ms.y);
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2) {
+                        o[d][i] = o[d][i] * keep + f * __uint_as_float(x[8 * d + (i >> 1)].x);
+                        o[d][i + 1] = o[d][i + 1] * keep + f * __uint_as_float(x[8 * d + (i >> 1)].y);
+                    }
+            }
+        }
+        if (threadIdx.x == 0) __hip_atomic_store(a.locks + unit, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    // a lane has 4 of every 8 values: the halves of the wavefront exchange blocks, so that each stores 16 bytes
+    const bool nothing = sum == 0.0f;  // no key, or none with a score above -inf: zero
+    const float inv = 1.0f / sum;
+    uint16_t* dst = a.out + (static_cast<int64_t>(t.start + tok) * a.heads + head * a.group + r - tok * a.group) * D + 8 * h;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = nothing ? 0.0f : o[d][8 * b + i] * inv;
+            const u4 y = from_f32<T>(x);
+            const auto e = __builtin_amdgcn_permlane32_swap(y[0], y[2], false, false);
+            const auto f = __builtin_amdgcn_permlane32_swap(y[1], y[3], false, false);
+            if (mine) *reinterpret_cast<u4*>(dst + 32 * d + 16 * b) = u4{e[0], f[0], e[1], f[1]};
+        }
+}
+
 constexpr int64_t kWorkspaceFloats = TW4_AUTO_SPLIT_FLOATS;
 
 int64_t tile_slots(int tokens, int batch, int group, int rows, bool single) {
@@ -452,8 +743,10 @@ int attn_launch(const AttnArgs& a, int rows, unsigned units, hipStream_t st) {
     const dim3 grid(units, a.splits);
     if (rows == 16)
         rows_kernel<T, D, 1><<<grid, 256, 0, st>>>(a);
-    else
+    else if (rows == 32)
         rows_kernel<T, D, 2><<<grid, 256, 0, st>>>(a);
+    else
+        chunk_kernel<T, D><<<grid, 256, 0, st>>>(a);
     TW4_LAUNCH_CHECK("paged_attention: launch");
     return TW4_OK;
 }
@@ -468,7 +761,8 @@ extern "C" int tw4_paged_attention_plan(int tokens, int batch, int heads, int kv
     TW4_REQUIRE(out && tokens >= 0 && batch >= 0 && kv_heads >= 1 && heads >= 1 && heads % kv_heads == 0 && head_dim >= 1 && cus >= 1,
                 TW4_EINVAL, "paged_attention_plan: bad sizes");
     const int group = heads / kv_heads;
-    const int rows = static_cast<int64_t>(max_query) * group > 16 ? 32 : 16;
+    const int64_t most = static_cast<int64_t>(max_query) * group;
+    const int rows = most > 32 ? 128 : most > 16 ? 32 : 16;
     const int64_t units = tile_slots(tokens, batch, group, rows, single) * kv_heads;
     const int64_t part = static_cast<int64_t>(single ? std::min(rows, group) : rows) * (head_dim + kTileFloats);
     int64_t splits = 1;
@@ -497,7 +791,7 @@ extern "C" int tw4_paged_attention(const uint16_t* q, int64_t q_token, int64_t q
     const int shift = page_shift(page_size);
     TW4_REQUIRE(shift >= 0, TW4_EINVAL, "paged_attention: page_size 16, 32, 64, 128 or 256 (%d)", page_size);
     TW4_REQUIRE(scale > 0.0f && scale < 1e30f, TW4_EINVAL, "paged_attention: a positive scale (%g)", scale);
-    TW4_REQUIRE(rows == 16 || rows == 32, TW4_ECONFIG, "paged_attention: tiles of 16 or 32 rows (%d)", rows);
+    TW4_REQUIRE(rows == 16 || rows == 32 || rows == 128, TW4_ECONFIG, "paged_attention: tiles of 16, 32 or 128 rows (%d)", rows);
     TW4_REQUIRE(width >= 0 && num_pages >= 0 && static_cast<int64_t>(num_pages) * page_size < 1LL << 31 &&
                     static_cast<int64_t>(width) * page_size < 1LL << 31,
                 TW4_EINVAL, "paged_attention: fewer than 2^31 slots (%d pages of %d, %d per request)", num_pages, page_size, width);
