@@ -485,11 +485,7 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {
 #pragma unroll
         for (int s = 0; s < KS; ++s) q[s] = mine ? *reinterpret_cast<const u4*>(src + 16 * s) : u4{0, 0, 0, 0};
     }
-    // the wavefront's and the tile's bounds
-    int low = mine ? limit : 0x7FFFFFFF;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) low = min(low, __shfl_xor(low, d));
-    low = __builtin_amdgcn_readfirstlane(low);
+    // the last keys that the wavefront's rows and the tile's see
     const int rows_here = min(t.rows - 32 * wave, 32);  // <= 0: none
     const int high = rows_here > 0 ? t.len - t.fresh + (t.first + 32 * wave + rows_here - 1) / a.group : -1;
     const int tile_high = t.len - t.fresh + (t.first + min(t.rows, B) - 1) / a.group;
@@ -518,14 +514,20 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {
     const int final16 = (stop - 1) & ~15;
     const uint32_t token_bytes = static_cast<uint32_t>(a.token_stride) * 2;
     const uint32_t lds_base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void*)lds));
-    auto entry = [&](int key) { return table[min(key + 16 * wave, final16) >> a.shift]; };  // page of this wavefront's 16 keys
     // where chunk c of key r lies in a tile: places of 16 bytes such that the reads below meet every bank once
     auto k_place = [](int row, int c) { return c ^ (D == 128 ? row & 15 : (row >> 1) & 7); };
     auto v_place = [](int row, int c) { return c ^ (D == 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2); };
-    auto fetch = [&](int key, int page, int stage) {  // keys key + 16 wave .. + 15 into a stage
+    // the pages of a tile's four sixteens
+    typedef int i4 __attribute__((ext_vector_type(4)));
+    auto entries = [&](int key) {
+        auto one = [&](int k) { return static_cast<int>(table[min(k, final16) >> a.shift]); };
+        return i4{one(key), one(key + 16), one(key + 32), one(key + 48)};
+    };
+    auto there = [&](int page) { return static_cast<uint32_t>(page) < static_cast<uint32_t>(a.num_pages); };
+    auto fetch = [&](int key, i4 pages, int stage) {  // keys key + 16 wave .. + 15 into a stage
         const int first = min(key + 16 * wave, final16), last = min(stop - 1 - first, 15);
-        const bool there = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.num_pages);
-        const int64_t at = (there ? page : 0) * a.page_stride + (first & ((1 << a.shift) - 1)) * a.token_stride;
+        const int page = __builtin_amdgcn_readfirstlane(wave < 2 ? (wave < 1 ? pages.x : pages.y) : (wave < 3 ? pages.z : pages.w));
+        const int64_t at = (there(page) ? page : 0) * a.page_stride + (first & ((1 << a.shift) - 1)) * a.token_stride;
         const u4 kr = lds_rsrc(kh + at), vr = lds_rsrc(vh + at);
         const uint32_t to = lds_base + stage * (2 * TILE * 16) + wave * (16 * C * 16);
 #pragma unroll
@@ -535,33 +537,33 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {
             lds_dma16<0>(kr, from + 16 * k_place(row, lane % C), 0, to + j * 1024);
             lds_dma16<0>(vr, from + 16 * v_place(row, lane % C), 0, to + TILE * 16 + j * 1024);
         }
-        return there;
     };
 
-    // which of a tile's four sixteens are absent pages: every wavefront looks all four up
-    auto absent_of = [&](int key) {
-        int bits = 0;
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-            bits |= static_cast<uint32_t>(table[min(key + 16 * w, final16) >> a.shift]) < static_cast<uint32_t>(a.num_pages) ? 0 : 1 << w;
-        return bits;
+    // Table entries are read two tiles before their keys are used, keys one tile before.
+    int stage = 0, absent = 0;
+    i4 next = i4{0, 0, 0, 0};
+    auto absent_of = [&](i4 page) {
+        return (there(page.x) ? 0 : 1) | (there(page.y) ? 0 : 2) | (there(page.z) ? 0 : 4) | (there(page.w) ? 0 : 8);
     };
-
-    int stage = 0, ahead = 0;
     if (begin < stop) {
-        fetch(begin, entry(begin), 0);
-        ahead = entry(min(begin + KEYS, final16));
+        const i4 page = entries(begin);
+        next = entries(min(begin + KEYS, final16));
+        fetch(begin, page, 0);
+        absent = absent_of(page);
     }
-    for (int base = begin; base < stop; base += KEYS, stage ^= 1) {
+    const int g = (lane >> 4) & 1, i16 = lane & 15;
+    auto tile = [&](int base, auto masked) {
+        constexpr bool kMasked = decltype(masked)::value;
         wait_stage<0>();
         ring_barrier();
-        const int page = ahead;
-        ahead = entry(min(base + 2 * KEYS, final16));
-        if (base + KEYS < stop) fetch(base + KEYS, page, stage ^ 1);
-        const int absent = absent_of(base);
-        if (base > high) continue;  // none of this wavefront's rows sees the tile
+        const int gone = absent;
+        absent = absent_of(next);
+        if (base + KEYS < stop) fetch(base + KEYS, next, stage ^ 1);
+        next = entries(min(base + 2 * KEYS, final16));
         const u4* kt = lds + stage * 2 * TILE;
         const u4* vt = kt + TILE;
+        stage ^= 1;
+        if (base > high) return;  // none of this wavefront's rows sees the tile
         f16v s[2];
 #pragma unroll
         for (int n = 0; n < 2; ++n)
@@ -571,19 +573,26 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {
         for (int i = 0; i < KS; ++i)
 #pragma unroll
             for (int n = 0; n < 2; ++n) s[n] = mma32<T>(kt[(32 * n + c32) * C + k_place(c32, 2 * i + h)], q[i], s[n]);
-        const bool masked = absent || base + KEYS > min(low + 1, stop);
+        // six reads ahead of the products that use them
+        __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+        for (int i = 0; i < 2 * KS - 6; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 6, 0);
         bool odd = false;
-        if (masked) {
+        if constexpr (kMasked) {
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const int key = 32 * n + 8 * (i >> 2) + 4 * h + (i & 3);
-                    if (base + key > min(limit, stop - 1) || (absent >> (key >> 4) & 1)) s[n][i] = kNone;
+                    if (base + key > min(limit, stop - 1) || (gone >> (key >> 4) & 1)) s[n][i] = kNone;
                 }
             // A probability of zero does not take an infinity or NaN away: where some row does not see a key, such values are
             // left out of the product and added to the rows that see them.
-#pragma unroll
+#pragma unroll 2
             for (int j = 0; j < TILE / 64; ++j) {
                 const u4 w = vt[64 * j + lane];
 #pragma unroll
@@ -612,23 +621,10 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {
                 for (int i = 0; i < 16; ++i) o[d][i] *= keep;
         }
         const float zero = top == kNone ? 0.0f : top;  // a row that has seen nothing yet
-        u4 p[4];
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                float x[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][8 * u + i], a.scale, -zero));
-                    sum += x[i];
-                }
-                p[2 * n + u] = from_f32<T>(x);
-            }
-        if (odd) {
+        if (kMasked && odd) {
 #pragma unroll 1
             for (int key = 0; key < KEYS; ++key) {
-                if (base + key > min(limit, stop - 1) || (absent >> (key >> 4) & 1)) continue;
+                if (base + key > min(limit, stop - 1) || (gone >> (key >> 4) & 1)) continue;
 #pragma unroll
                 for (int i = 0; i < 4 * DT; ++i) {  // four values from 8 i + 4 h on
                     const u2 four = *reinterpret_cast<const u2*>(reinterpret_cast<const char*>(vt) +
@@ -636,25 +632,38 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const uint16_t bits = static_cast<uint16_t>(four[e >> 1] >> (16 * (e & 1)));
-                        if ((bits & kExponent) == kExponent)
-                            o[i >> 2][4 * (i & 3) + e] += static_cast<float>(bitcast<T>(bits));
+                        if ((bits & kExponent) == kExponent) o[i >> 2][4 * (i & 3) + e] += static_cast<float>(bitcast<T>(bits));
                     }
                     __builtin_amdgcn_sched_barrier(0);  // one at a time: the rare path is not to take registers
                 }
             }
         }
-        const int g = (lane >> 4) & 1, i16 = lane & 15;
 #pragma unroll
-        for (int u = 0; u < 4; ++u)  // 16 keys: 16 u + 8 (j / 4) + 4 h + j % 4 in place 8 h + j
+        for (int u = 0; u < 4; ++u) {  // 16 keys: 16 u + 8 (j / 4) + 4 h + j % 4 in place 8 h + j
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u >> 1][8 * (u & 1) + i], a.scale, -zero));
+                sum += x[i];
+            }
+            const u4 p = from_f32<T>(x);
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                const int row = 16 * u + 4 * h + (i16 >> 2), at = (row * C + v_place(row, 4 * d + 2 * g + ((i16 & 3) >> 1))) * 16 + (i16 & 1) * 8;
+                const int row = 16 * u + 4 * h + (i16 >> 2);
+                const int at = (row * C + v_place(row, 4 * d + 2 * g + ((i16 & 3) >> 1))) * 16 + (i16 & 1) * 8;
                 const u2 lo = read_tr(vt, at), hi = read_tr(vt, at + 8 * C * 16);
                 u4 w = u4{lo.x, lo.y, hi.x, hi.y};
-                if (odd) w = read_odd_free(w, kExponent);
-                o[d] = mma32<T>(w, p[u], o[d]);
+                if (kMasked && odd) w = read_odd_free(w, kExponent);
+                o[d] = mma32<T>(w, p, o[d]);
             }
-    }
+        }
+    };
+    // Tiles that every row sees whole come first and run without a mask; from the first one that some row does not (or a page
+    // that is none) on, all are masked.
+    const int clear = min(t.len - t.fresh + t.first / a.group + 1, stop);
+    int base = begin;
+    for (; base + KEYS <= clear && !absent; base += KEYS) tile(base, std::false_type());
+    for (; base < stop; base += KEYS) tile(base, std::true_type());
 
     {
         const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
