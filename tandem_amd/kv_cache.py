@@ -10,13 +10,14 @@ alone. Nothing is read back: a step, with its pages, can be captured in a HIP gr
 
 from __future__ import annotations
 
+import functools
 from dataclasses import dataclass
 from typing import TYPE_CHECKING, NamedTuple, Sequence
 
 import torch
 
 from tandem_amd.layers import rotary, w4_hip
-from tandem_amd.layers.rotary import PAGE_SIZES, check_int32
+from tandem_amd.layers.rotary import PAGE_SIZES, check_int32, layout
 
 if TYPE_CHECKING:
     from tandem_amd.model import DecoderConfig
@@ -35,19 +36,29 @@ class PagePlan(NamedTuple):
     counts: torch.Tensor       # [4]
 
 
-def _check_table(who: str, page_table: torch.Tensor, free_pages: torch.Tensor, page_size: int) -> None:
-    if not (page_table.is_cuda and page_table.dim() == 2 and page_table.dtype == torch.int32) or (
-            page_table.shape[1] > 1 and page_table.stride(1) != 1) or (
-            page_table.shape[0] > 1 and page_table.stride(0) < page_table.shape[1]):
+@functools.lru_cache(maxsize=1 << 12)
+def _checked(who: str, table: tuple, free_pages: tuple, page_size: int, num_tokens: int,
+             *vectors: tuple[str, tuple, int | None]) -> tuple:
+    """(requests, pages per request, row stride, free pages, GPU); vectors: (name, layout, length, None for the number of requests).
+    Once for each combination of layouts: an eager call is bound by the host."""
+    shape, stride, dtype, index = table
+    if not (index >= 0 and len(shape) == 2 and dtype == torch.int32) or (shape[1] > 1 and stride[1] != 1) or (
+            shape[0] > 1 and stride[0] < shape[1]):
         raise RuntimeError(f"{who}: page_table must be an int32 GPU tensor [requests, pages per request] of separate contiguous rows "
-                           f"(got {page_table.dtype} {tuple(page_table.shape)} on {page_table.device})")
+                           f"(got {dtype} {tuple(shape)} on {index}, strides {stride})")
+    batch, width = shape
     if page_size not in PAGE_SIZES:
         raise RuntimeError(f"{who}: a page size of {PAGE_SIZES} (got {page_size})")
-    check_int32(who, "free_pages", free_pages, (free_pages.numel(),), page_table)
-
-
-def _row_stride(t: torch.Tensor) -> int:
-    return max(t.stride(0), t.shape[1])
+    if not 1 <= batch <= MAX_REQUESTS:
+        raise RuntimeError(f"{who}: 1 to {MAX_REQUESTS} requests (got {batch})")
+    if not 0 <= num_tokens < 1 << 30:
+        raise RuntimeError(f"{who}: 0 <= num_tokens < 2^30 (got {num_tokens})")
+    if len(free_pages[0]) != 1:
+        raise RuntimeError(f"{who}: free_pages must be one list (got {list(free_pages[0])})")
+    check_int32(who, "free_pages", free_pages, tuple(free_pages[0]), index)
+    for name, vector, length in vectors:
+        check_int32(who, name, vector, (batch if length is None else length,), index)
+    return batch, width, max(stride[0], width), free_pages[0][0], index
 
 
 def plan_pages(context_lens: torch.Tensor, query_lens: torch.Tensor, page_table: torch.Tensor, free_pages: torch.Tensor,
@@ -62,54 +73,44 @@ def plan_pages(context_lens: torch.Tensor, query_lens: torch.Tensor, page_table:
     int32 GPU tensors; lengths below zero count as zero, and the new tokens are fewer than 2^31 in all. seq_lens_out (context_lens
     itself, to advance it) and taken_out (taken itself) are written instead of new tensors. Nothing is read back; the caller that
     wants to know whether the pages sufficed reads counts[2]."""
-    who = "plan_pages"
-    _check_table(who, page_table, free_pages, page_size)
-    batch, width = page_table.shape
-    if not 1 <= batch <= MAX_REQUESTS:
-        raise RuntimeError(f"{who}: 1 to {MAX_REQUESTS} requests (got {batch})")
-    if not 0 <= num_tokens < 1 << 30:
-        raise RuntimeError(f"{who}: 0 <= num_tokens < 2^30 (got {num_tokens})")
-    dev = page_table.device
-    for name, t, shape in (("context_lens", context_lens, (batch,)), ("query_lens", query_lens, (batch,)), ("taken", taken, (1,)),
-                           ("seq_lens_out", seq_lens_out, (batch,)), ("taken_out", taken_out, (1,))):
-        if t is not None:
-            check_int32(who, name, t, shape, page_table)
-    # one allocation for what is new: each starts a 16-byte line
-    sizes = [batch + 1, 0 if seq_lens_out is not None else batch, num_tokens, num_tokens, 0 if taken_out is not None else 1, 4]
-    starts = [0]
-    for n in sizes:
-        starts.append(starts[-1] + (n + 3) // 4 * 4)
-    flat = torch.empty(starts[-1], dtype=torch.int32, device=dev)
-    query_start, lens, positions, slots, left, counts = (flat[s:s + n] for s, n in zip(starts, sizes))
-    plan = PagePlan(query_start, lens if seq_lens_out is None else seq_lens_out, positions, slots,
-                    left if taken_out is None else taken_out, counts)
-    index = page_table.get_device()
+    outs = () if seq_lens_out is None else (("seq_lens_out", layout(seq_lens_out), None),)
+    if taken_out is not None:
+        outs += (("taken_out", layout(taken_out), 1),)
+    batch, width, stride, n_free, index = _checked(
+        "plan_pages", layout(page_table), layout(free_pages), page_size, num_tokens, ("context_lens", layout(context_lens), None),
+        ("query_lens", layout(query_lens), None), ("taken", layout(taken), 1), *outs)
+    # one allocation for what is new
+    sizes = (batch + 1, num_tokens, num_tokens, 4, 1 if taken_out is None else 0, batch if seq_lens_out is None else 0)
+    flat = torch.empty(sum(sizes), dtype=torch.int32, device=page_table.device)
+    query_start, positions, slots, counts, left, lens = flat.split_with_sizes(sizes)
+    if seq_lens_out is not None:
+        lens = seq_lens_out
+    if taken_out is not None:
+        left = taken_out
+    base = flat.data_ptr()
     with w4_hip.on_device(index):
         w4_hip.check(w4_hip.library().tw4_plan_pages(
-            context_lens.data_ptr(), query_lens.data_ptr(), page_table.data_ptr(), _row_stride(page_table), width,
-            free_pages.data_ptr(), free_pages.numel(), taken.data_ptr(), plan.taken.data_ptr(), page_size,
-            plan.query_start.data_ptr(), plan.seq_lens.data_ptr(), plan.positions.data_ptr(), plan.slots.data_ptr(),
-            plan.counts.data_ptr(), batch, num_tokens, w4_hip.raw_stream(index)))
-    return plan
+            context_lens.data_ptr(), query_lens.data_ptr(), page_table.data_ptr(), stride, width, free_pages.data_ptr(), n_free,
+            taken.data_ptr(), left.data_ptr(), page_size, base, lens.data_ptr(), base + 4 * (batch + 1),
+            base + 4 * (batch + 1 + num_tokens), base + 4 * (batch + 1 + 2 * num_tokens), batch, num_tokens, w4_hip.raw_stream(index)))
+    return PagePlan(query_start, lens, positions, slots, left, counts)
 
 
 def release_pages(ended: torch.Tensor, context_lens: torch.Tensor, page_table: torch.Tensor, free_pages: torch.Tensor,
                   taken: torch.Tensor, page_size: int) -> None:
     """The pages of the requests ``ended`` (int32 [n], indices into page_table's rows; others are passed over) go back to the
     list: taken[0] falls by their number and they are the next to be given. Their rows become -1 and their lengths 0, all in place."""
-    who = "release_pages"
-    _check_table(who, page_table, free_pages, page_size)
-    batch, width = page_table.shape
-    check_int32(who, "ended", ended, (ended.numel(),), page_table)
-    check_int32(who, "context_lens", context_lens, (batch,), page_table)
-    check_int32(who, "taken", taken, (1,), page_table)
-    if ended.numel() == 0 or batch == 0:
+    if ended.dim() != 1:
+        raise RuntimeError(f"release_pages: ended must be one list (got {list(ended.shape)})")
+    batch, width, stride, n_free, index = _checked(
+        "release_pages", layout(page_table), layout(free_pages), page_size, 0, ("ended", layout(ended), ended.shape[0]),
+        ("context_lens", layout(context_lens), None), ("taken", layout(taken), 1))
+    if ended.shape[0] == 0:
         return
-    index = page_table.get_device()
     with w4_hip.on_device(index):
         w4_hip.check(w4_hip.library().tw4_release_pages(
-            ended.data_ptr(), ended.numel(), page_table.data_ptr(), _row_stride(page_table), width, context_lens.data_ptr(), batch,
-            free_pages.data_ptr(), free_pages.numel(), taken.data_ptr(), page_size, w4_hip.raw_stream(index)))
+            ended.data_ptr(), ended.shape[0], page_table.data_ptr(), stride, width, context_lens.data_ptr(), batch,
+            free_pages.data_ptr(), n_free, taken.data_ptr(), page_size, w4_hip.raw_stream(index)))
 
 
 @dataclass(frozen=True)

@@ -10,18 +10,49 @@ import math
 import torch
 
 from tandem_amd.layers import w4_hip
-from tandem_amd.layers.rotary import TYPES, check_cache, check_int32
+from tandem_amd.layers.rotary import TYPES, check_cache, check_int32, layout
 
 
+# Every check of a call but those of addresses and of who follows it, once for each combination of layouts and sizes: an eager call
+# is bound by the host (a decode step's, 15.6 -> 12.4 us).
 @functools.lru_cache(maxsize=1 << 14)
-def _plan(index: int, tokens: int, batch: int, heads: int, kv_heads: int, head_dim: int, max_query: int, max_keys: int,
-          single: bool) -> tuple[int, int, int, int]:
-    """(rows of a tile, splits, workspace floats, counters) of a call of these sizes on a GPU."""
-    out = (w4_hip._I * 4)()
-    cus = torch.cuda.get_device_properties(index).multi_processor_count
-    w4_hip.check(w4_hip.library().tw4_paged_attention_plan(tokens, batch, heads, kv_heads, head_dim, max_query, max_keys,
-                                                           int(single), cus, out))
-    return tuple(out)
+def _checked(q: tuple, k: tuple, v: tuple, table: tuple, lens: tuple, starts: tuple | None, out: tuple | None, most: int | None,
+             longest: int | None, scale: float | None) -> tuple:
+    """(strides of q, rows of a tile, splits and what else tw4_paged_attention takes by value)."""
+    who = "paged_attention"
+    shape, stride, dtype, index = q
+    if not (index >= 0 and len(shape) == 3 and dtype in TYPES and shape[2] in (64, 128) and stride[2] == 1):
+        raise RuntimeError(f"{who}: q must be float16 or bfloat16 GPU rows [tokens, heads, 64 or 128] (got {tuple(shape)}, {dtype})")
+    tokens, heads, d = shape
+    if any(stride[i] % 8 for i in (0, 1) if shape[i] > 1):
+        raise RuntimeError(f"{who}: rows and heads of q must be 16-byte aligned (strides {stride})")
+    pages, kv_heads, size = check_cache(who, k, v, dtype, index, None, d)
+    if kv_heads < 1 or heads < 1 or heads % kv_heads:
+        raise RuntimeError(f"{who}: heads must be a multiple of the cache's KV heads ({heads}, {kv_heads})")
+    if len(table[0]) != 2 or table[2] != torch.int32 or table[3] != index or (table[0][1] > 1 and table[1][1] != 1):
+        raise RuntimeError(f"{who}: page_table must be int32 [requests, pages per request] on q's GPU, rows contiguous "
+                           f"(got {table[2]} {tuple(table[0])})")
+    batch, width = table[0]
+    check_int32(who, "seq_lens", lens, (batch,), index)
+    if starts is not None:
+        check_int32(who, "query_start", starts, (batch + 1,), index)
+    elif tokens != batch:
+        raise RuntimeError(f"{who}: without query_start there is one token per request ({tokens} tokens, {batch} requests)")
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not (scale > 0 and math.isfinite(scale)):
+        raise RuntimeError(f"{who}: a positive scale (got {scale})")
+    if out is not None and out != (shape, (heads * d, d, 1), dtype, index):
+        raise RuntimeError(f"{who}: out must be a contiguous {dtype} tensor {list(shape)} on q's GPU")
+    rows, splits = 16, 1
+    if tokens and batch:
+        plan = (w4_hip._I * 4)()
+        w4_hip.check(w4_hip.library().tw4_paged_attention_plan(
+            tokens, batch, heads, kv_heads, d, 1 if starts is None else tokens if most is None else min(most, tokens),
+            width * size if longest is None else min(longest, width * size), int(starts is None),
+            torch.cuda.get_device_properties(index).multi_processor_count, plan))
+        rows, splits = plan[0], plan[1]
+    return ((stride[0] if tokens > 1 else 0, stride[1] if heads > 1 else 0), (*k[1][:3], pages, size),
+            (table[1][0] if batch > 1 else 0, width), (tokens, batch, heads, kv_heads, d, scale, rows, splits, TYPES[dtype]), index)
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
@@ -41,50 +72,27 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 
     max_query_len, max_seq_len: bounds the host knows; they only choose how the work is divided (T and the table's width
     otherwise). Results do not depend on the order in which workgroups run. Inference only."""
-    who = "paged_attention"
-    if not (q.is_cuda and q.dim() == 3 and q.dtype in TYPES and q.shape[2] in (64, 128) and q.stride(2) == 1):
-        raise RuntimeError(f"{who}: q must be float16 or bfloat16 GPU rows [tokens, heads, 64 or 128] (got {tuple(q.shape)}, "
-                           f"{q.dtype} on {q.device})")
-    if not w4_hip.plain(q):
-        raise RuntimeError(f"{who}: inference only, no gradient, transform or tracer can follow q")
-    tokens, heads, d = q.shape
-    if any(q.stride(i) % 8 for i in (0, 1) if q.shape[i] > 1) or q.data_ptr() % 16:
-        raise RuntimeError(f"{who}: rows and heads of q must be 16-byte aligned (strides {q.stride()})")
-    pages, kv_heads, size = check_cache(who, k_cache, v_cache, q, None, d)
-    if kv_heads < 1 or heads < 1 or heads % kv_heads:
-        raise RuntimeError(f"{who}: heads must be a multiple of the cache's KV heads ({heads}, {kv_heads})")
-    if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.device != q.device or (
-            page_table.shape[1] > 1 and page_table.stride(1) != 1):
-        raise RuntimeError(f"{who}: page_table must be int32 [requests, pages per request] on {q.device}, rows contiguous "
-                           f"(got {page_table.dtype} {tuple(page_table.shape)} on {page_table.device})")
-    batch, width = page_table.shape
-    check_int32(who, "seq_lens", seq_lens, (batch,), q)
-    if query_start is not None:
-        check_int32(who, "query_start", query_start, (batch + 1,), q)
-    elif tokens != batch:
-        raise RuntimeError(f"{who}: without query_start there is one token per request ({tokens} tokens, {batch} requests)")
-    scale = d ** -0.5 if scale is None else float(scale)
-    if not (scale > 0 and math.isfinite(scale)):
-        raise RuntimeError(f"{who}: a positive scale (got {scale})")
-    if out is None:
-        out = torch.empty((tokens, heads, d), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous() or out.data_ptr() % 16:
-        raise RuntimeError(f"{who}: out must be a contiguous 16-byte aligned {q.dtype} tensor {list(q.shape)} on {q.device}")
-    if tokens == 0 or batch == 0:
-        return out
-    index = q.get_device()
-    single = query_start is None
-    longest = width * size if max_seq_len is None else min(int(max_seq_len), width * size)
-    most = 1 if single else tokens if max_query_len is None else min(int(max_query_len), tokens)
     # the longest context in steps: a decode loop asks for a few plans only
-    rows, splits, floats, counters = _plan(index, tokens, batch, heads, kv_heads, d, most, (longest + 511) // 512 * 512, single)
+    (q_strides, cache, (table_stride, width), sizes, index) = _checked(
+        layout(q), layout(k_cache), layout(v_cache), layout(page_table), layout(seq_lens),
+        None if query_start is None else layout(query_start), None if out is None else layout(out),
+        max_query_len, None if max_seq_len is None else (max_seq_len + 511) // 512 * 512, scale)
+    if not w4_hip.plain(q):
+        raise RuntimeError("paged_attention: inference only, no gradient, transform or tracer can follow q")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    qp, kp, vp, op = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr()
+    if (qp | kp | vp | op) % 16:
+        raise RuntimeError("paged_attention: q, out and the caches must be 16-byte aligned")
+    if sizes[0] == 0 or sizes[1] == 0:
+        return out
     with w4_hip.on_device(index):
-        ws, locks = w4_hip.stream_workspace(q.device) if splits > 1 else (None, None)
+        wsp = locksp = floats = counters = 0
+        if sizes[7] > 1:
+            ws, locks = w4_hip.stream_workspace(q.device)
+            wsp, locksp, floats, counters = ws.data_ptr(), locks.data_ptr(), ws.numel(), locks.numel()
         w4_hip.check(w4_hip.library().tw4_paged_attention(
-            q.data_ptr(), q.stride(0) if tokens > 1 else 0, q.stride(1) if heads > 1 else 0, k_cache.data_ptr(),
-            v_cache.data_ptr(), *k_cache.stride()[:3], pages, size, page_table.data_ptr(),
-            page_table.stride(0) if batch > 1 else 0, width, seq_lens.data_ptr(),
-            None if single else query_start.data_ptr(), out.data_ptr(), None if ws is None else ws.data_ptr(),
-            0 if ws is None else ws.numel(), None if locks is None else locks.data_ptr(), 0 if locks is None else locks.numel(),
-            tokens, batch, heads, kv_heads, d, scale, rows, splits, TYPES[q.dtype], w4_hip.raw_stream(index)))
+            qp, *q_strides, kp, vp, *cache, page_table.data_ptr(), table_stride, width, seq_lens.data_ptr(),
+            None if query_start is None else query_start.data_ptr(), op, wsp, floats, locksp, counters, *sizes,
+            w4_hip.raw_stream(index)))
     return out

@@ -291,7 +291,7 @@ def test_strides_layouts_and_refusals():
         assert torch.equal(paged_attention(*other, lens, starts), want)
     ok = dict(q=q, k_cache=k, v_cache=v, page_table=table, seq_lens=lens, query_start=starts)
     for change, needle in ((dict(q=q.float()), "float16 or bfloat16"), (dict(q=q[..., :64]), "caches"), (dict(q=q[:, :6]), "multiple"),
-                           (dict(q=q.clone().requires_grad_()), "inference"), (dict(q=qkv.view(20, -1)[:, 4:132].view(20, 1, 128)), "aligned"),
+                           (dict(q=q.clone().requires_grad_()), "inference"), (dict(q=qkv.view(20, -1)[:, 4:1028].view(20, 8, 128)), "aligned"),
                            (dict(k_cache=k.half()), "caches of"), (dict(k_cache=k[:, :, :24], v_cache=v[:, :, :24]), "page size"),
                            (dict(v_cache=by_token[1]), "layout"), (dict(page_table=table.long()), "page_table"),
                            (dict(page_table=table.t()), "page_table"), (dict(seq_lens=lens[:1]), "seq_lens"),
