@@ -112,6 +112,18 @@ __device__ __forceinline__ bool odd16(uint32_t v, uint32_t exponent) {  // eithe
     return (v & exponent) == exponent || ((v >> 16) & exponent) == exponent;
 }
 
+// The page table by scalar loads: no kernel here writes it.
+typedef const __attribute__((address_space(4))) int32_t const_int;
+
+__device__ __forceinline__ u4 read_odd_free(u4 w, uint32_t exponent) {  // infinities and NaN of 16-bit halves as zero
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if ((w[i] & exponent) == exponent) w[i] &= 0xFFFF0000u;
+        if (((w[i] >> 16) & exponent) == exponent) w[i] &= 0xFFFFu;
+    }
+    return w;
+}
+
 constexpr float kNone = -__builtin_inff();
 
 template <typename T, int D, int MT>
@@ -122,7 +134,7 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(AttnArgs a) {
     __shared__ u4 lds[4 * 32 * C];
     __shared__ float stat[2][4][B];
     __shared__ int last_flag;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c16 = lane & 15, g4 = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c16 = lane & 15, g4 = lane >> 4;
     const int slot = blockIdx.x / a.kv_heads, head = blockIdx.x - slot * a.kv_heads, split = blockIdx.y;
     Tile t;
     if (!find_tile<B>(a, slot, lane, t)) return;
@@ -168,7 +180,7 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(AttnArgs a) {
         for (int d = 0; d < DT; ++d) o[m][d] = f4{0, 0, 0, 0};
     }
     u4* vt = lds + wave * 32 * C;
-    const int32_t* table = a.table + t.request * a.table_stride;
+    const_int* table = (const_int*)(a.table + t.request * a.table_stride);
     const char* kh = reinterpret_cast<const char*>(a.k + head * a.head_stride);
     const char* vh = reinterpret_cast<const char*>(a.v + head * a.head_stride);
     const int final16 = (stop - 1) & ~15;  // the last 16 keys that are there
@@ -177,9 +189,8 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(AttnArgs a) {
     // A block of 32 keys is two halves of 16, each in one page. Table entries are fetched a block before the keys they lead to,
     // K a block before its product, V a block before it goes to LDS: each load has a block's arithmetic to arrive in.
     u4 kf[2][KS], vf[VJ];
-    auto pages = [&](int base, int (&page)[2]) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) page[h] = table[min(base + 16 * h, final16) >> a.shift];
+    auto pages = [&](int base) {
+        return int2{table[min(base, final16) >> a.shift], table[min(base + 16, final16) >> a.shift]};
     };
     auto there = [&](int page) { return static_cast<uint32_t>(page) < static_cast<uint32_t>(a.num_pages); };
     // byte offset of half h's first key; a page the table does not have is page 0, read and left out
@@ -188,19 +199,19 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(AttnArgs a) {
         return ((there(page) ? page : 0) * a.page_stride + (first & ((1 << a.shift) - 1)) * a.token_stride) * 2;
     };
     auto last_row = [&](int base, int h) { return min(stop - 1 - min(base + 16 * h, final16), 15); };
-    auto load_k = [&](int base, const int (&page)[2]) {
+    auto load_k = [&](int base, int2 page) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const char* src = kh + offset(base, h, page[h]);
+            const char* src = kh + offset(base, h, h ? page.y : page.x);
             const uint32_t lane_off = min(c16, last_row(base, h)) * token_bytes + 16 * g4;
 #pragma unroll
             for (int s = 0; s < KS; ++s) kf[h][s] = *reinterpret_cast<const u4*>(src + (lane_off + 64 * s));
         }
     };
-    auto load_v = [&](int base, const int (&page)[2]) {
+    auto load_v = [&](int base, int2 page) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const char* src = vh + offset(base, h, page[h]);
+            const char* src = vh + offset(base, h, h ? page.y : page.x);
             const int last = last_row(base, h);
 #pragma unroll
             for (int j = 0; j < VJ / 2; ++j)  // chunk lane % C of row lane / C + j (64 / C)
@@ -208,10 +219,9 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(AttnArgs a) {
                     src + (min(lane / C + j * (64 / C), last) * token_bytes + 16 * (lane % C)));
         }
     };
-    auto block = [&](int base, const int (&now_page)[2], int (&next_page)[2], auto more) {
-        constexpr bool kMore = decltype(more)::value;
-        const int absent = (there(now_page[0]) ? 0 : 1) | (there(now_page[1]) ? 0 : 2);
-        const bool masked = absent || base + 32 > min(low + 1, stop);
+    auto block = [&](int base, int2 page, int2 next, auto more, auto careful) {
+        constexpr bool kMore = decltype(more)::value, kMasked = decltype(careful)::value;
+        const int absent = (there(page.x) ? 0 : 1) | (there(page.y) ? 0 : 2);
         f4 s[MT][2];
 #pragma unroll
         for (int m = 0; m < MT; ++m) s[m][0] = s[m][1] = f4{0, 0, 0, 0};
@@ -222,11 +232,11 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(AttnArgs a) {
                 s[m][0] = mma16<T>(kf[0][i], q[m][i], s[m][0]);
                 s[m][1] = mma16<T>(kf[1][i], q[m][i], s[m][1]);
             }
-        if constexpr (kMore) load_k(base + 128, next_page);
+        if constexpr (kMore) load_k(base + 128, next);
         // A probability of zero does not take an infinity or NaN away: where some row does not see a key, such values are left out
         // of the product and added to the rows that see them.
         bool odd = false;
-        if (masked) {
+        if constexpr (kMasked) {
 #pragma unroll
             for (int j = 0; j < VJ; ++j)
 #pragma unroll
@@ -235,7 +245,7 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(AttnArgs a) {
         }
 #pragma unroll
         for (int j = 0; j < VJ; ++j) vt[v_chunk<D>(lane / C + j * (64 / C), lane % C)] = vf[j];
-        if constexpr (kMore) load_v(base + 128, next_page);
+        if constexpr (kMore) load_v(base + 128, next);
 
         u4 p[MT];
 #pragma unroll
@@ -243,7 +253,7 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(AttnArgs a) {
             float x[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = s[m][i >> 2][i & 3] * a.scale;
-            if (masked) {
+            if constexpr (kMasked) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const int key = base + 16 * (i >> 2) + 4 * g4 + (i & 3);
@@ -271,7 +281,7 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(AttnArgs a) {
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
-        if (odd) {
+        if (kMasked && odd) {
 #pragma unroll 1
             for (int key = 0; key < 32; ++key)
 #pragma unroll
@@ -295,34 +305,30 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(AttnArgs a) {
             const int r = 4 * g4 + (c16 >> 2), c = 2 * d + ((c16 & 3) >> 1), half = (c16 & 1) * 8;
             const u2 lo = read_tr(vt, v_chunk<D>(r, c) * 16 + half), hi = read_tr(vt, v_chunk<D>(r + 16, c) * 16 + half);
             u4 w = u4{lo.x, lo.y, hi.x, hi.y};
-            if (odd) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if ((w[i] & kExponent) == kExponent) w[i] &= 0xFFFF0000u;
-                    if (((w[i] >> 16) & kExponent) == kExponent) w[i] &= 0xFFFFu;
-                }
-            }
+            if (kMasked && odd) w = read_odd_free(w, kExponent);
 #pragma unroll
             for (int m = 0; m < MT; ++m) o[m][d] = mma16<T>(w, p[m], o[m][d]);
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
         __builtin_amdgcn_wave_barrier();
     };
+    // Blocks that every row sees whole come first and run without a mask; from the first one that some row does not (or a page
+    // that is none) on, all are masked.
     int base = begin + 32 * wave;
     if (base < stop) {
-        int now_page[2], next_page[2];
-        pages(base, now_page);
-        load_k(base, now_page);
-        load_v(base, now_page);
-        pages(min(base + 128, final16), next_page);
-        for (; base + 128 < stop; base += 128) {
-            int after[2];
-            pages(min(base + 256, final16), after);
-            block(base, now_page, next_page, std::true_type());
-#pragma unroll
-            for (int h = 0; h < 2; ++h) now_page[h] = next_page[h], next_page[h] = after[h];
-        }
-        block(base, now_page, next_page, std::false_type());
+        int2 page = pages(base), next = pages(min(base + 128, final16));
+        load_k(base, page);
+        load_v(base, page);
+        const int clear = min(low + 1, stop);
+        auto step = [&](auto careful) {
+            const int2 after = pages(min(base + 256, final16));
+            block(base, page, next, std::true_type(), careful);
+            page = next, next = after;
+            base += 128;
+        };
+        while (base + 128 < stop && base + 32 <= clear && there(page.x) && there(page.y)) step(std::false_type());
+        while (base + 128 < stop) step(std::true_type());
+        block(base, page, next, std::false_type(), std::true_type());
     }
 
     // the four wavefronts' results become one, 16 rows at a time through LDS
@@ -439,17 +445,6 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(AttnArgs a) {
             *reinterpret_cast<u2*>(dst) = *reinterpret_cast<const u2*>(y);
         }
     }
-}
-
-typedef const __attribute__((address_space(4))) int32_t const_int;
-
-__device__ __forceinline__ u4 read_odd_free(u4 w, uint32_t exponent) {  // infinities and NaN of 16-bit halves as zero
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if ((w[i] & exponent) == exponent) w[i] &= 0xFFFF0000u;
-        if (((w[i] >> 16) & exponent) == exponent) w[i] &= 0xFFFFu;
-    }
-    return w;
 }
 
 template <typename T>
