@@ -41,8 +41,8 @@ struct AttnArgs {
     int tokens, batch, heads, kv_heads, group, num_pages, width, shift, splits, part_rows;
 };
 
-constexpr int kTileFloats = 2;  // per row beside its D sums: maximum and sum
-constexpr int kMinKeys = 128, kPerCu = 8;
+constexpr int kTileFloats = 4;  // per row of a partial result beside its D sums: maximum, sum, and two that keep rows 16-byte aligned
+constexpr int kMinKeys = 128, kLongKeys = 2048;
 
 // A tile of rows: its request, first row, and the keys it can see.
 struct Tile {
@@ -215,8 +215,8 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(AttnArgs a) {
             const int last = last_row(base, h);
 #pragma unroll
             for (int j = 0; j < VJ / 2; ++j)  // chunk lane % C of row lane / C + j (64 / C)
-                vf[h * (VJ / 2) + j] = *reinterpret_cast<const u4*>(
-                    src + (min(lane / C + j * (64 / C), last) * token_bytes + 16 * (lane % C)));
+                vf[h * (VJ / 2) + j] = __builtin_nontemporal_load(reinterpret_cast<const u4*>(
+                    src + (min(lane / C + j * (64 / C), last) * token_bytes + 16 * (lane % C))));
         }
     };
     auto block = [&](int base, int2 page, int2 next, auto more, auto careful) {
@@ -367,16 +367,16 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(AttnArgs a) {
         }
     }
     if (parts > 1) {
-        // [unit][split][row][D + 2]: the sums, then maximum and sum; rows that are there only
+        // [unit][split][row][D + 4]: the sums, then maximum and sum; rows that are there only
         const int64_t mine = (static_cast<int64_t>(unit) * a.splits + split) * a.part_rows;
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             if (16 * m + row >= t.rows) continue;
             const int to = static_cast<int>((mine + 16 * m + row) * kRowFloats * 4);
 #pragma unroll
-            for (int i = 0; i < PER; i += 2)
-                __builtin_amdgcn_raw_buffer_store_b64(u2{__float_as_uint(res[m][i]), __float_as_uint(res[m][i + 1])}, rs,
-                                                      to + (col + i) * 4, 0, kCoherentAux);
+            for (int i = 0; i < PER; i += 4)
+                __builtin_amdgcn_raw_buffer_store_b128(bitcast<u4>(f4{res[m][i], res[m][i + 1], res[m][i + 2], res[m][i + 3]}), rs,
+                                                       to + (col + i) * 4, 0, kCoherentAux);
             if (col == 0)
                 __builtin_amdgcn_raw_buffer_store_b64(u2{__float_as_uint(rtop[m]), __float_as_uint(rsum[m])}, rs, to + D * 4, 0,
                                                       kCoherentAux);
@@ -387,44 +387,63 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(AttnArgs a) {
             last_flag = __hip_atomic_fetch_add(a.locks + unit, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
         __syncthreads();
         if (!last_flag) return;
+        // Of the 16 rows' threads those of rows that are not there help with the others: 16 / R groups of R rows (R a power of two) take
+        // every (16 / R)-th part, eight of them in flight, and are added in order.
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-            if (16 * m + row >= t.rows) continue;
-            rtop[m] = kNone, rsum[m] = 0.0f;
+            const int have = min(t.rows - 16 * m, 16);
+            if (have <= 0) break;
+            const int bits = have > 8 ? 4 : have > 4 ? 3 : have > 2 ? 2 : have - 1;
+            const int jrow = min(row & ((1 << bits) - 1), have - 1), group = row >> bits, groups = 16 >> bits;
+            float jtop = kNone, jsum = 0.0f, jres[PER];
 #pragma unroll
-            for (int i = 0; i < PER; ++i) res[m][i] = 0.0f;
-            constexpr int VB = 8;  // parts in flight
-            for (int s0 = 0; s0 < parts; s0 += VB) {
-                u2 ms[VB], x[VB][PER / 2];
+            for (int i = 0; i < PER; ++i) jres[i] = 0.0f;
+            constexpr int VB = 8;
+            for (int s0 = group; s0 < parts; s0 += VB * groups) {
+                u2 ms[VB];
+                f4 x[VB][PER / 4];
 #pragma unroll
                 for (int v = 0; v < VB; ++v) {
-                    const int s = min(s0 + v, parts - 1);  // past the last: read again, not added
+                    const int s = min(s0 + v * groups, parts - 1);  // past the last: read again, not added
                     const int from = static_cast<int>(
-                        ((static_cast<int64_t>(unit) * a.splits + s) * a.part_rows + 16 * m + row) * kRowFloats * 4);
+                        ((static_cast<int64_t>(unit) * a.splits + s) * a.part_rows + 16 * m + jrow) * kRowFloats * 4);
                     ms[v] = bitcast<u2>(__builtin_amdgcn_raw_buffer_load_b64(rs, from + D * 4, 0, kCoherentAux));
 #pragma unroll
-                    for (int i = 0; i < PER / 2; ++i)
-                        x[v][i] = bitcast<u2>(__builtin_amdgcn_raw_buffer_load_b64(rs, from + (col + 2 * i) * 4, 0, kCoherentAux));
+                    for (int i = 0; i < PER / 4; ++i)
+                        x[v][i] = bitcast<f4>(__builtin_amdgcn_raw_buffer_load_b128(rs, from + (col + 4 * i) * 4, 0, kCoherentAux));
                 }
-                float now = rtop[m];
+                float now = jtop;
 #pragma unroll
                 for (int v = 0; v < VB; ++v) now = fmaxf(now, __uint_as_float(ms[v].x));
-                const float zero = now == kNone ? 0.0f : now, keep = __builtin_amdgcn_exp2f(rtop[m] - zero);
-                rtop[m] = now;
-                rsum[m] *= keep;
+                const float zero = now == kNone ? 0.0f : now, keep = __builtin_amdgcn_exp2f(jtop - zero);
+                jtop = now;
+                jsum *= keep;
 #pragma unroll
-                for (int i = 0; i < PER; ++i) res[m][i] *= keep;
+                for (int i = 0; i < PER; ++i) jres[i] *= keep;
 #pragma unroll
                 for (int v = 0; v < VB; ++v) {
-                    if (s0 + v >= parts) break;
+                    if (s0 + v * groups >= parts) break;
                     const float f = __builtin_amdgcn_exp2f(__uint_as_float(ms[v].x) - zero);
-                    rsum[m] += f * __uint_as_float(ms[v].y);
+                    jsum += f * __uint_as_float(ms[v].y);
 #pragma unroll
-                    for (int i = 0; i < PER / 2; ++i) {
-                        res[m][2 * i] += f * __uint_as_float(x[v][i].x);
-                        res[m][2 * i + 1] += f * __uint_as_float(x[v][i].y);
-                    }
+                    for (int i = 0; i < PER; ++i) jres[i] += f * x[v][i >> 2][i & 3];
                 }
+            }
+            __syncthreads();
+            if ((threadIdx.x & 15) == 0) stat[0][0][row] = jtop, stat[1][0][row] = jsum;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) od[row * D + col + i] = jres[i];
+            __syncthreads();
+            rtop[m] = kNone, rsum[m] = 0.0f;
+            for (int g = 0; g < groups; ++g) rtop[m] = fmaxf(rtop[m], stat[0][0][(g << bits) + jrow]);
+            const float zero = rtop[m] == kNone ? 0.0f : rtop[m];
+#pragma unroll
+            for (int i = 0; i < PER; ++i) res[m][i] = 0.0f;
+            for (int g = 0; g < groups; ++g) {
+                const float f = __builtin_amdgcn_exp2f(stat[0][0][(g << bits) + jrow] - zero);
+                rsum[m] += f * stat[1][0][(g << bits) + jrow];
+#pragma unroll
+                for (int i = 0; i < PER; ++i) res[m][i] += f * od[((g << bits) + jrow) * D + col + i];
             }
         }
         if (threadIdx.x == 0) __hip_atomic_store(a.locks + unit, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -665,7 +684,7 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {
         sum = __uint_as_float(x[0]) + __uint_as_float(x[1]);
     }
     if (parts > 1) {
-        // [unit][split][row][D + 2]: the sums, then maximum and sum
+        // [unit][split][row][D + 4]: the sums, then maximum and sum
         const int unit = slot * a.kv_heads + head;
         constexpr int kRowFloats = D + kTileFloats;
         const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(a.ws, 0, 0x7FFFFFFF, kBufferFlags);
@@ -675,9 +694,9 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
-                for (int i = 0; i < 16; i += 2)
-                    __builtin_amdgcn_raw_buffer_store_b64(u2{__float_as_uint(o[d][i]), __float_as_uint(o[d][i + 1])}, rs,
-                                                          to + (32 * d + 8 * (i >> 2) + 4 * h + (i & 3)) * 4, 0, kCoherentAux);
+                for (int i = 0; i < 16; i += 4)
+                    __builtin_amdgcn_raw_buffer_store_b128(bitcast<u4>(f4{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]}), rs,
+                                                           to + (32 * d + 2 * i + 4 * h) * 4, 0, kCoherentAux);
             if (h == 0)
                 __builtin_amdgcn_raw_buffer_store_b64(u2{__float_as_uint(top), __float_as_uint(sum)}, rs, to + D * 4, 0, kCoherentAux);
         }
@@ -697,11 +716,10 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {
             for (int s = 0; s < parts; ++s) {
                 const int from = static_cast<int>((first_row + static_cast<int64_t>(s) * a.part_rows) * kRowFloats * 4);
                 const u2 ms = bitcast<u2>(__builtin_amdgcn_raw_buffer_load_b64(rs, from + D * 4, 0, kCoherentAux));
-                u2 x[8 * DT];
+                f4 x[4 * DT];
 #pragma unroll
-                for (int i = 0; i < 8 * DT; ++i)
-                    x[i] = bitcast<u2>(__builtin_amdgcn_raw_buffer_load_b64(
-                        rs, from + (8 * (i >> 1) + 4 * h + 2 * (i & 1)) * 4, 0, kCoherentAux));
+                for (int i = 0; i < 4 * DT; ++i)
+                    x[i] = bitcast<f4>(__builtin_amdgcn_raw_buffer_load_b128(rs, from + (8 * i + 4 * h) * 4, 0, kCoherentAux));
                 const float other = __uint_as_float(ms.x), now = fmaxf(top, other), zero = now == kNone ? 0.0f : now;
                 const float keep = __builtin_amdgcn_exp2f(top - zero), f = __builtin_amdgcn_exp2f(other - zero);
                 top = now;
@@ -709,10 +727,7 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {
 #pragma unroll
                 for (int d = 0; d < DT; ++d)
 #pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        o[d][i] = o[d][i] * keep + f * __uint_as_float(x[8 * d + (i >> 1)].x);
-                        o[d][i + 1] = o[d][i + 1] * keep + f * __uint_as_float(x[8 * d + (i >> 1)].y);
-                    }
+                    for (int i = 0; i < 16; ++i) o[d][i] = o[d][i] * keep + f * x[4 * d + (i >> 2)][i & 3];
             }
         }
         if (threadIdx.x == 0) __hip_atomic_store(a.locks + unit, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -770,12 +785,13 @@ extern "C" int tw4_paged_attention_plan(int tokens, int batch, int heads, int kv
     const int64_t units = tile_slots(tokens, batch, group, rows, single) * kv_heads;
     const int64_t part = static_cast<int64_t>(single ? std::min(rows, group) : rows) * (head_dim + kTileFloats);
     int64_t splits = 1;
-    if (units > 0 && units < kPerCu * cus) {
-        splits = (kPerCu * cus + units - 1) / units;
-        splits = std::min<int64_t>(splits, (static_cast<int64_t>(max_keys) + kMinKeys - 1) / kMinKeys);
-        splits = std::min<int64_t>(splits, kWorkspaceFloats / (units * part));
-        splits = std::max<int64_t>(splits, 1);
+    for (int per_cu = 2; units > 0 && per_cu <= 4; per_cu *= 2) {
+        splits = std::max<int64_t>((per_cu * cus + units / 2) / units, 1);
+        if (max_keys <= kLongKeys * splits) break;
     }
+    splits = std::min<int64_t>(splits, (static_cast<int64_t>(max_keys) + kMinKeys - 1) / kMinKeys);
+    if (units > 0) splits = std::min<int64_t>(splits, kWorkspaceFloats / (units * part));
+    splits = std::max<int64_t>(splits, 1);
     out[0] = rows;
     out[1] = static_cast<int>(splits);
     out[2] = splits > 1 ? static_cast<int>(units * splits * part) : 0;
