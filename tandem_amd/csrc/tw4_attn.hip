@@ -474,15 +474,17 @@ __device__ __forceinline__ f16v mma32(const u4& a, const u4& b, const f16v& c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(bitcast<bf8>(a), bitcast<bf8>(b), c, 0, 0, 0);
 }
 
-// Chunk kernel: a tile of 128 rows, 32 for each of four wavefronts; K and V in tiles of 64 keys through LDS by direct loads, two
-// stages: while a tile is computed the next one is on its way. A wavefront fetches 16 keys of each tile, which lie in one page.
+// Chunk kernel: a tile of 128 rows, 32 for each of four wavefronts; K and V in tiles of 64 keys through LDS by direct loads, two stages
+// each: while a tile is computed the next one is on its way. A wavefront fetches 16 keys of each tile, which lie in one page. Two workgroups
+// share a CU, and their wavefronts' products and exponentials fill each other's time. A wavefront issues one instruction in four cycles,
+// whatever its kind, so the loop over unmasked tiles computes no address: a lane's places change stage by a bit.
 // Lane (c, h) = (lane % 32, lane / 32): scores S^T of row c, keys 8 (i / 4) + 4 h + i % 4 of 32.
 template <typename T, int D>
 __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {
-    constexpr int B = 128, KEYS = 64, C = D / 8, KS = D / 16, DT = D / 32, ROWS = 64 / C, NJ = 16 / ROWS;  // ROWS of a 1 KB load
-    constexpr int TILE = KEYS * C;                                                                          // 16-byte chunks of a tile
+    constexpr int NQ = 1, B = 128 * NQ, KEYS = 64, C = D / 8, KS = D / 16, DT = D / 32, ROWS = 64 / C, NJ = 16 / ROWS;  // ROWS of a 1 KB load
+    constexpr int TILE = KEYS * C;                                                                               // 16-byte chunks of a tile
     constexpr uint32_t kExponent = __is_same(T, h1) ? 0x7C00u : 0x7F80u;
-    __shared__ u4 lds[2 * 2 * TILE];  // [stage][K, V][key][chunk]
+    __shared__ u4 lds[2 * 2 * TILE];  // K [stage][key][chunk], V alike
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c32 = lane & 31, h = lane >> 5;
     // the last rows of a prompt see the most keys: they go first
     const int slot = static_cast<int>(gridDim.x / a.kv_heads) - 1 - blockIdx.x / a.kv_heads, head = blockIdx.x % a.kv_heads;
@@ -490,19 +492,20 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {
     Tile t;
     if (!find_tile<B>(a, slot, lane, t)) return;
 
-    const int r = t.first + 32 * wave + c32, tok = r / a.group;
-    const bool mine = 32 * wave + c32 < t.rows;
-    const int limit = mine ? t.len - t.fresh + tok : -1;
-    u4 q[KS];
-    {
+    int limit[NQ];
+    bool mine[NQ];
+    u4 q[NQ][KS];
+#pragma unroll
+    for (int m = 0; m < NQ; ++m) {
+        const int at = 32 * (NQ * wave + m) + c32, r = t.first + at, tok = r / a.group;
+        mine[m] = at < t.rows;
+        limit[m] = mine[m] ? t.len - t.fresh + tok : -1;
         const uint16_t* src = a.q + (t.start + tok) * a.q_token + (head * a.group + r - tok * a.group) * a.q_head + 8 * h;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) q[s] = mine ? *reinterpret_cast<const u4*>(src + 16 * s) : u4{0, 0, 0, 0};
+        for (int s = 0; s < KS; ++s) q[m][s] = mine[m] ? *reinterpret_cast<const u4*>(src + 16 * s) : u4{0, 0, 0, 0};
     }
-    // the last keys that the wavefront's rows and the tile's see
-    const int rows_here = min(t.rows - 32 * wave, 32);  // <= 0: none
-    const int high = rows_here > 0 ? t.len - t.fresh + (t.first + 32 * wave + rows_here - 1) / a.group : -1;
-    const int tile_high = t.len - t.fresh + (t.first + min(t.rows, B) - 1) / a.group;
+    const bool active = 32 * NQ * wave < t.rows;  // this wavefront has a row
+    const int tile_high = t.len - t.fresh + (t.first + min(t.rows, B) - 1) / a.group;  // the last key a row of the tile sees
     const int end = static_cast<int>(min(static_cast<int64_t>(tile_high) + 1, static_cast<int64_t>(a.width) << a.shift));
     int begin = 0, stop = max(end, 0), parts = 1;
     if (a.splits > 1 && end > 0) {
@@ -515,12 +518,16 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {
         return;
     }
 
-    f16v o[DT];
+    f16v o[NQ][DT];
+    float top[NQ], sum[NQ];
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
+    for (int m = 0; m < NQ; ++m) {
+        top[m] = kNone, sum[m] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
-    float top = kNone, sum = 0.0f;
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[m][d][i] = 0.0f;
+    }
 
     const_int* table = (const_int*)(a.table + t.request * a.table_stride);
     const uint16_t* kh = a.k + head * a.head_stride;
@@ -531,174 +538,308 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {
     // where chunk c of key r lies in a tile: places of 16 bytes such that the reads below meet every bank once
     auto k_place = [](int row, int c) { return c ^ (D == 128 ? row & 15 : (row >> 1) & 7); };
     auto v_place = [](int row, int c) { return c ^ (D == 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2); };
-    // the pages of a tile's four sixteens
-    typedef int i4 __attribute__((ext_vector_type(4)));
-    auto entries = [&](int key) {
-        auto one = [&](int k) { return static_cast<int>(table[min(k, final16) >> a.shift]); };
-        return i4{one(key), one(key + 16), one(key + 32), one(key + 48)};
-    };
     auto there = [&](int page) { return static_cast<uint32_t>(page) < static_cast<uint32_t>(a.num_pages); };
-    auto fetch = [&](int key, i4 pages, int stage) {  // keys key + 16 wave .. + 15 into a stage
-        const int first = min(key + 16 * wave, final16), last = min(stop - 1 - first, 15);
-        const int page = __builtin_amdgcn_readfirstlane(wave < 2 ? (wave < 1 ? pages.x : pages.y) : (wave < 3 ? pages.z : pages.w));
-        const int64_t at = (there(page) ? page : 0) * a.page_stride + (first & ((1 << a.shift) - 1)) * a.token_stride;
-        const u4 kr = lds_rsrc(kh + at), vr = lds_rsrc(vh + at);
-        const uint32_t to = lds_base + stage * (2 * TILE * 16) + wave * (16 * C * 16);
+    auto entry = [&](int key) { return static_cast<int>(table[min(key, final16) >> a.shift]); };
+    // offset of this wavefront's 16 keys of the tile at `key`, in values; a page the table does not have is page 0, read and left out
+    auto place_of = [&](int key, int page) {
+        const int first = min(key + 16 * wave, final16);
+        return (there(page) ? page : 0) * a.page_stride + (first & ((1 << a.shift) - 1)) * a.token_stride;
+    };
+    // What a lane loads of 16 whole keys; K's chunks change places with all of the row's number, V's with the part of it that every
+    // load of a lane has.
+    uint32_t k_from[NJ];
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            const int row = j * ROWS + lane / C;
-            const uint32_t from = min(row, last) * token_bytes;
-            lds_dma16<0>(kr, from + 16 * k_place(row, lane % C), 0, to + j * 1024);
-            lds_dma16<0>(vr, from + 16 * v_place(row, lane % C), 0, to + TILE * 16 + j * 1024);
+    for (int e = 0; e < NJ; ++e)
+        k_from[e] = (e * ROWS + lane / C) * token_bytes + 16 * k_place(e * ROWS + lane / C, lane % C);
+    const uint32_t v_from = lane / C * token_bytes + 16 * v_place(lane / C, lane % C);
+    uint32_t to = __builtin_amdgcn_readfirstlane(lds_base + wave * (16 * C * 16));  // the place in K's stage, V's 2 tiles on
+    // keys key + 16 wave .. + 15 into a stage; past the last key its values again, which nothing sees
+    auto fetch_k = [&](int key, int64_t at) {
+        const u4 rs = lds_rsrc(kh + at);
+        const int last = stop - 1 - min(key + 16 * wave, final16);
+        uint32_t from[NJ];
+#pragma unroll
+        for (int e = 0; e < NJ; ++e) from[e] = k_from[e];
+        if (last < 15) {
+#pragma unroll
+            for (int e = 0; e < NJ; ++e) {
+                const int row = e * ROWS + lane / C;
+                from[e] = min(row, last) * token_bytes + 16 * k_place(row, lane % C);
+            }
+        }
+        lds_dma16<0>(rs, from[0], 0, to);
+        lds_dma16<1024>(rs, from[1], 0, to);
+        if constexpr (NJ == 4) {
+            lds_dma16<2048>(rs, from[2], 0, to);
+            lds_dma16<3072>(rs, from[3], 0, to);
+        }
+    };
+    auto fetch_v = [&](int key, int64_t at) {
+        constexpr int S = 2 * TILE * 16;
+        const u4 rs = lds_rsrc(vh + at);
+        const int last = stop - 1 - min(key + 16 * wave, final16);
+        if (last < 15) {
+            auto from = [&](int e) {
+                return static_cast<uint32_t>(min(e * ROWS + lane / C, last)) * token_bytes + 16 * v_place(lane / C, lane % C);
+            };
+            lds_dma16<S>(rs, from(0), 0, to);
+            lds_dma16<S + 1024>(rs, from(1), 0, to);
+            if constexpr (NJ == 4) {
+                lds_dma16<S + 2048>(rs, from(2), 0, to);
+                lds_dma16<S + 3072>(rs, from(3), 0, to);
+            }
+            return;
+        }
+        lds_dma16<S>(rs, v_from, 0, to);
+        lds_dma16<S + 1024>(rs, v_from, ROWS * token_bytes, to);
+        if constexpr (NJ == 4) {
+            lds_dma16<S + 2048>(rs, v_from, 2 * ROWS * token_bytes, to);
+            lds_dma16<S + 3072>(rs, v_from, 3 * ROWS * token_bytes, to);
         }
     };
 
-    // Table entries are read two tiles before their keys are used, keys one tile before.
-    int stage = 0, absent = 0;
-    i4 next = i4{0, 0, 0, 0};
-    auto absent_of = [&](i4 page) {
-        return (there(page.x) ? 0 : 1) | (there(page.y) ? 0 : 2) | (there(page.z) ? 0 : 4) | (there(page.w) ? 0 : 8);
-    };
-    if (begin < stop) {
-        const i4 page = entries(begin);
-        next = entries(min(begin + KEYS, final16));
-        fetch(begin, page, 0);
-        absent = absent_of(page);
-    }
     const int g = (lane >> 4) & 1, i16 = lane & 15;
-    auto tile = [&](int base, auto masked) {
-        constexpr bool kMasked = decltype(masked)::value;
-        wait_stage<0>();
-        ring_barrier();
-        const int gone = absent;
-        absent = absent_of(next);
-        if (base + KEYS < stop) fetch(base + KEYS, next, stage ^ 1);
-        next = entries(min(base + 2 * KEYS, final16));
-        const u4* kt = lds + stage * 2 * TILE;
-        const u4* vt = kt + TILE;
-        stage ^= 1;
-        if (base > high) return;  // none of this wavefront's rows sees the tile
-        f16v s[2];
+    // a lane's places in LDS: chunk 2 s + h of key c; 16 keys' 8 (j / 4) + 4 h + j % 4 in place 8 h + j, values 32 d ..
+    int k_lane[KS], v_lane[DT];
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+    for (int e = 0; e < KS; ++e) k_lane[e] = (c32 * C + k_place(c32, 2 * e + h)) * 16;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[n][i] = 0.0f;
+    for (int d = 0; d < DT; ++d) {
+        const int row = 4 * h + (i16 >> 2);
+        v_lane[d] = (2 * TILE + row * C + v_place(row, 4 * d + 2 * g + ((i16 & 3) >> 1))) * 16 + (i16 & 1) * 8;
+    }
+    auto read_k = [&](int e) {  // step e / 2 of keys 32 (e % 2) ..
+        return *reinterpret_cast<const u4*>(reinterpret_cast<const char*>(lds) + k_lane[e >> 1] + (e & 1) * (32 * C * 16));
+    };
+    auto read_v = [&](int e) {  // keys 16 (e / DT) .., values 32 (e % DT) ..
+        const int at = v_lane[e % DT] + (e / DT) * (16 * C * 16);
+        const u2 lo = read_tr(lds, at), hi = read_tr(lds, at + 8 * C * 16);
+        return u4{lo.x, lo.y, hi.x, hi.y};
+    };
+    const f16v none = {};
+    f16v s[NQ][2];
+    auto scores = [&] {
+        u4 k[2 * KS];
+        constexpr int KA = 6;  // reads ahead of their products
 #pragma unroll
-        for (int i = 0; i < KS; ++i)
+        for (int e = 0; e < KA; ++e) k[e] = read_k(e);
 #pragma unroll
-            for (int n = 0; n < 2; ++n) s[n] = mma32<T>(kt[(32 * n + c32) * C + k_place(c32, 2 * i + h)], q[i], s[n]);
-        // six reads ahead of the products that use them
-        __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+        for (int e = 0; e < 2 * KS; ++e) {
+            if (e + KA < 2 * KS) k[e + KA] = read_k(e + KA);
 #pragma unroll
-        for (int i = 0; i < 2 * KS - 6; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            for (int m = 0; m < NQ; ++m) s[m][e & 1] = mma32<T>(k[e], q[m][e >> 1], e < 2 ? none : s[m][e & 1]);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        __builtin_amdgcn_sched_group_barrier(0x008, 6, 0);
-        bool odd = false;
-        if constexpr (kMasked) {
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int key = 32 * n + 8 * (i >> 2) + 4 * h + (i & 3);
-                    if (base + key > min(limit, stop - 1) || (gone >> (key >> 4) & 1)) s[n][i] = kNone;
-                }
-            // A probability of zero does not take an infinity or NaN away: where some row does not see a key, such values are
-            // left out of the product and added to the rows that see them.
-#pragma unroll 2
-            for (int j = 0; j < TILE / 64; ++j) {
-                const u4 w = vt[64 * j + lane];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) odd |= odd16(w[i], kExponent);
-            }
-            odd = __ballot(odd) != 0;
-        }
+    };
+    auto best_of = [&](const f16v (&s)[2]) {
         float best = s[0][0];
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int i = 0; i < 16; ++i) best = fmaxf(best, s[n][i]);
-        {
-            const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(best), __float_as_uint(best), false, false);
-            best = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * a.scale;
-        }
-        // The sums are scaled to a new maximum only when it is more than 2^8 times the old: probabilities up to 256 instead of 1
-        // are as exact, and most tiles need no pass over the sums.
-        if (__ballot(best > top + 8.0f)) {
-            const float now = fmaxf(top, best), keep = __builtin_amdgcn_exp2f(top - (now == kNone ? 0.0f : now));
-            top = now;
-            sum *= keep;
+        const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(best), __float_as_uint(best), false, false);
+        return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * a.scale;
+    };
+    // The sums are scaled to a new maximum only when it is more than 2^8 times the old: probabilities up to 256 instead of 1 are as
+    // exact, and most tiles need no pass over the sums.
+    auto raise = [&](const float (&best)[NQ]) {
+        bool any = false;
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
+        for (int m = 0; m < NQ; ++m) any |= best[m] > top[m] + 8.0f;
+        if (__ballot(any)) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) o[d][i] *= keep;
-        }
-        const float zero = top == kNone ? 0.0f : top;  // a row that has seen nothing yet
-        if (kMasked && odd) {
-#pragma unroll 1
-            for (int key = 0; key < KEYS; ++key) {
-                if (base + key > min(limit, stop - 1) || (gone >> (key >> 4) & 1)) continue;
+            for (int m = 0; m < NQ; ++m) {
+                const float now = fmaxf(top[m], best[m]), keep = __builtin_amdgcn_exp2f(top[m] - (now == kNone ? 0.0f : now));
+                top[m] = now;
+                sum[m] *= keep;
 #pragma unroll
-                for (int i = 0; i < 4 * DT; ++i) {  // four values from 8 i + 4 h on
-                    const u2 four = *reinterpret_cast<const u2*>(reinterpret_cast<const char*>(vt) +
-                                                                 (key * C + v_place(key, i)) * 16 + h * 8);
+                for (int d = 0; d < DT; ++d)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const uint16_t bits = static_cast<uint16_t>(four[e >> 1] >> (16 * (e & 1)));
-                        if ((bits & kExponent) == kExponent) o[i >> 2][4 * (i & 3) + e] += static_cast<float>(bitcast<T>(bits));
-                    }
-                    __builtin_amdgcn_sched_barrier(0);  // one at a time: the rare path is not to take registers
-                }
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {  // 16 keys: 16 u + 8 (j / 4) + 4 h + j % 4 in place 8 h + j
-            float x[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u >> 1][8 * (u & 1) + i], a.scale, -zero));
-                sum += x[i];
-            }
-            const u4 p = from_f32<T>(x);
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                const int row = 16 * u + 4 * h + (i16 >> 2);
-                const int at = (row * C + v_place(row, 4 * d + 2 * g + ((i16 & 3) >> 1))) * 16 + (i16 & 1) * 8;
-                const u2 lo = read_tr(vt, at), hi = read_tr(vt, at + 8 * C * 16);
-                u4 w = u4{lo.x, lo.y, hi.x, hi.y};
-                if (kMasked && odd) w = read_odd_free(w, kExponent);
-                o[d] = mma32<T>(w, p, o[d]);
+                    for (int i = 0; i < 16; ++i) o[m][d][i] *= keep;
             }
         }
     };
-    // Tiles that every row sees whole come first and run without a mask; from the first one that some row does not (or a page
-    // that is none) on, all are masked.
-    const int clear = min(t.len - t.fresh + t.first / a.group + 1, stop);
-    int base = begin;
-    for (; base + KEYS <= clear && !absent; base += KEYS) tile(base, std::false_type());
-    for (; base < stop; base += KEYS) tile(base, std::true_type());
+    // four probabilities, of keys 16 u + 8 x + 4 h ..
+    auto weights = [&](const f16v (&s)[NQ][2], int m, int u, int x, float zero) {
+        f4 w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[m][u >> 1][8 * (u & 1) + 4 * x + i], a.scale, -zero));
+            sum[m] += w[i];
+        }
+        return w;
+    };
+    auto pack = [](const f4& x, const f4& y) {
+        const float w[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+        return from_f32<T>(w);
+    };
 
-    {
-        const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
-        sum = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+    // Keys below `clear` are seen by every row and lie in pages that are there.
+    int clear = min(t.len - t.fresh + t.first / a.group + 1, stop);
+    int ahead = 0;  // the table's entry of this wavefront's keys of the next tile
+    if (begin < stop) {
+        const int64_t at = place_of(begin, entry(begin + 16 * wave));
+        ahead = entry(begin + KEYS + 16 * wave);
+        fetch_k(begin, at);
+        fetch_v(begin, at);
+        int* first_gone = reinterpret_cast<int*>(lds + TILE);  // the second stage is not in use yet
+        if (threadIdx.x == 0) *first_gone = 0x7FFFFFFF;
+        __syncthreads();
+        const int e1 = (stop - 1) >> a.shift;
+        int gone = 0x7FFFFFFF;
+#pragma unroll 4
+        for (int e = (begin >> a.shift) + static_cast<int>(threadIdx.x); e <= e1; e += 256)
+            if (!there(a.table[t.request * a.table_stride + e])) gone = min(gone, e << a.shift);
+        if (gone != 0x7FFFFFFF) atomicMin(first_gone, gone);
+        __syncthreads();
+        clear = min(clear, __builtin_amdgcn_readfirstlane(*first_gone));
+    }
+    // Start of the tile at `key`: it has arrived, and the next one is sent for, into the place of the one before it.
+    auto turn = [&](int key) {
+        wait_stage<0>();
+        ring_barrier();
+        to ^= TILE * 16;
+        if (key + KEYS < stop) {
+            const int64_t at = place_of(key + KEYS, ahead);
+            fetch_k(key + KEYS, at);
+            fetch_v(key + KEYS, at);
+            ahead = entry(key + 2 * KEYS + 16 * wave);
+        }
+    };
+    auto other_stage = [&] {
+#pragma unroll
+        for (int e = 0; e < KS; ++e) k_lane[e] ^= TILE * 16;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) v_lane[d] ^= TILE * 16;
+    };
+    int base = begin;
+    for (; base + KEYS <= clear; base += KEYS) {
+        turn(base);  // a wavefront without rows goes along
+        scores();
+        u4 v[4 * DT];
+        constexpr int VA = DT;  // reads ahead of their products
+        float best[NQ];
+#pragma unroll
+        for (int m = 0; m < NQ; ++m) best[m] = best_of(s[m]);
+        raise(best);
+        const float zero = top[0] == kNone ? 0.0f : top[0];
+#pragma unroll
+        for (int e = 0; e < VA; ++e) v[e] = read_v(e);
+        f4 x = weights(s, 0, 0, 0, zero), y = weights(s, 0, 0, 1, zero);
+        u4 p = pack(x, y);
+        __builtin_amdgcn_sched_barrier(0);
+        // a step: the products of 16 keys beside the probabilities of the next 16
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const int e = u * DT + d;
+                if (e + VA < 4 * DT) v[e + VA] = read_v(e + VA);
+                o[0][d] = mma32<T>(v[e], p, o[0][d]);
+                if (u < 3 && d == 0) x = weights(s, 0, u + 1, 0, zero);
+                if (u < 3 && d == DT / 2) y = weights(s, 0, u + 1, 1, zero);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (u < 3) p = pack(x, y);
+        }
+        other_stage();
+    }
+    // From the first tile on that some row does not see whole, or that lies in a page that is none, all are masked.
+    for (; base < stop; base += KEYS) {
+        turn(base);
+        if (!active) continue;
+        scores();
+        const u4* vt = lds + (2 + ((base - begin) / KEYS & 1)) * TILE;
+        const int off = (there(entry(base)) ? 0 : 1) | (there(entry(base + 16)) ? 0 : 2) | (there(entry(base + 32)) ? 0 : 4) |
+                        (there(entry(base + 48)) ? 0 : 8);
+        bool odd = false;
+#pragma unroll
+        for (int m = 0; m < NQ; ++m)
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int key = 32 * n + 8 * (i >> 2) + 4 * h + (i & 3);
+                    if (base + key > min(limit[m], stop - 1) || (off >> (key >> 4) & 1)) s[m][n][i] = kNone;
+                }
+        // A probability of zero does not take an infinity or NaN away: where some row does not see a key, such values are left out
+        // of the product and added to the rows that see them.
+#pragma unroll 2
+        for (int e = 0; e < TILE / 64; ++e) {
+            const u4 w = vt[64 * e + lane];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) odd |= odd16(w[i], kExponent);
+        }
+        odd = __ballot(odd) != 0;
+        float best[NQ];
+#pragma unroll
+        for (int m = 0; m < NQ; ++m) best[m] = best_of(s[m]);
+        raise(best);
+        if (odd) {
+#pragma unroll 1
+            for (int key = 0; key < KEYS; ++key)
+#pragma unroll
+                for (int m = 0; m < NQ; ++m) {
+                    if (base + key > min(limit[m], stop - 1) || (off >> (key >> 4) & 1)) continue;
+#pragma unroll
+                    for (int i = 0; i < 4 * DT; ++i) {  // four values from 8 i + 4 h on
+                        const u2 four = *reinterpret_cast<const u2*>(reinterpret_cast<const char*>(vt) +
+                                                                     (key * C + v_place(key, i)) * 16 + h * 8);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint16_t bits = static_cast<uint16_t>(four[e >> 1] >> (16 * (e & 1)));
+                            if ((bits & kExponent) == kExponent)
+                                o[m][i >> 2][4 * (i & 3) + e] += static_cast<float>(bitcast<T>(bits));
+                        }
+                        __builtin_amdgcn_sched_barrier(0);  // one at a time: the rare path is not to take registers
+                    }
+                }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            u4 p[NQ];
+#pragma unroll
+            for (int m = 0; m < NQ; ++m) {
+                const float zero = top[m] == kNone ? 0.0f : top[m];  // a row that has seen nothing yet
+                const f4 x = weights(s, m, u, 0, zero), y = weights(s, m, u, 1, zero);
+                p[m] = pack(x, y);
+            }
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                u4 w = read_v(u * DT + d);
+                if (odd) w = read_odd_free(w, kExponent);
+#pragma unroll
+                for (int m = 0; m < NQ; ++m) o[m][d] = mma32<T>(w, p[m], o[m][d]);
+            }
+        }
+        other_stage();
+    }
+
+#pragma unroll
+    for (int m = 0; m < NQ; ++m) {
+        const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum[m]), __float_as_uint(sum[m]), false, false);
+        sum[m] = __uint_as_float(x[0]) + __uint_as_float(x[1]);
     }
     if (parts > 1) {
         // [unit][split][row][D + 4]: the sums, then maximum and sum
         const int unit = slot * a.kv_heads + head;
         constexpr int kRowFloats = D + kTileFloats;
         const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(a.ws, 0, 0x7FFFFFFF, kBufferFlags);
-        const int64_t first_row = static_cast<int64_t>(unit) * a.splits * a.part_rows + 32 * wave + c32;
-        if (mine) {
-            const int to = static_cast<int>((first_row + static_cast<int64_t>(split) * a.part_rows) * kRowFloats * 4);
+        const int64_t first_row = static_cast<int64_t>(unit) * a.splits * a.part_rows + 32 * NQ * wave + c32;
+#pragma unroll
+        for (int m = 0; m < NQ; ++m) {
+            if (!mine[m]) continue;
+            const int to = static_cast<int>((first_row + 32 * m + static_cast<int64_t>(split) * a.part_rows) * kRowFloats * 4);
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
                 for (int i = 0; i < 16; i += 4)
-                    __builtin_amdgcn_raw_buffer_store_b128(bitcast<u4>(f4{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]}), rs,
-                                                           to + (32 * d + 2 * i + 4 * h) * 4, 0, kCoherentAux);
+                    __builtin_amdgcn_raw_buffer_store_b128(
+                        bitcast<u4>(f4{o[m][d][i], o[m][d][i + 1], o[m][d][i + 2], o[m][d][i + 3]}), rs,
+                        to + (32 * d + 2 * i + 4 * h) * 4, 0, kCoherentAux);
             if (h == 0)
-                __builtin_amdgcn_raw_buffer_store_b64(u2{__float_as_uint(top), __float_as_uint(sum)}, rs, to + D * 4, 0, kCoherentAux);
+                __builtin_amdgcn_raw_buffer_store_b64(u2{__float_as_uint(top[m]), __float_as_uint(sum[m])}, rs, to + D * 4, 0,
+                                                      kCoherentAux);
         }
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
@@ -707,47 +848,53 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {
             *flag = __hip_atomic_fetch_add(a.locks + unit, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
         __syncthreads();
         if (!*flag) return;
-        if (mine) {
-            top = kNone, sum = 0.0f;
+#pragma unroll
+        for (int m = 0; m < NQ; ++m) {
+            if (!mine[m]) continue;
+            top[m] = kNone, sum[m] = 0.0f;
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
-            for (int s = 0; s < parts; ++s) {
-                const int from = static_cast<int>((first_row + static_cast<int64_t>(s) * a.part_rows) * kRowFloats * 4);
+                for (int i = 0; i < 16; ++i) o[m][d][i] = 0.0f;
+            for (int part = 0; part < parts; ++part) {
+                const int from = static_cast<int>((first_row + 32 * m + static_cast<int64_t>(part) * a.part_rows) * kRowFloats * 4);
                 const u2 ms = bitcast<u2>(__builtin_amdgcn_raw_buffer_load_b64(rs, from + D * 4, 0, kCoherentAux));
                 f4 x[4 * DT];
 #pragma unroll
                 for (int i = 0; i < 4 * DT; ++i)
                     x[i] = bitcast<f4>(__builtin_amdgcn_raw_buffer_load_b128(rs, from + (8 * i + 4 * h) * 4, 0, kCoherentAux));
-                const float other = __uint_as_float(ms.x), now = fmaxf(top, other), zero = now == kNone ? 0.0f : now;
-                const float keep = __builtin_amdgcn_exp2f(top - zero), f = __builtin_amdgcn_exp2f(other - zero);
-                top = now;
-                sum = sum * keep + f * __uint_as_float(ms.y);
+                const float other = __uint_as_float(ms.x), now = fmaxf(top[m], other), zero = now == kNone ? 0.0f : now;
+                const float keep = __builtin_amdgcn_exp2f(top[m] - zero), f = __builtin_amdgcn_exp2f(other - zero);
+                top[m] = now;
+                sum[m] = sum[m] * keep + f * __uint_as_float(ms.y);
 #pragma unroll
                 for (int d = 0; d < DT; ++d)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) o[d][i] = o[d][i] * keep + f * x[4 * d + (i >> 2)][i & 3];
+                    for (int i = 0; i < 16; ++i) o[m][d][i] = o[m][d][i] * keep + f * x[4 * d + (i >> 2)][i & 3];
             }
         }
         if (threadIdx.x == 0) __hip_atomic_store(a.locks + unit, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     // a lane has 4 of every 8 values: the halves of the wavefront exchange blocks, so that each stores 16 bytes
-    const bool nothing = sum == 0.0f;  // no key, or none with a score above -inf: zero
-    const float inv = 1.0f / sum;
-    uint16_t* dst = a.out + (static_cast<int64_t>(t.start + tok) * a.heads + head * a.group + r - tok * a.group) * D + 8 * h;
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
+    for (int m = 0; m < NQ; ++m) {
+        const bool nothing = sum[m] == 0.0f;  // no key, or none with a score above -inf: zero
+        const float inv = 1.0f / sum[m];
+        const int r = t.first + 32 * (NQ * wave + m) + c32, tok = r / a.group;
+        uint16_t* dst = a.out + (static_cast<int64_t>(t.start + tok) * a.heads + head * a.group + r - tok * a.group) * D + 8 * h;
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            float x[8];
+        for (int d = 0; d < DT; ++d)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = nothing ? 0.0f : o[d][8 * b + i] * inv;
-            const u4 y = from_f32<T>(x);
-            const auto e = __builtin_amdgcn_permlane32_swap(y[0], y[2], false, false);
-            const auto f = __builtin_amdgcn_permlane32_swap(y[1], y[3], false, false);
-            if (mine) *reinterpret_cast<u4*>(dst + 32 * d + 16 * b) = u4{e[0], f[0], e[1], f[1]};
-        }
+            for (int b = 0; b < 2; ++b) {
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = nothing ? 0.0f : o[m][d][8 * b + i] * inv;
+                const u4 y = from_f32<T>(x);
+                const auto e = __builtin_amdgcn_permlane32_swap(y[0], y[2], false, false);
+                const auto f = __builtin_amdgcn_permlane32_swap(y[1], y[3], false, false);
+                if (mine[m]) *reinterpret_cast<u4*>(dst + 32 * d + 16 * b) = u4{e[0], f[0], e[1], f[1]};
+            }
+    }
 }
 
 constexpr int64_t kWorkspaceFloats = TW4_AUTO_SPLIT_FLOATS;
@@ -811,7 +958,8 @@ extern "C" int tw4_paged_attention(const uint16_t* q, int64_t q_token, int64_t q
     const int shift = page_shift(page_size);
     TW4_REQUIRE(shift >= 0, TW4_EINVAL, "paged_attention: page_size 16, 32, 64, 128 or 256 (%d)", page_size);
     TW4_REQUIRE(scale > 0.0f && scale < 1e30f, TW4_EINVAL, "paged_attention: a positive scale (%g)", scale);
-    TW4_REQUIRE(rows == 16 || rows == 32 || rows == 128, TW4_ECONFIG, "paged_attention: tiles of 16, 32 or 128 rows (%d)", rows);
+    TW4_REQUIRE(rows == 16 || rows == 32 || rows == 128, TW4_ECONFIG,
+                "paged_attention: tiles of 16, 32 or 128 rows (%d)", rows);
     TW4_REQUIRE(width >= 0 && num_pages >= 0 && static_cast<int64_t>(num_pages) * page_size < 1LL << 31 &&
                     static_cast<int64_t>(width) * page_size < 1LL << 31,
                 TW4_EINVAL, "paged_attention: fewer than 2^31 slots (%d pages of %d, %d per request)", num_pages, page_size, width);

@@ -194,7 +194,7 @@ def test_every_split_and_tile(splits, rows):
     args = build([1000, 40, 0, 129], [3, 1, 20, 1], 8, 2, 128, torch.float16, 16, seed=2)
     q, k, v, table, lens, starts = args
     out = torch.full_like(q, float("nan"))
-    ws = torch.empty(1 << 24, device="cuda")
+    ws = torch.empty(1 << 25, device="cuda")
     locks = torch.zeros(1 << 12, dtype=torch.int32, device="cuda")
     for _ in range(2):
         w4_hip.check(w4_hip.library().tw4_paged_attention(
