@@ -19,6 +19,7 @@
 // wavefront's own LDS, read back transposed. With few rows in flight the keys are split over `splits` workgroups; the last to arrive
 // joins their results in order.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "tw4_attn.h"
@@ -42,7 +43,7 @@ struct AttnArgs {
 };
 
 constexpr int kTileFloats = 4;  // per row of a partial result beside its D sums: maximum, sum, and two that keep rows 16-byte aligned
-constexpr int kMinKeys = 128, kLongKeys = 2048;
+constexpr int kMinKeys = 128;  // of a split
 
 // A tile of rows: its request, first row, and the keys it can see.
 struct Tile {
@@ -921,24 +922,53 @@ int attn_launch(const AttnArgs& a, int rows, unsigned units, hipStream_t st) {
 
 using namespace tw4;
 
+// Microseconds of a call with tiles of kRows[i] rows and `splits` splits, as fitted to 150 calls of all sizes with each tile and 1 to
+// 128 splits (batches 1 to 200, 1 to 2000 new tokens, 0 to 100000 keys, heads of 64 and 128). A workgroup takes `start`, its keys' latency,
+// and, with splits, the store of its part and the last one's reading of all; two workgroups share a CU, so beyond 2 cus of them the
+// keys' throughput counts. What the rule picks took 1.02 times the fastest tile and split on average, 1.13 at most (decode of 15 requests of
+// up to 1114 keys, 40 heads: 17.6 us with 3 splits, 15.6 with 2). Without it: tiles by rows alone (16, 32, or 128 past 32 rows) and
+// splits for two workgroups per CU took 1.3 on average, 5.8 at most (7 new tokens of 24 heads over 7638 keys: 119 us with tiles of 128 rows
+// and 60 splits, 20.4 with 16 rows and 12).
+constexpr int kRows[3] = {16, 32, 128};
+double cost_us(int i, int64_t units, int splits, int group, int head_dim, int max_keys, int single, int cus) {
+    constexpr double kStart[3] = {5.9, 8.4, 9.0}, kLatency[3] = {0.0113, 0.0083, 0.0135}, kRate[3] = {0.012, 0.018, 0.048},
+                     kJoin[3] = {0.41, 0.14, 0.096};
+    const int quantum = kRows[i] == 128 ? 64 : 128;
+    const int64_t share =
+        (std::max<int64_t>((static_cast<int64_t>(max_keys) + splits - 1) / splits, kMinKeys) + quantum - 1) / quantum * quantum;
+    const int64_t parts = std::max<int64_t>((max_keys + share - 1) / share, 1);
+    const double keys = static_cast<double>(std::min<int64_t>(share, max_keys)) * (head_dim == 64 ? 0.375 : 1.0);
+    const double load = static_cast<double>(units) * parts / (2.0 * cus);
+    const double rounds = load > 1.0 ? load + 0.155 * (std::ceil(load) - load) : load;
+    double us = kStart[i] + std::pow(std::pow(kLatency[i] * keys, 1.34) + std::pow(kRate[i] * keys * rounds, 1.34), 1 / 1.34) +
+                1.37 * std::max(load - 1.0, 0.0);
+    if (parts > 1) us += 2.7 + kJoin[i] * parts * (single ? std::min(kRows[i], group) : kRows[i]) / 16.0 + 2.2 * load;
+    return us;
+}
+
 // out: rows of a tile, splits, workspace floats, counters
 extern "C" int tw4_paged_attention_plan(int tokens, int batch, int heads, int kv_heads, int head_dim, int max_query, int max_keys,
                                         int single, int cus, int* out) {
-    TW4_REQUIRE(out && tokens >= 0 && batch >= 0 && kv_heads >= 1 && heads >= 1 && heads % kv_heads == 0 && head_dim >= 1 && cus >= 1,
+    TW4_REQUIRE(out && tokens >= 0 && batch >= 0 && kv_heads >= 1 && heads >= 1 && heads % kv_heads == 0 && head_dim >= 1 && cus >= 1 &&
+                    max_keys >= 0,
                 TW4_EINVAL, "paged_attention_plan: bad sizes");
     const int group = heads / kv_heads;
-    const int64_t most = static_cast<int64_t>(max_query) * group;
-    const int rows = most > 32 ? 128 : most > 16 ? 32 : 16;
-    const int64_t units = tile_slots(tokens, batch, group, rows, single) * kv_heads;
-    const int64_t part = static_cast<int64_t>(single ? std::min(rows, group) : rows) * (head_dim + kTileFloats);
-    int64_t splits = 1;
-    for (int per_cu = 2; units > 0 && per_cu <= 4; per_cu *= 2) {
-        splits = std::max<int64_t>((per_cu * cus + units / 2) / units, 1);
-        if (max_keys <= kLongKeys * splits) break;
+    double best = 0.0;
+    int rows = 0, splits = 1;
+    int64_t units = 0, part = 0;
+    for (int i = 0; i < 3; ++i) {
+        const int64_t u = tile_slots(tokens, batch, group, kRows[i], single) * kv_heads;
+        const int64_t floats = static_cast<int64_t>(single ? std::min(kRows[i], group) : kRows[i]) * (head_dim + kTileFloats);
+        // and what fills the CUs once or twice
+        const int once = static_cast<int>(u ? 2 * cus / u : 0), twice = static_cast<int>(u ? 4 * cus / u : 0);
+        for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 64, once, twice}) {
+            if (s < 1 || (s > 1 && (static_cast<int64_t>(s - 1) * kMinKeys >= max_keys || u * s * floats > kWorkspaceFloats ||
+                                    u > TW4_AUTO_SPLIT_COUNTERS)))
+                continue;
+            const double us = cost_us(i, u, s, group, head_dim, max_keys, single, cus);
+            if (rows == 0 || us < best) best = us, rows = kRows[i], splits = s, units = u, part = floats;
+        }
     }
-    splits = std::min<int64_t>(splits, (static_cast<int64_t>(max_keys) + kMinKeys - 1) / kMinKeys);
-    if (units > 0) splits = std::min<int64_t>(splits, kWorkspaceFloats / (units * part));
-    splits = std::max<int64_t>(splits, 1);
     out[0] = rows;
     out[1] = static_cast<int>(splits);
     out[2] = splits > 1 ? static_cast<int>(units * splits * part) : 0;

@@ -76,7 +76,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     (q_strides, cache, (table_stride, width), sizes, index) = _checked(
         layout(q), layout(k_cache), layout(v_cache), layout(page_table), layout(seq_lens),
         None if query_start is None else layout(query_start), None if out is None else layout(out),
-        max_query_len, None if max_seq_len is None else (max_seq_len + 511) // 512 * 512, scale)
+        max_query_len, None if max_seq_len is None else (max_seq_len + 127) // 128 * 128, scale)
     if not w4_hip.plain(q):
         raise RuntimeError("paged_attention: inference only, no gradient, transform or tracer can follow q")
     if out is None:
