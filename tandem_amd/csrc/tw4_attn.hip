@@ -482,8 +482,8 @@ __device__ __forceinline__ f16v mma32(const u4& a, const u4& b, const f16v& c) {
 // Lane (c, h) = (lane % 32, lane / 32): scores S^T of row c, keys 8 (i / 4) + 4 h + i % 4 of 32.
 template <typename T, int D>
 __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {
-    constexpr int NQ = 1, B = 128 * NQ, KEYS = 64, C = D / 8, KS = D / 16, DT = D / 32, ROWS = 64 / C, NJ = 16 / ROWS;  // ROWS of a 1 KB load
-    constexpr int TILE = KEYS * C;                                                                               // 16-byte chunks of a tile
+    constexpr int B = 128, KEYS = 64, C = D / 8, KS = D / 16, DT = D / 32, ROWS = 64 / C, NJ = 16 / ROWS;  // ROWS of a 1 KB load
+    constexpr int TILE = KEYS * C;                                                                          // 16-byte chunks of a tile
     constexpr uint32_t kExponent = __is_same(T, h1) ? 0x7C00u : 0x7F80u;
     __shared__ u4 lds[2 * 2 * TILE];  // K [stage][key][chunk], V alike
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c32 = lane & 31, h = lane >> 5;
@@ -493,19 +493,15 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {
     Tile t;
     if (!find_tile<B>(a, slot, lane, t)) return;
 
-    int limit[NQ];
-    bool mine[NQ];
-    u4 q[NQ][KS];
-#pragma unroll
-    for (int m = 0; m < NQ; ++m) {
-        const int at = 32 * (NQ * wave + m) + c32, r = t.first + at, tok = r / a.group;
-        mine[m] = at < t.rows;
-        limit[m] = mine[m] ? t.len - t.fresh + tok : -1;
+    const int r = t.first + 32 * wave + c32, tok = r / a.group;
+    const bool mine = 32 * wave + c32 < t.rows, active = 32 * wave < t.rows;  // this lane, this wavefront has a row
+    const int limit = mine ? t.len - t.fresh + tok : -1;
+    u4 q[KS];
+    {
         const uint16_t* src = a.q + (t.start + tok) * a.q_token + (head * a.group + r - tok * a.group) * a.q_head + 8 * h;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) q[m][s] = mine[m] ? *reinterpret_cast<const u4*>(src + 16 * s) : u4{0, 0, 0, 0};
+        for (int e = 0; e < KS; ++e) q[e] = mine ? *reinterpret_cast<const u4*>(src + 16 * e) : u4{0, 0, 0, 0};
     }
-    const bool active = 32 * NQ * wave < t.rows;  // this wavefront has a row
     const int tile_high = t.len - t.fresh + (t.first + min(t.rows, B) - 1) / a.group;  // the last key a row of the tile sees
     const int end = static_cast<int>(min(static_cast<int64_t>(tile_high) + 1, static_cast<int64_t>(a.width) << a.shift));
     int begin = 0, stop = max(end, 0), parts = 1;
@@ -519,16 +515,11 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {
         return;
     }
 
-    f16v o[NQ][DT];
-    float top[NQ], sum[NQ];
+    const f16v none = {};
+    f16v o[DT], s[2];
+    float top = kNone, sum = 0.0f;
 #pragma unroll
-    for (int m = 0; m < NQ; ++m) {
-        top[m] = kNone, sum[m] = 0.0f;
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[m][d][i] = 0.0f;
-    }
+    for (int d = 0; d < DT; ++d) o[d] = none;
 
     const_int* table = (const_int*)(a.table + t.request * a.table_stride);
     const uint16_t* kh = a.k + head * a.head_stride;
@@ -617,8 +608,6 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {
         const u2 lo = read_tr(lds, at), hi = read_tr(lds, at + 8 * C * 16);
         return u4{lo.x, lo.y, hi.x, hi.y};
     };
-    const f16v none = {};
-    f16v s[NQ][2];
     auto scores = [&] {
         u4 k[2 * KS];
         constexpr int KA = 6;  // reads ahead of their products
@@ -627,12 +616,11 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {
 #pragma unroll
         for (int e = 0; e < 2 * KS; ++e) {
             if (e + KA < 2 * KS) k[e + KA] = read_k(e + KA);
-#pragma unroll
-            for (int m = 0; m < NQ; ++m) s[m][e & 1] = mma32<T>(k[e], q[m][e >> 1], e < 2 ? none : s[m][e & 1]);
+            s[e & 1] = mma32<T>(k[e], q[e >> 1], e < 2 ? none : s[e & 1]);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    auto best_of = [&](const f16v (&s)[2]) {
+    auto best_of = [&] {
         float best = s[0][0];
 #pragma unroll
         for (int n = 0; n < 2; ++n)
@@ -643,30 +631,25 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {
     };
     // The sums are scaled to a new maximum only when it is more than 2^8 times the old: probabilities up to 256 instead of 1 are as
     // exact, and most tiles need no pass over the sums.
-    auto raise = [&](const float (&best)[NQ]) {
-        bool any = false;
+    auto raise = [&](float best) {
+        if (__ballot(best > top + 8.0f)) {
+            const float now = fmaxf(top, best), keep = __builtin_amdgcn_exp2f(top - (now == kNone ? 0.0f : now));
+            top = now;
+            sum *= keep;
 #pragma unroll
-        for (int m = 0; m < NQ; ++m) any |= best[m] > top[m] + 8.0f;
-        if (__ballot(any)) {
+            for (int d = 0; d < DT; ++d)
 #pragma unroll
-            for (int m = 0; m < NQ; ++m) {
-                const float now = fmaxf(top[m], best[m]), keep = __builtin_amdgcn_exp2f(top[m] - (now == kNone ? 0.0f : now));
-                top[m] = now;
-                sum[m] *= keep;
-#pragma unroll
-                for (int d = 0; d < DT; ++d)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[m][d][i] *= keep;
-            }
+                for (int i = 0; i < 16; ++i) o[d][i] *= keep;
         }
+        return top == kNone ? 0.0f : top;  // nothing seen yet
     };
     // four probabilities, of keys 16 u + 8 x + 4 h ..
-    auto weights = [&](const f16v (&s)[NQ][2], int m, int u, int x, float zero) {
+    auto weights = [&](int u, int x, float zero) {
         f4 w;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[m][u >> 1][8 * (u & 1) + 4 * x + i], a.scale, -zero));
-            sum[m] += w[i];
+            w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u >> 1][8 * (u & 1) + 4 * x + i], a.scale, -zero));
+            sum += w[i];
         }
         return w;
     };
@@ -719,14 +702,10 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {
         scores();
         u4 v[4 * DT];
         constexpr int VA = DT;  // reads ahead of their products
-        float best[NQ];
-#pragma unroll
-        for (int m = 0; m < NQ; ++m) best[m] = best_of(s[m]);
-        raise(best);
-        const float zero = top[0] == kNone ? 0.0f : top[0];
+        const float zero = raise(best_of());
 #pragma unroll
         for (int e = 0; e < VA; ++e) v[e] = read_v(e);
-        f4 x = weights(s, 0, 0, 0, zero), y = weights(s, 0, 0, 1, zero);
+        f4 x = weights(0, 0, zero), y = weights(0, 1, zero);
         u4 p = pack(x, y);
         __builtin_amdgcn_sched_barrier(0);
         // a step: the products of 16 keys beside the probabilities of the next 16
@@ -736,9 +715,9 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {
             for (int d = 0; d < DT; ++d) {
                 const int e = u * DT + d;
                 if (e + VA < 4 * DT) v[e + VA] = read_v(e + VA);
-                o[0][d] = mma32<T>(v[e], p, o[0][d]);
-                if (u < 3 && d == 0) x = weights(s, 0, u + 1, 0, zero);
-                if (u < 3 && d == DT / 2) y = weights(s, 0, u + 1, 1, zero);
+                o[d] = mma32<T>(v[e], p, o[d]);
+                if (u < 3 && d == 0) x = weights(u + 1, 0, zero);
+                if (u < 3 && d == DT / 2) y = weights(u + 1, 1, zero);
                 __builtin_amdgcn_sched_barrier(0);
             }
             if (u < 3) p = pack(x, y);
@@ -755,14 +734,12 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {
                         (there(entry(base + 48)) ? 0 : 8);
         bool odd = false;
 #pragma unroll
-        for (int m = 0; m < NQ; ++m)
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int key = 32 * n + 8 * (i >> 2) + 4 * h + (i & 3);
-                    if (base + key > min(limit[m], stop - 1) || (off >> (key >> 4) & 1)) s[m][n][i] = kNone;
-                }
+            for (int i = 0; i < 16; ++i) {
+                const int key = 32 * n + 8 * (i >> 2) + 4 * h + (i & 3);
+                if (base + key > min(limit, stop - 1) || (off >> (key >> 4) & 1)) s[n][i] = kNone;
+            }
         // A probability of zero does not take an infinity or NaN away: where some row does not see a key, such values are left out
         // of the product and added to the rows that see them.
 #pragma unroll 2
@@ -772,75 +749,58 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {
             for (int i = 0; i < 4; ++i) odd |= odd16(w[i], kExponent);
         }
         odd = __ballot(odd) != 0;
-        float best[NQ];
-#pragma unroll
-        for (int m = 0; m < NQ; ++m) best[m] = best_of(s[m]);
-        raise(best);
+        const float zero = raise(best_of());
         if (odd) {
 #pragma unroll 1
-            for (int key = 0; key < KEYS; ++key)
+            for (int key = 0; key < KEYS; ++key) {
+                if (base + key > min(limit, stop - 1) || (off >> (key >> 4) & 1)) continue;
 #pragma unroll
-                for (int m = 0; m < NQ; ++m) {
-                    if (base + key > min(limit[m], stop - 1) || (off >> (key >> 4) & 1)) continue;
+                for (int i = 0; i < 4 * DT; ++i) {  // four values from 8 i + 4 h on
+                    const u2 four = *reinterpret_cast<const u2*>(reinterpret_cast<const char*>(vt) +
+                                                                 (key * C + v_place(key, i)) * 16 + h * 8);
 #pragma unroll
-                    for (int i = 0; i < 4 * DT; ++i) {  // four values from 8 i + 4 h on
-                        const u2 four = *reinterpret_cast<const u2*>(reinterpret_cast<const char*>(vt) +
-                                                                     (key * C + v_place(key, i)) * 16 + h * 8);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const uint16_t bits = static_cast<uint16_t>(four[e >> 1] >> (16 * (e & 1)));
-                            if ((bits & kExponent) == kExponent)
-                                o[m][i >> 2][4 * (i & 3) + e] += static_cast<float>(bitcast<T>(bits));
-                        }
-                        __builtin_amdgcn_sched_barrier(0);  // one at a time: the rare path is not to take registers
+                    for (int e = 0; e < 4; ++e) {
+                        const uint16_t bits = static_cast<uint16_t>(four[e >> 1] >> (16 * (e & 1)));
+                        if ((bits & kExponent) == kExponent) o[i >> 2][4 * (i & 3) + e] += static_cast<float>(bitcast<T>(bits));
                     }
+                    __builtin_amdgcn_sched_barrier(0);  // one at a time: the rare path is not to take registers
                 }
+            }
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            u4 p[NQ];
-#pragma unroll
-            for (int m = 0; m < NQ; ++m) {
-                const float zero = top[m] == kNone ? 0.0f : top[m];  // a row that has seen nothing yet
-                const f4 x = weights(s, m, u, 0, zero), y = weights(s, m, u, 1, zero);
-                p[m] = pack(x, y);
-            }
+            const f4 x = weights(u, 0, zero), y = weights(u, 1, zero);
+            const u4 p = pack(x, y);
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
                 u4 w = read_v(u * DT + d);
                 if (odd) w = read_odd_free(w, kExponent);
-#pragma unroll
-                for (int m = 0; m < NQ; ++m) o[m][d] = mma32<T>(w, p[m], o[m][d]);
+                o[d] = mma32<T>(w, p, o[d]);
             }
         }
         other_stage();
     }
 
-#pragma unroll
-    for (int m = 0; m < NQ; ++m) {
-        const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum[m]), __float_as_uint(sum[m]), false, false);
-        sum[m] = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+    {
+        const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
+        sum = __uint_as_float(x[0]) + __uint_as_float(x[1]);
     }
     if (parts > 1) {
         // [unit][split][row][D + 4]: the sums, then maximum and sum
         const int unit = slot * a.kv_heads + head;
         constexpr int kRowFloats = D + kTileFloats;
         const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(a.ws, 0, 0x7FFFFFFF, kBufferFlags);
-        const int64_t first_row = static_cast<int64_t>(unit) * a.splits * a.part_rows + 32 * NQ * wave + c32;
-#pragma unroll
-        for (int m = 0; m < NQ; ++m) {
-            if (!mine[m]) continue;
-            const int to = static_cast<int>((first_row + 32 * m + static_cast<int64_t>(split) * a.part_rows) * kRowFloats * 4);
+        const int64_t first_row = static_cast<int64_t>(unit) * a.splits * a.part_rows + 32 * wave + c32;
+        if (mine) {
+            const int to = static_cast<int>((first_row + static_cast<int64_t>(split) * a.part_rows) * kRowFloats * 4);
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
                 for (int i = 0; i < 16; i += 4)
-                    __builtin_amdgcn_raw_buffer_store_b128(
-                        bitcast<u4>(f4{o[m][d][i], o[m][d][i + 1], o[m][d][i + 2], o[m][d][i + 3]}), rs,
-                        to + (32 * d + 2 * i + 4 * h) * 4, 0, kCoherentAux);
+                    __builtin_amdgcn_raw_buffer_store_b128(bitcast<u4>(f4{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]}), rs,
+                                                           to + (32 * d + 2 * i + 4 * h) * 4, 0, kCoherentAux);
             if (h == 0)
-                __builtin_amdgcn_raw_buffer_store_b64(u2{__float_as_uint(top[m]), __float_as_uint(sum[m])}, rs, to + D * 4, 0,
-                                                      kCoherentAux);
+                __builtin_amdgcn_raw_buffer_store_b64(u2{__float_as_uint(top), __float_as_uint(sum)}, rs, to + D * 4, 0, kCoherentAux);
         }
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
@@ -849,53 +809,45 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {
             *flag = __hip_atomic_fetch_add(a.locks + unit, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
         __syncthreads();
         if (!*flag) return;
+        if (mine) {
+            top = kNone, sum = 0.0f;
 #pragma unroll
-        for (int m = 0; m < NQ; ++m) {
-            if (!mine[m]) continue;
-            top[m] = kNone, sum[m] = 0.0f;
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[m][d][i] = 0.0f;
+            for (int d = 0; d < DT; ++d) o[d] = none;
             for (int part = 0; part < parts; ++part) {
-                const int from = static_cast<int>((first_row + 32 * m + static_cast<int64_t>(part) * a.part_rows) * kRowFloats * 4);
+                const int from = static_cast<int>((first_row + static_cast<int64_t>(part) * a.part_rows) * kRowFloats * 4);
                 const u2 ms = bitcast<u2>(__builtin_amdgcn_raw_buffer_load_b64(rs, from + D * 4, 0, kCoherentAux));
                 f4 x[4 * DT];
 #pragma unroll
                 for (int i = 0; i < 4 * DT; ++i)
                     x[i] = bitcast<f4>(__builtin_amdgcn_raw_buffer_load_b128(rs, from + (8 * i + 4 * h) * 4, 0, kCoherentAux));
-                const float other = __uint_as_float(ms.x), now = fmaxf(top[m], other), zero = now == kNone ? 0.0f : now;
-                const float keep = __builtin_amdgcn_exp2f(top[m] - zero), f = __builtin_amdgcn_exp2f(other - zero);
-                top[m] = now;
-                sum[m] = sum[m] * keep + f * __uint_as_float(ms.y);
+                const float other = __uint_as_float(ms.x), now = fmaxf(top, other), zero = now == kNone ? 0.0f : now;
+                const float keep = __builtin_amdgcn_exp2f(top - zero), f = __builtin_amdgcn_exp2f(other - zero);
+                top = now;
+                sum = sum * keep + f * __uint_as_float(ms.y);
 #pragma unroll
                 for (int d = 0; d < DT; ++d)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) o[m][d][i] = o[m][d][i] * keep + f * x[4 * d + (i >> 2)][i & 3];
+                    for (int i = 0; i < 16; ++i) o[d][i] = o[d][i] * keep + f * x[4 * d + (i >> 2)][i & 3];
             }
         }
         if (threadIdx.x == 0) __hip_atomic_store(a.locks + unit, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     // a lane has 4 of every 8 values: the halves of the wavefront exchange blocks, so that each stores 16 bytes
+    const bool nothing = sum == 0.0f;  // no key, or none with a score above -inf: zero
+    const float inv = 1.0f / sum;
+    uint16_t* dst = a.out + (static_cast<int64_t>(t.start + tok) * a.heads + head * a.group + r - tok * a.group) * D + 8 * h;
 #pragma unroll
-    for (int m = 0; m < NQ; ++m) {
-        const bool nothing = sum[m] == 0.0f;  // no key, or none with a score above -inf: zero
-        const float inv = 1.0f / sum[m];
-        const int r = t.first + 32 * (NQ * wave + m) + c32, tok = r / a.group;
-        uint16_t* dst = a.out + (static_cast<int64_t>(t.start + tok) * a.heads + head * a.group + r - tok * a.group) * D + 8 * h;
+    for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
+        for (int b = 0; b < 2; ++b) {
+            float x[8];
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                float x[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = nothing ? 0.0f : o[m][d][8 * b + i] * inv;
-                const u4 y = from_f32<T>(x);
-                const auto e = __builtin_amdgcn_permlane32_swap(y[0], y[2], false, false);
-                const auto f = __builtin_amdgcn_permlane32_swap(y[1], y[3], false, false);
-                if (mine[m]) *reinterpret_cast<u4*>(dst + 32 * d + 16 * b) = u4{e[0], f[0], e[1], f[1]};
-            }
-    }
+            for (int i = 0; i < 8; ++i) x[i] = nothing ? 0.0f : o[d][8 * b + i] * inv;
+            const u4 y = from_f32<T>(x);
+            const auto e = __builtin_amdgcn_permlane32_swap(y[0], y[2], false, false);
+            const auto f = __builtin_amdgcn_permlane32_swap(y[1], y[3], false, false);
+            if (mine) *reinterpret_cast<u4*>(dst + 32 * d + 16 * b) = u4{e[0], f[0], e[1], f[1]};
+        }
 }
 
 constexpr int64_t kWorkspaceFloats = TW4_AUTO_SPLIT_FLOATS;
