@@ -80,7 +80,8 @@ def _inputs(tokens, heads, kv, d, dtype, norm, seed):
 
 CASES = [(1, 32, 8, 128, torch.float16, True), (1, 1, 1, 64, torch.bfloat16, True), (3, 7, 1, 128, torch.bfloat16, False),
          (5, 5, 5, 64, torch.float16, False), (77, 40, 8, 128, torch.float16, True), (300, 24, 2, 64, torch.bfloat16, True),
-         (2100, 16, 8, 128, torch.bfloat16, True), (1031, 3, 3, 64, torch.float16, True)]
+         (2100, 16, 8, 128, torch.bfloat16, True), (6000, 32, 8, 128, torch.float16, True), (9001, 15, 7, 128, torch.bfloat16, False),
+         (1031, 3, 3, 64, torch.float16, True)]
 
 
 @pytest.mark.gpu
