@@ -15,9 +15,15 @@
 // as the rounding of the result); their sum is of the unrounded values.
 //
 // Rows kernel: a workgroup has one tile of 16 MT rows and a range of keys; its four wavefronts take blocks of 32 keys in turn, each
-// with a softmax of its own, joined at the end. K comes straight into registers (a lane has 16 bytes of a key), V through a
-// wavefront's own LDS, read back transposed. With few rows in flight the keys are split over `splits` workgroups; the last to arrive
-// joins their results in order.
+// with a softmax of its own, joined at the end. K comes straight into registers (a lane has 16 bytes of a key: half lines, which the
+// first-level cache joins, so they are ordinary loads), V as whole rows past the caches and through a wavefront's own LDS, read back
+// transposed; both a block ahead. It is bound by reading K and V: 3 requests of 40002 keys, 16 + 8 heads of 128, 75-77 us (6.4-6.5 TB/s; a plain
+// read reaches 7.1), 32 of 1 to 8192 keys, 32 + 8 heads, 91 (6.0). Measured and not kept: V by ordinary loads 113 us at 32 requests against 92, K
+// through LDS as well 100, three wavefronts per SIMD (they spill) 95. With few rows in flight the keys are split over up to `splits`
+// workgroups; the last to arrive joins their results in order: one request of 1024 keys 9.6 us, most of it ten dependent round trips to memory
+// (lengths, table, keys, the partial results' way out and in, the counter), of 32001 keys 31.
+//
+// Tiles of 128 rows (chunks of prompts): the chunk kernel below. Its K and V are read by 128 rows at a time from LDS.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -479,6 +485,11 @@ __device__ __forceinline__ f16v mma32(const u4& a, const u4& b, const f16v& c) {
 // each: while a tile is computed the next one is on its way. A wavefront fetches 16 keys of each tile, which lie in one page. Two workgroups
 // share a CU, and their wavefronts' products and exponentials fill each other's time. A wavefront issues one instruction in four cycles,
 // whatever its kind, so the loop over unmasked tiles computes no address: a lane's places change stage by a bit.
+// A prompt of 8192 tokens, 32 + 8 heads of 128, 557-594 us (925-987 TFLOP/s; between boxes), 5 chunks of up to 700 tokens behind up to 5000 keys, 40 + 8
+// heads, 167-175 (770-805). The matrix cores run half of the cycles, at the 1.8 GHz that the card's power leaves (hipBLASLt's product of 8192^3:
+// 1530 TFLOP/s); every wavefront reads all of K and V from LDS, 128 KB a tile and workgroup, which takes 62 % of the cycles. Measured and not
+// kept: 64 rows a wavefront, half the LDS reads but a SIMD's registers for one wavefront, 638 us against 577; the scores a tile ahead
+// 575 against 570; wavefront priorities 557 against 560.
 // Lane (c, h) = (lane % 32, lane / 32): scores S^T of row c, keys 8 (i / 4) + 4 h + i % 4 of 32.
 template <typename T, int D>
 __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {

@@ -9,9 +9,11 @@
 //   slot = table[i][position / P] P + position % P    (-1: no page, or a row behind the last request)
 //   taken <- min(first_last, length of the list)
 //
-// It moves a few KB and is bound by a launch and two or three dependent round trips to memory. One workgroup does the scan
-// and the tables, and for up to kInline rows the rows too: one launch for a decode step. Past that a second launch spreads
-// the rows over the GPU, finding each row's request by bisection in the starts.
+// It moves a few KB and is bound by a launch and three dependent round trips to memory (lengths, the list's entries, the table's): one
+// request 3.3 us, 512 in decode 5.0, 64 prompts of 350 tokens on average 7.4. One workgroup does the scan and the tables, and for up to
+// kInline rows the rows too: one launch for a decode step (against 4.7 us for one request in two). Past that a second launch spreads the
+// rows over the GPU, finding each row's request by bisection in the starts: 8 requests of 1000 tokens take 6.3 us in two launches and 7.3 in
+// one, but called eagerly 16.7 and 15.1, for the host's second launch; 16000 tokens take 6.4 and 12.1.
 #include "tw4_attn.h"
 
 namespace tw4 {
