@@ -126,7 +126,8 @@ int rope_launch(RopeArgs& a, hipStream_t st) {
     auto blocks = [&](int u) {
         return (static_cast<int64_t>(a.tokens) * ((a.groups + u - 1) / u) + 3) / 4;
     };
-    TW4_REQUIRE(blocks(1) < (1LL << 29), TW4_EINVAL, "norm_rope: too many values (%d tokens)", a.tokens);
+    // a launch has fewer than 2^32 threads
+    TW4_REQUIRE(blocks(D == 128 ? 4 : 1) < (1LL << 24), TW4_EINVAL, "norm_rope: too many values (%d tokens)", a.tokens);
     // One group a wavefront has the most loads under way (64 tokens 2.8 us against 4.2 with four). Where the data pass what the caches
     // hold, four that share the angles' loads are faster: heads of 128, 32 + 8 of them, 8192 tokens 43.3 us -> 38.9, 6000 33.1 -> 30.1, 4000
     // level at 22.8, 2000 13.2 -> 13.8; heads of 64 17.4 -> 19.0 at 6000.

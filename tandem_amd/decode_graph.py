@@ -60,6 +60,7 @@ class DecodeGraphRunner:
         self.query_lens = torch.zeros(self.max_bs, dtype=torch.int32, device=device)
         self.graphs: dict[int, torch.cuda.CUDAGraph] = {}
         self.outputs: dict[int, torch.Tensor] = {}
+        self.counts: dict[int, torch.Tensor] = {}  # kv_cache.PagePlan.counts of a bucket's last step
         self._capture_all()
 
     def _fn(self, bs: int) -> Callable[[], torch.Tensor]:
@@ -67,7 +68,9 @@ class DecodeGraphRunner:
             if self.cache is None:
                 hidden = self.model(self.input_ids[:bs])
             else:
-                hidden = self.model(self.input_ids[:bs], self.cache.plan(self.query_lens[:bs], bs, max_query_len=1))
+                batch = self.cache.plan(self.query_lens[:bs], bs, max_query_len=1)
+                self.counts[bs] = batch.counts
+                hidden = self.model(self.input_ids[:bs], batch)
             return self.model.compute_logits(hidden) if self.logits else hidden
         return run
 
@@ -100,7 +103,8 @@ class DecodeGraphRunner:
     def run(self, input_ids: Sequence[int] | torch.Tensor) -> torch.Tensor:
         """Token ids of b <= max_bs sequences -> the first b rows of the bucket's output (a view of a
         static buffer, overwritten by the next replay of that bucket). With a cache sequence i is lane i; a lane with an id below
-        zero sits the step out, and the rows are those of the others in order."""
+        zero sits the step out, and the rows are those of the others in order. A lane past the cache's max_seq_len answers NaN; one that the
+        cache had no page for misses its token's keys and values, and counts[bucket][2] says that it happened."""
         ids = torch.as_tensor(input_ids, dtype=torch.long)
         b = int(ids.numel())
         if not self.can_run(b):

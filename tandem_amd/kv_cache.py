@@ -70,7 +70,7 @@ def plan_pages(context_lens: torch.Tensor, query_lens: torch.Tensor, page_table:
     behind the last request's position 0 and slot -1. Where the list has no page left, or a request outgrows its row of the
     table, the entry and the slots there are -1.
 
-    int32 GPU tensors; lengths below zero count as zero, and the new tokens are fewer than 2^31 in all. seq_lens_out (context_lens
+    int32 GPU tensors; lengths below zero count as zero, and each new length and all new tokens together are below 2^31. seq_lens_out (context_lens
     itself, to advance it) and taken_out (taken itself) are written instead of new tensors. Nothing is read back; the caller that
     wants to know whether the pages sufficed reads counts[2]."""
     outs = () if seq_lens_out is None else (("seq_lens_out", layout(seq_lens_out), None),)
@@ -153,7 +153,7 @@ class PagedKVCache:
         self.context_lens = torch.zeros(max_requests, dtype=torch.int32, device=dev)
         self.free_pages = torch.arange(num_pages, dtype=torch.int32, device=dev)
         self.taken = torch.zeros(1, dtype=torch.int32, device=dev)
-        self.rotary = rotary.rotary_table(max_seq_len, head_dim, rope_theta, dev)
+        self.rotary = rotary.rotary_table(width * page_size, head_dim, rope_theta, dev)
 
     @classmethod
     def for_model(cls, config: "DecoderConfig", num_pages: int, max_requests: int, max_seq_len: int, page_size: int = 16,

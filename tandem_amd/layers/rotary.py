@@ -8,7 +8,8 @@
 A head x of D values becomes y = x rsqrt(mean(x^2) + eps) weight (no weight: y = x), and then, with the angle a_i of its
 token's position, (y[i] cos a_i - y[i + D/2] sin a_i, y[i + D/2] cos a_i + y[i] sin a_i): the halves of a head rotate
 against each other, as in the Qwen3 and Llama checkpoints of Hugging Face. fp32 arithmetic, one rounding. float16 and
-bfloat16, heads of 64 or 128 values. Inference only: tensors that autograd follows are refused.
+bfloat16, heads of 64 or 128 values. Inference only: a projection or a cache that autograd follows is refused, and the weights are
+taken as values, as in layers/norm.py.
 """
 
 from __future__ import annotations
@@ -61,7 +62,7 @@ def check_int32(who: str, name: str, t: tuple, shape: tuple[int, ...], index: in
 
 
 # Every check of a call but those of addresses and of who follows it, once for each combination of layouts: an eager call is bound by
-# the host (a decode step's, 15.6 -> 11.9 us).
+# the host (a decode step's, 16.6 -> 13.0 us).
 @functools.lru_cache(maxsize=1 << 12)
 def _checked(who: str, qkv: tuple, positions: tuple, table: tuple, heads: int, kv_heads: int, q_weight: tuple | None,
              k_weight: tuple | None, k: tuple | None, v: tuple | None, slots: tuple | None) -> tuple:
@@ -82,12 +83,17 @@ def _checked(who: str, qkv: tuple, positions: tuple, table: tuple, heads: int, k
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
         if w is not None and w != ((d,), (1,), dtype, index):
             raise RuntimeError(f"{who}: {name} must be a contiguous {dtype} tensor [{d}] on GPU {index}")
-    cache = (0, 0, 0, 0, 0)
+    cache: tuple = (0, 0, 0, 0, 0)
     if k is not None:
         pages, _, size = check_cache(who, k, v, dtype, index, kv_heads, d)
+        room = d
+        for step, n in sorted(zip(k[1][:3], k[0][:3])):
+            if n > 1 and step < room:
+                raise RuntimeError(f"{who}: the caches' places must not overlap (strides {k[1]})")
+            room = max(room, step * (n - 1) + room)
         check_int32(who, "slots", slots, (tokens,), index)
         cache = (pages, size, *k[1][:3])
-    return max(stride[0], shape[1]), d, cache, TYPES[dtype], index
+    return stride[0] if tokens > 1 else shape[1], d, cache, TYPES[dtype], index
 
 
 def _run(who: str, qkv, positions, table, num_heads: int, num_kv_heads: int, q_weight, k_weight, eps: float, k, v, slots):
@@ -95,8 +101,8 @@ def _run(who: str, qkv, positions, table, num_heads: int, num_kv_heads: int, q_w
                                              None if q_weight is None else layout(q_weight),
                                              None if k_weight is None else layout(k_weight), None if k is None else layout(k),
                                              None if v is None else layout(v), None if slots is None else layout(slots))
-    if not w4_hip.plain(qkv):
-        raise RuntimeError(f"{who}: inference only, no gradient, transform or tracer can follow qkv")
+    if not w4_hip.plain(qkv) or (slots is not None and torch.is_grad_enabled() and (k.requires_grad or v.requires_grad)):
+        raise RuntimeError(f"{who}: inference only, no gradient, transform or tracer can follow qkv or the caches")
     tokens = qkv.shape[0]
     q = torch.empty((tokens, num_heads, d), dtype=qkv.dtype, device=qkv.device)
     if slots is None:

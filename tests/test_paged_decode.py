@@ -192,8 +192,35 @@ def test_graph_runner_decodes_over_the_cache(monkeypatch):
             for c in caches:
                 c.release([0])
             seqs[0] = []
+    before = state(caches[0])
+    assert runner.run([-1, -1, -1]).shape[0] == 0
+    assert all(torch.equal(a, b) for a, b in zip(before, state(caches[0])))
     with pytest.raises(ValueError, match="lanes"):
         decode_graph.DecodeGraphRunner(model, max_bs=6, device=torch.device("cuda", 0), cache=caches[0])
+
+
+@pytest.mark.gpu
+def test_lanes_past_their_table_or_without_a_page_stay_alone(monkeypatch):
+    """A lane that outgrows its row of the table answers NaN, one that the list has no page for is counted; the others' rows are those of a
+    cache with room for all, bit for bit."""
+    model, _ = _model(monkeypatch, 15)
+    device = torch.device("cuda", 0)
+    prompts = [list(range(30)), list(range(9)), list(range(16))]
+    rows = []
+    for pages, longest in ((30, 64), (30, 32), (5, 32)):
+        cache = PagedKVCache.for_model(CFG, num_pages=pages, max_requests=3, max_seq_len=longest)
+        _step(model, cache, prompts)  # 2, 1 and 1 pages
+        runner = decode_graph.DecodeGraphRunner(model, max_bs=3, device=device, cache=cache)
+        rows.append([runner.run([1, 2, -1]).clone() for _ in range(4)])
+    for step, (full, narrow, few) in enumerate(zip(*rows)):
+        assert torch.equal(narrow[1], full[1]) and torch.equal(few, narrow) if step < 2 else torch.equal(few[1], full[1])
+        assert torch.equal(narrow, full) if step < 2 else torch.isnan(narrow[0]).all() and torch.isnan(few[0]).all()
+        assert torch.equal(narrow[1], full[1])
+    # the last page goes to lane 2; lane 1 fills its page, and then there is none
+    for ids, given, lacking in (([-1, 5, 3], 1, 0), ([-1, 5, -1], 0, 0), ([-1, 5, -1], 0, 0), ([-1, 5, 3], 0, 1)):
+        got = runner.run(ids)
+        assert runner.counts[3].tolist() == [len(got), given, lacking, 0] and torch.isfinite(got).all()
+    assert cache.page_table[:, 1].tolist()[1:] == [-1, 4] and int(cache.taken) == 5
 
 
 @pytest.mark.gpu

@@ -170,8 +170,14 @@ def test_refusals():
     for k, v, s, needle in ((cache[..., :32], cache[..., :32], slots, "caches"), (cache.bfloat16(), cache.bfloat16(), slots, "float16"),
                             (cache[:, :1], cache[:, :1], slots, "caches"), (cache[:, :, :8], cache[:, :, :8], slots, "caches"),
                             (cache, cache[:1], slots, "caches"), (cache, cache, slots.long(), "slots"),
-                            (cache, cache.transpose(0, 1).contiguous().transpose(0, 1), slots, "layout")):
+                            (cache, cache.transpose(0, 1).contiguous().transpose(0, 1), slots, "layout"),
+                            (cache[:1].expand(2, -1, -1, -1), cache[1:].expand(2, -1, -1, -1), slots, "overlap"),
+                            (cache.view(-1).as_strided(cache.shape, (2048, 1024, 56, 1)),) * 2 + (slots, "overlap"),
+                            (cache, cache.clone().requires_grad_(), slots, "inference")):
         with pytest.raises(RuntimeError, match=needle):
             rotary.norm_rope_cache(*ok, k, v, s)
+    # one row has no stride
+    one = torch.zeros(3, 8 * d + 1, dtype=torch.float16, device="cuda")[:1, :8 * d]
+    assert (rotary.norm_rope(one, pos[:1], table, heads, kv)[0] == 0).all()
     q, k = rotary.norm_rope(qkv[:0], pos[:0], table, heads, kv)
     assert q.shape == (0, heads, d) and k.shape == (0, kv, d)
