@@ -328,7 +328,7 @@ int tw4_paged_attention(const uint16_t* q, int64_t q_token, int64_t q_head, cons
                         void* stream);
 
 /* How tw4_paged_attention divides a call of these sizes on a device of `cus` CUs (max_query, max_keys: the most new tokens and
- * keys a request can have; single: starts is NULL): writes rows of a tile, splits, and the floats and counters that takes to
+ * keys a request is expected to have; single: starts is NULL): writes rows of a tile, splits, and the floats and counters that takes to
  * out[0 .. 4). Splits stay within TW4_AUTO_SPLIT_FLOATS and TW4_AUTO_SPLIT_COUNTERS. Host code. */
 int tw4_paged_attention_plan(int tokens, int batch, int heads, int kv_heads, int head_dim, int max_query, int max_keys,
                              int single, int cus, int* out);

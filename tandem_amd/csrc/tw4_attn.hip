@@ -12,13 +12,15 @@
 // of several keys, its limit, maximum and sum are one register each, and its probabilities are already where the second
 // product O^T = V^T P^T wants them (the order of keys inside a product is free: K's rows and V^T's columns only have to agree).
 // Probabilities are rounded to the cache's type for that product (at most half a step of the type, relative, each: the same size
-// as the rounding of the result); their sum is of the unrounded values.
+// as the rounding of the result); their sum is of the unrounded values. fp16 has 14 binary places below 1 before its steps stop shrinking,
+// and a long context can hold many keys of less than that each, so there both sums are of 2^14 p (2^6 p in the chunk kernel, whose p reaches
+// 2^8): the factor cancels in their quotient.
 //
 // Rows kernel: a workgroup has one tile of 16 MT rows and a range of keys; its four wavefronts take blocks of 32 keys in turn, each
 // with a softmax of its own, joined at the end. K comes straight into registers (a lane has 16 bytes of a key: half lines, which the
 // first-level cache joins, so they are ordinary loads), V as whole rows past the caches and through a wavefront's own LDS, read back
-// transposed; both a block ahead. It is bound by reading K and V: 3 requests of 40002 keys, 16 + 8 heads of 128, 75-77 us (6.4-6.5 TB/s; a plain
-// read reaches 7.1), 32 of 1 to 8192 keys, 32 + 8 heads, 91 (6.0). Measured and not kept: V by ordinary loads 113 us at 32 requests against 92, K
+// transposed; both a block ahead. It is bound by reading K and V: 3 requests of 40002 keys, 16 + 8 heads of 128, 75-77 us (6.4-6.6 TB/s; a plain
+// read reaches 7.1), 32 of 1 to 8192 keys, 32 + 8 heads, 91-94 (5.8-6.0). Measured and not kept: V by ordinary loads 113 us at 32 requests against 92, K
 // through LDS as well 100, three wavefronts per SIMD (they spill) 95. With few rows in flight the keys are split over up to `splits`
 // workgroups; the last to arrive joins their results in order: one request of 1024 keys 9.6 us, most of it ten dependent round trips to memory
 // (lengths, table, keys, the partial results' way out and in, the counter), of 32001 keys 31.
@@ -57,29 +59,34 @@ struct Tile {
     int start, len, fresh;     // the request's first token, keys, new tokens
 };
 
-// Slot s of the grid is a tile of request i, the last i with base_i = floor(start_i G / B) + i <= s: the base of the next request
-// is at least ceil(n_i G / B) further on, so no scan of the lengths is needed; slots past a request's rows have none. Each wavefront
-// looks at 64 requests at a time.
+// Slot s of the grid is the first tile of request s, and from slot `batch` on a further one: of request i, the last with
+// base_i = floor(start_i G / B) <= s - batch. A request has at most floor(n_i G / B) of those, and the base of the next is at least as far
+// on, so no scan of the lengths is needed; slots past a request's rows have none. So the slots of requests of one tile each, which
+// most calls have, lie together: with one or two slots in turn for a request, where the second is empty, the work gathered on half of the
+// shader engines (3 requests of 2 new tokens, 64 + 8 heads, 8000 keys: 31.6 us against 28.2; 40
+// of 8, 32 + 8 heads, 3000 keys: 108 against 88).
 template <int B>
 __device__ __forceinline__ bool find_tile(const AttnArgs& a, int slot, int lane, Tile& t) {
     int start, fresh;
     if (a.starts) {
-        int lo = 0, step = 64;
-        while (step < a.batch) step *= 64;
-        for (; step > 1;) {
-            step /= 64;
-            const int64_t i = lo + static_cast<int64_t>(lane) * step;
-            bool before = false;
-            if (i < a.batch) {
-                const int s = min(max(a.starts[i], 0), a.tokens);
-                before = static_cast<int64_t>(s) * a.group / B + i <= slot;
+        t.request = slot, t.first = 0;
+        if (slot >= a.batch) {
+            slot -= a.batch;
+            int lo = 0, step = 64;  // a wavefront looks at 64 requests at a time
+            while (step < a.batch) step *= 64;
+            for (; step > 1;) {
+                step /= 64;
+                const int64_t i = lo + static_cast<int64_t>(lane) * step;
+                bool before = false;
+                if (i < a.batch) before = static_cast<int64_t>(min(max(a.starts[i], 0), a.tokens)) * a.group / B <= slot;
+                lo += step * max(__popcll(__ballot(before)) - 1, 0);
             }
-            lo += step * max(__popcll(__ballot(before)) - 1, 0);
+            t.request = __builtin_amdgcn_readfirstlane(lo);
+            const int64_t base = static_cast<int64_t>(min(max(a.starts[t.request], 0), a.tokens)) * a.group / B;
+            t.first = (slot - static_cast<int>(base) + 1) * B;
         }
-        t.request = __builtin_amdgcn_readfirstlane(lo);
         start = min(max(a.starts[t.request], 0), a.tokens);
         fresh = min(max(a.starts[t.request + 1], start), a.tokens) - start;
-        t.first = (slot - static_cast<int>(static_cast<int64_t>(start) * a.group / B) - t.request) * B;
     } else {
         const int per = (a.group + B - 1) / B;
         t.request = slot / per;
@@ -89,7 +96,7 @@ __device__ __forceinline__ bool find_tile(const AttnArgs& a, int slot, int lane,
     }
     t.start = start;
     t.fresh = fresh;
-    t.len = a.lens[t.request];
+    t.len = max(a.lens[t.request], 0);
     t.rows = fresh * a.group - t.first;
     return t.first >= 0 && t.rows > 0;
 }
@@ -132,6 +139,10 @@ __device__ __forceinline__ u4 read_odd_free(u4 w, uint32_t exponent) {  // infin
 }
 
 constexpr float kNone = -__builtin_inff();
+
+// Probabilities of at most 2^BITS are summed times 2^kLift, up to 2^14 of fp16's 2^16 (bf16 has fp32's exponents).
+template <typename T, int BITS>
+constexpr float kLift = __is_same(T, h1) ? 14 - BITS : 0;
 
 template <typename T, int D, int MT>
 __global__ void __launch_bounds__(256, 2) rows_kernel(AttnArgs a) {
@@ -272,12 +283,12 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(AttnArgs a) {
             for (int i = 1; i < 8; ++i) high8 = fmaxf(high8, x[i]);
             const float now = fmaxf(top[m], max_rows(high8));
             const float zero = now == kNone ? 0.0f : now;  // a row that has seen nothing yet
-            const float keep = __builtin_amdgcn_exp2f(top[m] - zero);
+            const float keep = __builtin_amdgcn_exp2f(top[m] - zero), lifted = zero - kLift<T, 0>;
             top[m] = now;
             sum[m] *= keep;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                x[i] = __builtin_amdgcn_exp2f(x[i] - zero);
+                x[i] = __builtin_amdgcn_exp2f(x[i] - lifted);
                 sum[m] += x[i];
             }
             p[m] = from_f32<T>(x);
@@ -485,8 +496,8 @@ __device__ __forceinline__ f16v mma32(const u4& a, const u4& b, const f16v& c) {
 // each: while a tile is computed the next one is on its way. A wavefront fetches 16 keys of each tile, which lie in one page. Two workgroups
 // share a CU, and their wavefronts' products and exponentials fill each other's time. A wavefront issues one instruction in four cycles,
 // whatever its kind, so the loop over unmasked tiles computes no address: a lane's places change stage by a bit.
-// A prompt of 8192 tokens, 32 + 8 heads of 128, 557-594 us (925-987 TFLOP/s; between boxes), 5 chunks of up to 700 tokens behind up to 5000 keys, 40 + 8
-// heads, 167-175 (770-805). The matrix cores run half of the cycles, at the 1.8 GHz that the card's power leaves (hipBLASLt's product of 8192^3:
+// A prompt of 8192 tokens, 32 + 8 heads of 128, 551-594 us (925-998 TFLOP/s; between cards), 5 chunks of up to 700 tokens behind up to 5000 keys, 40 + 8
+// heads, 167-177 (760-805). The matrix cores run half of the cycles, at the 1.8 GHz that the card's power leaves (hipBLASLt's product of 8192^3:
 // 1530 TFLOP/s); every wavefront reads all of K and V from LDS, 128 KB a tile and workgroup, which takes 62 % of the cycles. Measured and not
 // kept: 64 rows a wavefront, half the LDS reads but a SIMD's registers for one wavefront, 638 us against 577; the scores a tile ahead
 // 575 against 570; wavefront priorities 557 against 560.
@@ -498,8 +509,10 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {
     constexpr uint32_t kExponent = __is_same(T, h1) ? 0x7C00u : 0x7F80u;
     __shared__ u4 lds[2 * 2 * TILE];  // K [stage][key][chunk], V alike
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c32 = lane & 31, h = lane >> 5;
-    // the last rows of a prompt see the most keys: they go first
-    const int slot = static_cast<int>(gridDim.x / a.kv_heads) - 1 - blockIdx.x / a.kv_heads, head = blockIdx.x % a.kv_heads;
+    // The last rows of a prompt see the most keys: they go first, but behind all requests' first tiles, or the last to start would be one
+    // of the longest request's (5 chunks as above: 218 us).
+    const int turn_of = blockIdx.x / a.kv_heads, head = blockIdx.x - turn_of * a.kv_heads;
+    const int slot = a.starts && turn_of >= a.batch ? static_cast<int>(gridDim.x / a.kv_heads) - 1 - (turn_of - a.batch) : turn_of;
     const int split = blockIdx.y;
     Tile t;
     if (!find_tile<B>(a, slot, lane, t)) return;
@@ -652,7 +665,7 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[d][i] *= keep;
         }
-        return top == kNone ? 0.0f : top;  // nothing seen yet
+        return (top == kNone ? 0.0f : top) - kLift<T, 8>;  // none: nothing seen yet
     };
     // four probabilities, of keys 16 u + 8 x + 4 h ..
     auto weights = [&](int u, int x, float zero) {
@@ -885,27 +898,28 @@ int attn_launch(const AttnArgs& a, int rows, unsigned units, hipStream_t st) {
 
 using namespace tw4;
 
-// Microseconds of a call with tiles of kRows[i] rows and `splits` splits, as fitted to 150 calls of all sizes with each tile and 1 to
+// Microseconds of a call with tiles of kRows[i] rows and `splits` splits, as fitted to 300 calls of all sizes with each tile and 1 to
 // 128 splits (batches 1 to 200, 1 to 2000 new tokens, 0 to 100000 keys, heads of 64 and 128). A workgroup takes `start`, its keys' latency,
 // and, with splits, the store of its part and the last one's reading of all; two workgroups share a CU, so beyond 2 cus of them the
-// keys' throughput counts. What the rule picks took 1.02 times the fastest tile and split on average, 1.13 at most (decode of 15 requests of
-// up to 1114 keys, 40 heads: 17.6 us with 3 splits, 15.6 with 2). Without it: tiles by rows alone (16, 32, or 128 past 32 rows) and
-// splits for two workgroups per CU took 1.3 on average, 5.8 at most (7 new tokens of 24 heads over 7638 keys: 119 us with tiles of 128 rows
-// and 60 splits, 20.4 with 16 rows and 12).
+// keys' throughput counts. What the rule picks took 1.011 times the fastest tile and split on average, 1.20 at most (4 chunks of 65 tokens:
+// 12.0 us with 16 rows, 10.0 with 128); on 75 calls it was not fitted to 1.017, 1.19 at most (5 chunks of 188 tokens of 7 heads behind 1908
+// keys: 33.2 us with 3 splits, 27.8 with one). Without it: tiles by rows alone (16, 32, or 128 past 32 rows) and splits for two
+// workgroups per CU took 1.3 on average, 5.8 at most (7 new tokens of 24 heads over 7638 keys: 119 us with tiles of 128 rows and 60
+// splits, 20.4 with 16 rows and 12).
 constexpr int kRows[3] = {16, 32, 128};
 double cost_us(int i, int64_t units, int splits, int group, int head_dim, int max_keys, int single, int cus) {
-    constexpr double kStart[3] = {5.9, 8.4, 9.0}, kLatency[3] = {0.0113, 0.0083, 0.0135}, kRate[3] = {0.012, 0.018, 0.048},
-                     kJoin[3] = {0.41, 0.14, 0.096};
+    constexpr double kStart[3] = {6.097, 7.606, 7.066}, kLatency[3] = {0.0089, 0.0092, 0.0165}, kRate[3] = {0.0185, 0.0165, 0.0443},
+                     kJoin[3] = {0.36, 0.288, 0.373};
     const int quantum = kRows[i] == 128 ? 64 : 128;
     const int64_t share =
         (std::max<int64_t>((static_cast<int64_t>(max_keys) + splits - 1) / splits, kMinKeys) + quantum - 1) / quantum * quantum;
     const int64_t parts = std::max<int64_t>((max_keys + share - 1) / share, 1);
-    const double keys = static_cast<double>(std::min<int64_t>(share, max_keys)) * (head_dim == 64 ? 0.375 : 1.0);
+    const double keys = static_cast<double>(std::min<int64_t>(share, max_keys)) * (head_dim == 64 ? 0.467 : 1.0);
     const double load = static_cast<double>(units) * parts / (2.0 * cus);
-    const double rounds = load > 1.0 ? load + 0.155 * (std::ceil(load) - load) : load;
-    double us = kStart[i] + std::pow(std::pow(kLatency[i] * keys, 1.34) + std::pow(kRate[i] * keys * rounds, 1.34), 1 / 1.34) +
-                1.37 * std::max(load - 1.0, 0.0);
-    if (parts > 1) us += 2.7 + kJoin[i] * parts * (single ? std::min(kRows[i], group) : kRows[i]) / 16.0 + 2.2 * load;
+    const double rounds = load > 1.0 ? load + 0.074 * (std::ceil(load) - load) : load;
+    double us = kStart[i] + std::pow(std::pow(kLatency[i] * keys, 1.5) + std::pow(kRate[i] * keys * rounds, 1.5), 1 / 1.5) +
+                1.945 * std::max(load - 1.0, 0.0);
+    if (parts > 1) us += 2.246 + kJoin[i] * parts * (single ? std::min(kRows[i], group) : kRows[i]) / 16.0 + 2.004 * load;
     return us;
 }
 
@@ -913,22 +927,28 @@ double cost_us(int i, int64_t units, int splits, int group, int head_dim, int ma
 extern "C" int tw4_paged_attention_plan(int tokens, int batch, int heads, int kv_heads, int head_dim, int max_query, int max_keys,
                                         int single, int cus, int* out) {
     TW4_REQUIRE(out && tokens >= 0 && batch >= 0 && kv_heads >= 1 && heads >= 1 && heads % kv_heads == 0 && head_dim >= 1 && cus >= 1 &&
-                    max_keys >= 0,
+                    max_keys >= 0 && max_query >= 0,
                 TW4_EINVAL, "paged_attention_plan: bad sizes");
     const int group = heads / kv_heads;
     double best = 0.0;
     int rows = 0, splits = 1;
     int64_t units = 0, part = 0;
     for (int i = 0; i < 3; ++i) {
+        // A tile no larger than a request's rows need (16 rows against 32, the fastest split of each: 3 new tokens of 32 + 8 heads over
+        // 2000 keys 12.8 us against 14.6, 60 of those 73.1 against 74.2, 33 requests of 16 rows 14.7 against 17.0; 3 of 16 rows over
+        // 8000 keys 28.2 against 26.4)
+        if (i > 0 && kRows[i - 1] >= static_cast<int64_t>(max_query) * group) break;
         const int64_t u = tile_slots(tokens, batch, group, kRows[i], single) * kv_heads;
         const int64_t floats = static_cast<int64_t>(single ? std::min(kRows[i], group) : kRows[i]) * (head_dim + kTileFloats);
+        // those that can have rows
+        const int64_t per = (static_cast<int64_t>(max_query) * group + kRows[i] - 1) / kRows[i], work = std::min(u, batch * per * kv_heads);
         // and what fills the CUs once or twice
-        const int once = static_cast<int>(u ? 2 * cus / u : 0), twice = static_cast<int>(u ? 4 * cus / u : 0);
+        const int once = static_cast<int>(work ? 2 * cus / work : 0), twice = static_cast<int>(work ? 4 * cus / work : 0);
         for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 64, once, twice}) {
             if (s < 1 || (s > 1 && (static_cast<int64_t>(s - 1) * kMinKeys >= max_keys || u * s * floats > kWorkspaceFloats ||
                                     u > TW4_AUTO_SPLIT_COUNTERS)))
                 continue;
-            const double us = cost_us(i, u, s, group, head_dim, max_keys, single, cus);
+            const double us = cost_us(i, work, s, group, head_dim, max_keys, single, cus);
             if (rows == 0 || us < best) best = us, rows = kRows[i], splits = s, units = u, part = floats;
         }
     }
@@ -954,9 +974,10 @@ extern "C" int tw4_paged_attention(const uint16_t* q, int64_t q_token, int64_t q
     TW4_REQUIRE(rows == 16 || rows == 32 || rows == 128, TW4_ECONFIG,
                 "paged_attention: tiles of 16, 32 or 128 rows (%d)", rows);
     TW4_REQUIRE(width >= 0 && num_pages >= 0 && static_cast<int64_t>(num_pages) * page_size < 1LL << 31 &&
-                    static_cast<int64_t>(width) * page_size < 1LL << 31,
-                TW4_EINVAL, "paged_attention: fewer than 2^31 slots (%d pages of %d, %d per request)", num_pages, page_size, width);
-    TW4_REQUIRE(static_cast<int64_t>(tokens) * heads < 1LL << 31, TW4_EINVAL, "paged_attention: too many rows (%d tokens)", tokens);
+                    static_cast<int64_t>(width) * page_size <= 1LL << 30,
+                TW4_EINVAL, "paged_attention: fewer than 2^31 slots, at most 2^30 keys of a request (%d pages of %d, %d per request)",
+                num_pages, page_size, width);
+    TW4_REQUIRE(static_cast<int64_t>(tokens) * heads <= 1LL << 30, TW4_EINVAL, "paged_attention: too many rows (%d tokens)", tokens);
     TW4_REQUIRE(starts || tokens == batch, TW4_EINVAL, "paged_attention: without query starts one token per request (%d, %d)",
                 tokens, batch);
     if (tokens == 0 || batch == 0) return TW4_OK;
@@ -971,7 +992,8 @@ extern "C" int tw4_paged_attention(const uint16_t* q, int64_t q_token, int64_t q
                 TW4_EINVAL, "paged_attention: strides must be multiples of 8");
     const int group = heads / kv_heads;
     const int64_t slots = tile_slots(tokens, batch, group, rows, !starts), units = slots * kv_heads;
-    TW4_REQUIRE(units < 1LL << 31 && splits >= 1 && splits <= 65535, TW4_EINVAL, "paged_attention: grid (%lld tiles, %d splits)",
+    // a launch has fewer than 2^32 threads along an axis
+    TW4_REQUIRE(units < 1LL << 24 && splits >= 1 && splits <= 65535, TW4_EINVAL, "paged_attention: grid (%lld tiles, %d splits)",
                 static_cast<long long>(units), splits);
     const int part_rows = starts ? rows : std::min(rows, group);
     if (splits > 1) {

@@ -8,7 +8,8 @@ A = sum_j w_j |v_j|:
                            sum_i |q_i k_i| (largest over the keys), once for the probability and once for their sum; the
                            exponential itself is good to 2^-22
     n 2^-23 A              the fp32 sums over the keys, numerator and denominator
-    n 2^-25 max |v|        (fp16) probabilities below 2^-14 are subnormal: half a step is 2^-25 of the largest"""
+    n 2^-31 max |v|        (fp16) probabilities are held times 2^6 at least, so below 2^-20 they are subnormal: half a step is 2^-31 of
+                           the largest"""
 
 from __future__ import annotations
 
@@ -37,7 +38,7 @@ def test_argument_errors_return_before_launch():
                               (7, 12, "multiples"), (8, 1 << 28, "2^31"), (12, 1 << 28, "2^31"), (8, 0, "without pages"),
                               (9, 48, "page_size"), (22, 30, "multiple"), (23, 0, "multiple"), (24, 96, "head_dim"), (25, 0.0, "scale"),
                               (25, float("nan"), "scale"), (25, -1.0, "scale"), (20, 1 << 28, "too many"), (14, None, "one token"),
-                              (27, 0, "splits"), (10, None, "null"), (13, None, "null")):
+                              (12, (1 << 26) + 1, "2^30"), (21, 1 << 22, "grid"), (27, 0, "splits"), (10, None, "null"), (13, None, "null")):
         args = _good()
         args[at] = value
         assert lib.tw4_paged_attention(*args, None) == w4_hip.TW4_EINVAL, (at, value)
@@ -76,6 +77,11 @@ def test_plan_fits_the_workspace():
         assert (splits == 1) == (floats == 0) == (counters == 0)
     assert _plan(1, 1, 32, 8, 128, 1, 100, 1)[1] == 1  # too few keys to split
     assert _plan(1, 1, 32, 8, 128, 1, 40000, 1)[1] > 8
+    # a tile is no larger than a request's rows need
+    for keys in (100, 2000, 40000):
+        for batch in (1, 5, 60):
+            assert _plan(batch * 3, batch, 32, 8, 128, 3, keys, 0)[0] == 16
+            assert _plan(batch * 8, batch, 32, 8, 128, 8, keys, 0)[0] <= 32
 
 
 def test_refusals_on_the_cpu():
@@ -116,7 +122,7 @@ def exact(q, k_cache, v_cache, table, lens, starts, scale=None, absent=()):
     pages, kv, page, _ = k_cache.shape
     group = heads // kv
     scale = d ** -0.5 if scale is None else scale
-    u, tiny = HALF_STEP[q.dtype], 2.0 ** -25 if q.dtype == torch.float16 else 0.0
+    u, tiny = HALF_STEP[q.dtype], 2.0 ** -31 if q.dtype == torch.float16 else 0.0
     out = torch.zeros(t, heads, d, dtype=torch.float64, device=q.device)
     tol = torch.zeros_like(out)
     for i, (n_keys, a, b) in enumerate(zip(lens.tolist(), starts.tolist(), starts.tolist()[1:])):
@@ -216,6 +222,22 @@ def test_large_and_small_scores(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("new", [1, 20, 129])
+def test_many_small_probabilities(dtype, new):
+    """30000 keys of 2^-25 of the largest each: less than fp16 has steps for, more than its rounding together."""
+    q, k, v, table, lens, starts = build([30000], [new], 1, 1, 64, dtype, 16, seed=11)
+    q.zero_()[..., 0] = 4.0
+    first = table[0, 0]
+    k.zero_()[first, 0, 0, 0] = 4.4
+    v.fill_(1.0)[first, 0, 0] = 0.0
+    got = check((q, k, v, table, lens, starts), scale=1.0)
+    assert (got > 5e-4).all()
+    if new == 1:
+        assert (check((q, k, v, table, lens, starts), scale=1.0, max_seq_len=30001) > 5e-4).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("new", [[1, 1, 1], [5, 3, 200]])
 def test_odd_values_reach_the_rows_that_see_them_only(new):
     """Infinities and NaN in keys and values of the chunk's later tokens leave its earlier ones as they are; behind the last key
@@ -257,6 +279,7 @@ def test_rows_without_a_key_and_rows_behind_the_last_request():
     table2 = table.clone()
     got = paged_attention(q, k, v, table2, lens2, starts)
     assert (got[:3] == 0).all() and (got[5:] == 0).all() and not (got[3:5] == 0).all(-1).any()
+    assert (paged_attention(q, k, v, table2, lens2 * 0 - 2 ** 31, starts) == 0).all()
     for bad in (-1, k.shape[0], 2 ** 31 - 1, -2 ** 31):  # entries that are no page
         table2 = table.clone()
         table2[0, 1], table2[1, 0], table2[2, 0] = bad, bad, bad
@@ -291,7 +314,7 @@ def test_strides_layouts_and_refusals():
         assert torch.equal(paged_attention(*other, lens, starts), want)
     ok = dict(q=q, k_cache=k, v_cache=v, page_table=table, seq_lens=lens, query_start=starts)
     for change, needle in ((dict(q=q.float()), "float16 or bfloat16"), (dict(q=q[..., :64]), "caches"), (dict(q=q[:, :6]), "multiple"),
-                           (dict(q=q.clone().requires_grad_()), "inference"), (dict(q=qkv.view(20, -1)[:, 4:1028].view(20, 8, 128)), "aligned"),
+                           (dict(q=q.clone().requires_grad_()), "inference"), (dict(v_cache=v.clone().requires_grad_()), "inference"), (dict(q=qkv.view(20, -1)[:, 4:1028].view(20, 8, 128)), "aligned"),
                            (dict(k_cache=k.half()), "caches of"), (dict(k_cache=k[:, :, :24], v_cache=v[:, :, :24]), "page size"),
                            (dict(v_cache=by_token[1]), "layout"), (dict(page_table=table.long()), "page_table"),
                            (dict(page_table=table.t()), "page_table"), (dict(seq_lens=lens[:1]), "seq_lens"),
