@@ -70,7 +70,7 @@ def fused_add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Te
 
 class HipOps:
     """The norm half of the reference's ops interface (python/tandem/layers/ops.py:62-120) on the
-    HIP kernels; the attention-side ops (RoPE) belong to another path."""
+    HIP kernels; the attention-side ops are in ``rotary`` and ``paged_attention``."""
 
     name = "hip"
 
