@@ -214,6 +214,56 @@ def test_every_split_and_tile(splits, rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("rows", [16, 32, 128])
+@pytest.mark.parametrize("heads,kv,d", [(40, 1, 128), (24, 2, 64), (8, 8, 128)])
+def test_single_tokens_in_every_tile(heads, kv, d, rows, splits):
+    args = build([1000, 40, 0, 300], [1] * 4, heads, kv, d, torch.float16, 16, seed=4)
+    q, k, v, table, lens, starts = args
+    out = torch.full_like(q, float("nan"))
+    ws = torch.empty(1 << 23, device="cuda")
+    locks = torch.zeros(1 << 12, dtype=torch.int32, device="cuda")
+    w4_hip.check(w4_hip.library().tw4_paged_attention(
+        q.data_ptr(), *q.stride()[:2], k.data_ptr(), v.data_ptr(), *k.stride()[:3], k.shape[0], k.shape[2], table.data_ptr(),
+        table.stride(0), table.shape[1], lens.data_ptr(), None, out.data_ptr(), ws.data_ptr(), ws.numel(),
+        locks.data_ptr(), locks.numel(), q.shape[0], 4, heads, kv, d, d ** -0.5, rows, splits, 0,
+        torch.cuda.current_stream().cuda_stream))
+    want, tol = exact(*args)
+    assert ((out.double() - want).abs() <= tol).all() and not locks.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,most", [(65, 40), (300, 70), (4200, 3)])
+def test_many_requests(batch, most):
+    """More requests than a wavefront looks at in one step, or in two, of no token, one, and several tiles."""
+    rng = random.Random(batch)
+    new = [rng.choice((0, 1, 1, 2, rng.randint(0, most))) for _ in range(batch)]
+    context = [rng.randint(0, 40) for _ in range(batch)]
+    args = build(context, new, 2, 1, 64, torch.float16, 16, seed=12)
+    check(args)
+    check(args, max_query_len=most, max_seq_len=40 + most)
+
+
+@pytest.mark.gpu
+def test_bounds_and_starts_that_do_not_hold_and_rows_of_nan():
+    """max_query_len and max_seq_len only divide the work; a query of NaN stays alone."""
+    args = build([3000, 10, 100], [1, 150, 9], 8, 2, 128, torch.float16, 16, seed=14)
+    for bounds in ((1, 1), (0, 0), (-3, -3), (10 ** 9, 10 ** 9), (2, 10 ** 5), (200, 16)):
+        check(args, max_query_len=bounds[0], max_seq_len=bounds[1])
+    # starts that are none: the rows are anything, and the calls after it right (no counter stays up)
+    for wrong in ([5, 0, 900, -7], [0, 160, 3, 160], [160, 160, 0, 0], [-2 ** 31, 2 ** 31 - 1, 0, 70]):
+        assert paged_attention(*args[:5], torch.tensor(wrong, dtype=torch.int32, device="cuda")).shape == args[0].shape
+        check(args)
+    want, tol = exact(*args)
+    q = args[0].clone()
+    q[77, 3], q[0, 0], q[155, 7] = float("nan"), float("inf"), float("nan")
+    got = paged_attention(q, *args[1:])
+    hit = torch.zeros(q.shape[:2], dtype=torch.bool, device="cuda")
+    hit[77, 3] = hit[0, 0] = hit[155, 7] = True
+    assert ((got.double() - want).abs() <= tol)[~hit].all() and not torch.isfinite(got[hit]).any()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_large_and_small_scores(dtype):
     """Scores far apart (one key takes all), all alike, and a scale of the caller's."""
