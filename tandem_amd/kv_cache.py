@@ -81,7 +81,7 @@ def plan_pages(context_lens: torch.Tensor, query_lens: torch.Tensor, page_table:
         ("query_lens", layout(query_lens), None), ("taken", layout(taken), 1), *outs)
     # one allocation for what is new
     sizes = (batch + 1, num_tokens, num_tokens, 4, 1 if taken_out is None else 0, batch if seq_lens_out is None else 0)
-    flat = torch.empty(sum(sizes), dtype=torch.int32, device=page_table.device)
+    flat = page_table.new_empty(sum(sizes))
     query_start, positions, slots, counts, left, lens = flat.split_with_sizes(sizes)
     if seq_lens_out is not None:
         lens = seq_lens_out

@@ -104,9 +104,9 @@ def _run(who: str, qkv, positions, table, num_heads: int, num_kv_heads: int, q_w
     if not w4_hip.plain(qkv) or (slots is not None and torch.is_grad_enabled() and (k.requires_grad or v.requires_grad)):
         raise RuntimeError(f"{who}: inference only, no gradient, transform or tracer can follow qkv or the caches")
     tokens = qkv.shape[0]
-    q = torch.empty((tokens, num_heads, d), dtype=qkv.dtype, device=qkv.device)
+    q = qkv.new_empty((tokens, num_heads, d))
     if slots is None:
-        k = torch.empty((tokens, num_kv_heads, d), dtype=qkv.dtype, device=qkv.device)
+        k = qkv.new_empty((tokens, num_kv_heads, d))
     if tokens:
         xp, tp, kp, vp = qkv.data_ptr(), table.data_ptr(), k.data_ptr(), 0 if v is None else v.data_ptr()
         qw, kw = 0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr()
