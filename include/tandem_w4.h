@@ -314,7 +314,8 @@ int tw4_release_pages(const int32_t* ended, int count, int32_t* table, int64_t t
 /* Causal attention of new tokens over a paged cache: q [tokens, heads, head_dim] (strides q_token, q_head), caches as
  * tw4_norm_rope writes them, table [batch, width] int32 (row stride table_stride), lens [batch] keys of each request (its new tokens
  * among them), starts [batch + 1] first row of each request, or NULL: one row per request (tokens == batch). out [tokens, heads,
- * head_dim], fp16 (bf16 = 1: bfloat16). Row t of a request's n sees keys j <= len - n + t. Entries of the table that are no page,
+ * head_dim], fp16 (bf16 = 1: bfloat16). Row t of a request's n = starts[i + 1] - starts[i] sees keys j <= len - n + t; starts may run past
+ * tokens, the rows that are there are computed. Entries of the table that are no page,
  * and keys behind its width, are left out; a row that sees no key is zero; rows from starts[batch] on are not written. No
  * content of table, lens or starts makes it touch anything outside of the operands. rows, splits: from tw4_paged_attention_plan
  * (any of its values is valid for any call); splits > 1 takes ws and locks (zero before the first call, and after each; calls

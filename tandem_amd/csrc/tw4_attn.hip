@@ -56,7 +56,7 @@ constexpr int kMinKeys = 128;  // of a split
 // A tile of rows: its request, first row, and the keys it can see.
 struct Tile {
     int request, first, rows;  // rows of the request from `first` on, at least 1
-    int start, len, fresh;     // the request's first token, keys, new tokens
+    int start, before;         // the request's first token; keys before its new tokens' own: token t sees before + t and all below
 };
 
 // Slot s of the grid is the first tile of request s, and from slot `batch` on a further one: of request i, the last with
@@ -67,7 +67,8 @@ struct Tile {
 // of 8, 32 + 8 heads, 3000 keys: 108 against 88).
 template <int B>
 __device__ __forceinline__ bool find_tile(const AttnArgs& a, int slot, int lane, Tile& t) {
-    int start, fresh;
+    int start, have;  // tokens of the request that q has
+    int64_t fresh;    // new tokens that its keys count, those behind q's last row among them
     if (a.starts) {
         t.request = slot, t.first = 0;
         if (slot >= a.batch) {
@@ -85,19 +86,21 @@ __device__ __forceinline__ bool find_tile(const AttnArgs& a, int slot, int lane,
             const int64_t base = static_cast<int64_t>(min(max(a.starts[t.request], 0), a.tokens)) * a.group / B;
             t.first = (slot - static_cast<int>(base) + 1) * B;
         }
-        start = min(max(a.starts[t.request], 0), a.tokens);
-        fresh = min(max(a.starts[t.request + 1], start), a.tokens) - start;
+        const int from = a.starts[t.request], to = a.starts[t.request + 1];
+        start = min(max(from, 0), a.tokens);
+        have = min(max(to, start), a.tokens) - start;
+        fresh = static_cast<int64_t>(to) - from;
     } else {
         const int per = (a.group + B - 1) / B;
         t.request = slot / per;
         start = t.request;
-        fresh = 1;
+        have = 1, fresh = 1;
         t.first = (slot - t.request * per) * B;
     }
     t.start = start;
-    t.fresh = fresh;
-    t.len = max(a.lens[t.request], 0);
-    t.rows = fresh * a.group - t.first;
+    // with rows there is fresh >= have, so before + t < len; no token number reaches 2^30, so what lies further down sees nothing either
+    t.before = static_cast<int>(max(max(a.lens[t.request], 0) - fresh, static_cast<int64_t>(-(1 << 30))));
+    t.rows = have * a.group - t.first;
     return t.first >= 0 && t.rows > 0;
 }
 
@@ -165,7 +168,7 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(AttnArgs a) {
         const int r = t.first + 16 * m + c16;
         const bool there = 16 * m + c16 < t.rows;
         const int tok = r / a.group, g = r - tok * a.group;
-        limit[m] = there ? t.len - t.fresh + tok : -1;
+        limit[m] = there ? t.before + tok : -1;
         if (there) low = min(low, limit[m]), high = max(high, limit[m]);
         const uint16_t* src = a.q + (t.start + tok) * a.q_token + (head * a.group + g) * a.q_head + 8 * g4;
 #pragma unroll
@@ -519,14 +522,14 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {
 
     const int r = t.first + 32 * wave + c32, tok = r / a.group;
     const bool mine = 32 * wave + c32 < t.rows, active = 32 * wave < t.rows;  // this lane, this wavefront has a row
-    const int limit = mine ? t.len - t.fresh + tok : -1;
+    const int limit = mine ? t.before + tok : -1;
     u4 q[KS];
     {
         const uint16_t* src = a.q + (t.start + tok) * a.q_token + (head * a.group + r - tok * a.group) * a.q_head + 8 * h;
 #pragma unroll
         for (int e = 0; e < KS; ++e) q[e] = mine ? *reinterpret_cast<const u4*>(src + 16 * e) : u4{0, 0, 0, 0};
     }
-    const int tile_high = t.len - t.fresh + (t.first + min(t.rows, B) - 1) / a.group;  // the last key a row of the tile sees
+    const int tile_high = t.before + (t.first + min(t.rows, B) - 1) / a.group;  // the last key a row of the tile sees
     const int end = static_cast<int>(min(static_cast<int64_t>(tile_high) + 1, static_cast<int64_t>(a.width) << a.shift));
     int begin = 0, stop = max(end, 0), parts = 1;
     if (a.splits > 1 && end > 0) {
@@ -683,7 +686,7 @@ __global__ void __launch_bounds__(256, 2) chunk_kernel(AttnArgs a) {
     };
 
     // Keys below `clear` are seen by every row and lie in pages that are there.
-    int clear = min(t.len - t.fresh + t.first / a.group + 1, stop);
+    int clear = min(t.before + t.first / a.group + 1, stop);
     int ahead = 0;  // the table's entry of this wavefront's keys of the next tile
     if (begin < stop) {
         const int64_t at = place_of(begin, entry(begin + 16 * wave));

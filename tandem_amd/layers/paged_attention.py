@@ -62,7 +62,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     """Attention of q [T, heads, head_dim] (float16 or bfloat16, head_dim 64 or 128) over caches [pages, KV heads, page size,
     head_dim]. Request i of B has seq_lens[i] keys, the last of them its new tokens' own: key j lies in page
     page_table[i, j // page size]. Its new tokens are rows query_start[i] .. query_start[i + 1] - 1 of q, and the t-th of
-    n sees the keys j <= seq_lens[i] - n + t. query_start None: one new token per request (T == B). Query head h reads KV head
+    n = query_start[i + 1] - query_start[i] sees the keys j <= seq_lens[i] - n + t; of a request that runs past row T - 1 the tokens
+    that have a row are computed. query_start None: one new token per request (T == B). Query head h reads KV head
     h // (heads / KV heads). scale: of the scores, head_dim^-0.5 by default.
 
     page_table int32 [B, pages per request] (any row stride), seq_lens int32 [B], query_start int32 [B + 1], ascending from 0.

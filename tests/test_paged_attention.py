@@ -428,3 +428,32 @@ def test_streams_and_graphs():
         assert torch.equal(outs[0], paged_attention(*sets[0])), cut
         w, tol = exact(*sets[0])
         assert ((outs[0].double() - w).abs() <= tol).all()
+
+
+def _direct(args, rows, splits):
+    """paged_attention with a tile and a number of splits of the caller's."""
+    q, k, v, table, lens, starts = args
+    out = torch.full_like(q, float("nan"))
+    ws = torch.empty(1 << 25, device="cuda")
+    locks = torch.zeros(1 << 12, dtype=torch.int32, device="cuda")
+    w4_hip.check(w4_hip.library().tw4_paged_attention(
+        q.data_ptr(), *q.stride()[:2], k.data_ptr(), v.data_ptr(), *k.stride()[:3], k.shape[0], k.shape[2], table.data_ptr(),
+        table.stride(0), table.shape[1], lens.data_ptr(), starts.data_ptr(), out.data_ptr(), ws.data_ptr(), ws.numel(),
+        locks.data_ptr(), locks.numel(), q.shape[0], lens.shape[0], q.shape[1], k.shape[1], q.shape[2], q.shape[2] ** -0.5, rows, splits,
+        int(q.dtype == torch.bfloat16), torch.cuda.current_stream().cuda_stream))
+    assert not locks.any()
+    return out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("rows", [16, 32, 128])
+def test_rows_of_a_step_cut_short_see_no_later_key(rows, splits):
+    """q has fewer rows than query_start says (plan_pages counts such tokens): those it has see what they see in the whole step."""
+    q, k, v, table, lens, starts = args = build([40, 1000, 7], [5, 150, 9], 8, 2, 128, torch.float16, 16, seed=31)
+    want, tol = exact(*args)
+    for cut in (1, 3, 5, 6, 100, 154, 155, 160):
+        got = _direct((q[:cut], k, v, table, lens, starts), rows, splits)
+        assert ((got.double() - want[:cut]).abs() <= tol[:cut]).all(), cut
+        got = paged_attention(q[:cut], k, v, table, lens, starts)
+        assert ((got.double() - want[:cut]).abs() <= tol[:cut]).all(), cut
