@@ -306,6 +306,12 @@ int tw4_plan_pages(const int32_t* context, const int32_t* fresh, int32_t* table,
                    int32_t* starts, int32_t* lens, int32_t* positions, int32_t* slots, int32_t* counts, int batch,
                    int tokens, void* stream);
 
+/* tw4_plan_pages for a cache that keeps its requests' lengths from step to step: context and taken are advanced in place, and lens
+ * (another array) are the step's own, which later steps leave as they are. */
+int tw4_plan_step(int32_t* context, const int32_t* fresh, int32_t* table, int64_t table_stride, int width, const int32_t* free_pages,
+                  int n_free, int32_t* taken, int page_size, int32_t* starts, int32_t* lens, int32_t* positions, int32_t* slots,
+                  int32_t* counts, int batch, int tokens, void* stream);
+
 /* The pages of requests ended[0 .. count) back to the list, in place: *taken falls by their number, their rows of the table become
  * -1 and their lengths 0. Indices outside of 0 .. batch - 1 are passed over. */
 int tw4_release_pages(const int32_t* ended, int count, int32_t* table, int64_t table_stride, int width, int32_t* lens,

@@ -33,6 +33,7 @@ struct PageArgs {
     int32_t* positions;
     int32_t* slots;
     int32_t* counts;
+    int32_t* advance;  // tw4_plan_step: the requests' lengths for the next step, else null
     int batch, tokens, width, n_free, shift;
 };
 
@@ -114,6 +115,7 @@ __global__ void __launch_bounds__(kThreads) pages_kernel(PageArgs a, int rows) {
             starts[i] = sum_n, first[i] = sum_need;
             a.starts[i] = sum_n;
             a.lens[i] = context[i] + n[j];  // the lengths' arrays may be one: read above, written here
+            if (a.advance) a.advance[i] = context[i] + n[j];
             sum_n += n[j], sum_need += need[j];
         }
     }
@@ -183,31 +185,45 @@ __global__ void __launch_bounds__(kThreads) release_kernel(const int32_t* ended,
 
 using namespace tw4;
 
+static int plan(const char* who, PageArgs a, int page_size, hipStream_t st) {
+    a.shift = page_shift(page_size);
+    TW4_REQUIRE(a.shift >= 0, TW4_EINVAL, "%s: page_size 16, 32, 64, 128 or 256 (%d)", who, page_size);
+    TW4_REQUIRE(a.batch >= 1 && a.batch <= kMaxBatch, TW4_EINVAL, "%s: 1 to %d requests (%d)", who, kMaxBatch, a.batch);
+    TW4_REQUIRE(a.tokens >= 0 && a.tokens < 1 << 30, TW4_EINVAL, "%s: 0 <= tokens < 2^30 (%d)", who, a.tokens);
+    TW4_REQUIRE(a.width >= 0 && a.n_free >= 0 && a.table_stride >= a.width && static_cast<int64_t>(a.batch) * a.width < 1LL << 31,
+                TW4_EINVAL, "%s: a table of fewer than 2^31 entries whose rows do not overlap (width %d, stride %lld)", who,
+                a.width, static_cast<long long>(a.table_stride));
+    TW4_REQUIRE(a.context && a.fresh && a.taken && a.taken_out && a.starts && a.lens && a.counts && (a.table || !a.width) &&
+                    (a.free_pages || !a.n_free) && ((a.positions && a.slots) || !a.tokens),
+                TW4_EINVAL, "%s: null pointer", who);
+    const bool one = a.tokens <= kInline;
+    pages_kernel<<<1, kThreads, 0, st>>>(a, one ? a.tokens : 0);
+    TW4_LAUNCH_CHECK("plan_pages: launch");
+    if (!one) {
+        rows_kernel<<<(a.tokens + 255) / 256, 256, 0, st>>>(a);
+        TW4_LAUNCH_CHECK("plan_pages: launch");
+    }
+    return TW4_OK;
+}
+
 extern "C" int tw4_plan_pages(const int32_t* context, const int32_t* fresh, int32_t* table, int64_t table_stride, int width,
                               const int32_t* free_pages, int n_free, const int32_t* taken, int32_t* taken_out, int page_size,
                               int32_t* starts, int32_t* lens, int32_t* positions, int32_t* slots, int32_t* counts, int batch,
                               int tokens, void* stream) {
-    const int shift = page_shift(page_size);
-    TW4_REQUIRE(shift >= 0, TW4_EINVAL, "plan_pages: page_size 16, 32, 64, 128 or 256 (%d)", page_size);
-    TW4_REQUIRE(batch >= 1 && batch <= kMaxBatch, TW4_EINVAL, "plan_pages: 1 to %d requests (%d)", kMaxBatch, batch);
-    TW4_REQUIRE(tokens >= 0 && tokens < 1 << 30, TW4_EINVAL, "plan_pages: 0 <= tokens < 2^30 (%d)", tokens);
-    TW4_REQUIRE(width >= 0 && n_free >= 0 && table_stride >= width && static_cast<int64_t>(batch) * width < 1LL << 31,
-                TW4_EINVAL, "plan_pages: a table of fewer than 2^31 entries whose rows do not overlap (width %d, stride %lld)",
-                width, static_cast<long long>(table_stride));
-    TW4_REQUIRE(context && fresh && taken && taken_out && starts && lens && counts && (table || !width) &&
-                    (free_pages || !n_free) && ((positions && slots) || !tokens),
-                TW4_EINVAL, "plan_pages: null pointer");
-    PageArgs a{context, fresh, table, table_stride, free_pages, taken, taken_out, starts, lens, positions, slots, counts,
-               batch, tokens, width, n_free, shift};
-    auto st = static_cast<hipStream_t>(stream);
-    const bool one = tokens <= kInline;
-    pages_kernel<<<1, kThreads, 0, st>>>(a, one ? tokens : 0);
-    TW4_LAUNCH_CHECK("plan_pages: launch");
-    if (!one) {
-        rows_kernel<<<(tokens + 255) / 256, 256, 0, st>>>(a);
-        TW4_LAUNCH_CHECK("plan_pages: launch");
-    }
-    return TW4_OK;
+    return plan("plan_pages",
+                PageArgs{context, fresh, table, table_stride, free_pages, taken, taken_out, starts, lens, positions, slots, counts,
+                         nullptr, batch, tokens, width, n_free, 0},
+                page_size, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int tw4_plan_step(int32_t* context, const int32_t* fresh, int32_t* table, int64_t table_stride, int width,
+                             const int32_t* free_pages, int n_free, int32_t* taken, int page_size, int32_t* starts, int32_t* lens,
+                             int32_t* positions, int32_t* slots, int32_t* counts, int batch, int tokens, void* stream) {
+    TW4_REQUIRE(lens != context, TW4_EINVAL, "plan_step: the step's lengths and the requests' must be two arrays");
+    return plan("plan_step",
+                PageArgs{context, fresh, table, table_stride, free_pages, taken, taken, starts, lens, positions, slots, counts,
+                         context, batch, tokens, width, n_free, 0},
+                page_size, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int tw4_release_pages(const int32_t* ended, int count, int32_t* table, int64_t table_stride, int width,

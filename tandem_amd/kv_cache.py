@@ -2,7 +2,7 @@
 list of the free ones, a table of each request's pages, and the positions and slots of a step's tokens from the requests' lengths
 alone. Nothing is read back: a step, with its pages, can be captured in a HIP graph and replayed.
 
-    plan_pages         pages, positions and slots of one step (tw4_plan_pages)
+    plan_pages         pages, positions and slots of one step (tw4_plan_pages; a PagedKVCache's own, tw4_plan_step)
     release_pages      pages of ended requests back to the list (tw4_release_pages)
     PagedKVCache       keys and values of every layer, the table and the lists
     PagedBatch         one step over a cache, as tandem_amd.model's attention takes it
@@ -115,7 +115,8 @@ def release_pages(ended: torch.Tensor, context_lens: torch.Tensor, page_table: t
 
 @dataclass(frozen=True)
 class PagedBatch:
-    """One step over a PagedKVCache: which tokens, where they go, and what they may see."""
+    """One step over a PagedKVCache: which tokens, where they go, and what they may see. Its tensors but page_table, the cache's, are its
+    own, so the next steps may be planned before it has run. Its lanes are released after it has run: released pages go to others."""
 
     cache: "PagedKVCache"
     page_table: torch.Tensor
@@ -172,10 +173,21 @@ class PagedKVCache:
         if query_lens.dim() != 1 or not 1 <= query_lens.numel() <= self.max_requests:
             raise RuntimeError(f"PagedKVCache.plan: query_lens [1 .. {self.max_requests}] expected (got {tuple(query_lens.shape)})")
         b = query_lens.numel()
-        lens = self.context_lens[:b]
-        plan = plan_pages(lens, query_lens, self.page_table[:b], self.free_pages, self.taken, self.page_size, num_tokens,
-                          seq_lens_out=lens, taken_out=self.taken)
-        return PagedBatch(self, self.page_table[:b], lens, plan.query_start, plan.positions, plan.slots, plan.counts,
+        table = self.page_table[:b]
+        _, width, stride, n_free, index = _checked(
+            "PagedKVCache.plan", layout(table), layout(self.free_pages), self.page_size, num_tokens,
+            ("query_lens", layout(query_lens), None), ("context_lens", layout(self.context_lens), self.max_requests),
+            ("taken", layout(self.taken), 1))
+        sizes = (b + 1, num_tokens, num_tokens, 4, b)
+        flat = self.page_table.new_empty(sum(sizes))
+        query_start, positions, slots, counts, lens = flat.split_with_sizes(sizes)
+        base = flat.data_ptr()
+        with w4_hip.on_device(index):
+            w4_hip.check(w4_hip.library().tw4_plan_step(
+                self.context_lens.data_ptr(), query_lens.data_ptr(), table.data_ptr(), stride, width, self.free_pages.data_ptr(), n_free,
+                self.taken.data_ptr(), self.page_size, base, lens.data_ptr(), base + 4 * (b + 1), base + 4 * (b + 1 + num_tokens),
+                base + 4 * (b + 1 + 2 * num_tokens), b, num_tokens, w4_hip.raw_stream(index)))
+        return PagedBatch(self, table, lens, query_start, positions, slots, counts,
                           num_tokens if max_query_len is None else max_query_len,
                           self.max_seq_len if max_seq_len is None else max_seq_len)
 

@@ -204,3 +204,25 @@ def test_cache_lives_through_many_steps():
         held = [p for i, r in enumerate(cache.page_table.tolist()) for p in r[:-(-lens[i] // 16)]]
         left = cache.free_pages.tolist()[int(cache.taken):]
         assert sorted(held + left) == list(range(64)), step
+
+
+@pytest.mark.gpu
+def test_a_batch_keeps_its_lengths_when_the_next_is_planned():
+    cache = kv_cache.PagedKVCache(1, 1, 64, num_pages=16, max_requests=3, max_seq_len=96)
+    first = cache.plan(_int([3, 20, 0]), 23)
+    second = cache.plan(_int([1, 30, 5]), 36)
+    assert first.seq_lens.tolist() == [3, 20, 0] and second.seq_lens.tolist() == [4, 50, 5]
+    assert cache.context_lens.tolist() == [4, 50, 5] and second.counts.tolist() == [36, 3, 0, 0]
+    assert second.positions.tolist() == [3, *range(20, 50), *range(5)]
+
+
+def test_step_refuses_bad_arguments():
+    lib, p = w4_hip.library(), ctypes.c_void_p(4096)
+    #       context fresh table stride width free n_free taken size starts lens pos slots counts batch tokens
+    good = [p, p, p, 10, 10, p, 5, p, 16, p, ctypes.c_void_p(8192), p, p, p, 4, 4]
+    for at, value, needle in ((8, 12, "page_size"), (14, 0, "requests"), (14, 4097, "requests"), (15, -1, "tokens"), (4, 11, "overlap"),
+                              (0, None, "null"), (7, None, "null"), (13, None, "null"), (6, -1, "overlap"), (10, p, "two arrays")):
+        args = list(good)
+        args[at] = value
+        assert lib.tw4_plan_step(*args, None) == w4_hip.TW4_EINVAL, (at, value)
+        assert needle in lib.tw4_last_error().decode() and "plan_step" in lib.tw4_last_error().decode(), (at, value)
