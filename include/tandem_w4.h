@@ -307,7 +307,9 @@ int tw4_plan_pages(const int32_t* context, const int32_t* fresh, int32_t* table,
                    int tokens, void* stream);
 
 /* tw4_plan_pages for a cache that keeps its requests' lengths from step to step: context and taken are advanced in place, and lens
- * (another array) are the step's own, which later steps leave as they are. */
+ * (another array) are the step's own, which later steps leave as they are. The table's entries behind a request's length are its pages or
+ * -1: where context was taken back (tokens that were not accepted) the pages stay in their places, and only entries that are -1 take
+ * new ones. */
 int tw4_plan_step(int32_t* context, const int32_t* fresh, int32_t* table, int64_t table_stride, int width, const int32_t* free_pages,
                   int n_free, int32_t* taken, int page_size, int32_t* starts, int32_t* lens, int32_t* positions, int32_t* slots,
                   int32_t* counts, int batch, int tokens, void* stream);
@@ -315,6 +317,10 @@ int tw4_plan_step(int32_t* context, const int32_t* fresh, int32_t* table, int64_
 /* The pages of requests ended[0 .. count) back to the list, in place: *taken falls by their number, their rows of the table become
  * -1 and their lengths 0. Indices outside of 0 .. batch - 1 are passed over. */
 int tw4_release_pages(const int32_t* ended, int count, int32_t* table, int64_t table_stride, int width, int32_t* lens,
+                      int batch, int32_t* free_pages, int n_free, int32_t* taken, int page_size, void* stream);
+
+/* tw4_release_pages for tw4_plan_step's table: every page of the requests' rows goes back, also those behind their lengths. */
+int tw4_release_lanes(const int32_t* ended, int count, int32_t* table, int64_t table_stride, int width, int32_t* lens,
                       int batch, int32_t* free_pages, int n_free, int32_t* taken, int page_size, void* stream);
 
 /* Causal attention of new tokens over a paged cache: q [tokens, heads, head_dim] (strides q_token, q_head), caches as

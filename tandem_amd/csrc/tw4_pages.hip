@@ -88,6 +88,9 @@ __device__ __forceinline__ void scan2(int& x, int& y, int& tx, int& ty, int (*pa
     y = by + sy - y;
 }
 
+// STEP: the table is a cache's own, so an entry behind a request's length is a page it already has (its length was taken back): it stays, and
+// only entries that are none (-1) take pages, in the order of their places.
+template <bool STEP>
 __global__ void __launch_bounds__(kThreads) pages_kernel(PageArgs a, int rows) {
     __shared__ int part[kThreads / 64][2];
     __shared__ int32_t starts[kMaxBatch + 1], first[kMaxBatch + 1], context[kMaxBatch];
@@ -115,23 +118,52 @@ __global__ void __launch_bounds__(kThreads) pages_kernel(PageArgs a, int rows) {
             starts[i] = sum_n, first[i] = sum_need;
             a.starts[i] = sum_n;
             a.lens[i] = context[i] + n[j];  // the lengths' arrays may be one: read above, written here
-            if (a.advance) a.advance[i] = context[i] + n[j];
+            if constexpr (STEP) a.advance[i] = context[i] + n[j];
             sum_n += n[j], sum_need += need[j];
         }
     }
     if (tid == 0) {
         starts[a.batch] = total, first[a.batch] = pages;
         a.starts[a.batch] = total;
-        const int given = min(pages, a.n_free - taken);
-        *a.taken_out = taken + given;
-        a.counts[0] = total, a.counts[1] = given, a.counts[2] = pages - given;
-        a.counts[3] = max(total - a.tokens, 0);
     }
     __syncthreads();
-    for (int p = tid; p < pages; p += kThreads) {
-        const int i = request_of(first, a.batch, p);
-        const int from = taken + p;
-        a.table[i * a.table_stride + pages_of(context[i], a) + (p - first[i])] = from < a.n_free ? a.free_pages[from] : -1;
+    int missing = 0;  // of the places so far; without STEP all are
+    if constexpr (STEP) {
+        const int lane = tid & 63, wave = tid >> 6;
+        for (int p0 = 0; p0 < pages; p0 += kThreads) {
+            const int p = p0 + tid;
+            int32_t* entry = nullptr;
+            if (p < pages) {
+                const int i = request_of(first, a.batch, p);
+                entry = a.table + i * a.table_stride + pages_of(context[i], a) + (p - first[i]);
+            }
+            const bool none = entry && *entry < 0;
+            const uint64_t all = __ballot(none);
+            if (lane == 0) part[wave][0] = __popcll(all);
+            __syncthreads();
+            int before = missing;
+#pragma unroll
+            for (int w = 0; w < kThreads / 64; ++w) {
+                if (w < wave) before += part[w][0];
+                missing += part[w][0];
+            }
+            const int64_t from = static_cast<int64_t>(taken) + before + __popcll(all & ((1ULL << lane) - 1));
+            if (none) *entry = from < a.n_free ? a.free_pages[from] : -1;
+            __syncthreads();
+        }
+    } else {
+        missing = pages;
+        for (int p = tid; p < pages; p += kThreads) {
+            const int i = request_of(first, a.batch, p);
+            const int from = taken + p;
+            a.table[i * a.table_stride + pages_of(context[i], a) + (p - first[i])] = from < a.n_free ? a.free_pages[from] : -1;
+        }
+    }
+    if (tid == 0) {
+        const int given = min(missing, a.n_free - taken);
+        *a.taken_out = taken + given;
+        a.counts[0] = total, a.counts[1] = given, a.counts[2] = missing - given;
+        a.counts[3] = max(total - a.tokens, 0);
     }
     if (rows == 0) return;
     __threadfence_block();
@@ -145,8 +177,11 @@ __global__ void __launch_bounds__(256) rows_kernel(PageArgs a) {
     if (t < a.tokens) place_row(a, a.starts, [&](int i) { return a.lens[i] - (a.starts[i + 1] - a.starts[i]); }, t);
 }
 
-// The pages of the listed requests go back to the front of what is left of the free list, in order of request and page;
-// their rows of the table become -1 and their lengths 0. One workgroup: it runs when requests end.
+// The pages of the listed requests go back to the front of what is left of the free list, each request's (1024 of them at a time) before
+// those of the one before it;
+// their rows of the table become -1 and their lengths 0. WHOLE: every page of the row, not those of the request's length only. One
+// workgroup: it runs when requests end.
+template <bool WHOLE>
 __global__ void __launch_bounds__(kThreads) release_kernel(const int32_t* ended, int count, int32_t* table, int64_t table_stride,
                                                            int width, int32_t* lens, int batch, int32_t* free_pages, int n_free,
                                                            int32_t* taken, int shift) {
@@ -156,8 +191,9 @@ __global__ void __launch_bounds__(kThreads) release_kernel(const int32_t* ended,
     for (int e = 0; e < count; ++e) {
         const int i = ended[e];
         if (i < 0 || i >= batch) continue;  // uniform
-        const int held = static_cast<int>(min((static_cast<int64_t>(max(lens[i], 0)) + (1 << shift) - 1) >> shift,
-                                              static_cast<int64_t>(width)));
+        const int held = WHOLE ? width
+                               : static_cast<int>(min((static_cast<int64_t>(max(lens[i], 0)) + (1 << shift) - 1) >> shift,
+                                                      static_cast<int64_t>(width)));
         for (int p0 = 0; p0 < width; p0 += kThreads) {
             const int p = p0 + static_cast<int>(threadIdx.x);
             const int id = p < held ? table[i * table_stride + p] : -1;
@@ -197,7 +233,10 @@ static int plan(const char* who, PageArgs a, int page_size, hipStream_t st) {
                     (a.free_pages || !a.n_free) && ((a.positions && a.slots) || !a.tokens),
                 TW4_EINVAL, "%s: null pointer", who);
     const bool one = a.tokens <= kInline;
-    pages_kernel<<<1, kThreads, 0, st>>>(a, one ? a.tokens : 0);
+    if (a.advance)
+        pages_kernel<true><<<1, kThreads, 0, st>>>(a, one ? a.tokens : 0);
+    else
+        pages_kernel<false><<<1, kThreads, 0, st>>>(a, one ? a.tokens : 0);
     TW4_LAUNCH_CHECK("plan_pages: launch");
     if (!one) {
         rows_kernel<<<(a.tokens + 255) / 256, 256, 0, st>>>(a);
@@ -226,17 +265,32 @@ extern "C" int tw4_plan_step(int32_t* context, const int32_t* fresh, int32_t* ta
                 page_size, static_cast<hipStream_t>(stream));
 }
 
+static int release(const char* who, bool whole, const int32_t* ended, int count, int32_t* table, int64_t table_stride, int width,
+                   int32_t* lens, int batch, int32_t* free_pages, int n_free, int32_t* taken, int page_size, hipStream_t st) {
+    const int shift = page_shift(page_size);
+    TW4_REQUIRE(shift >= 0, TW4_EINVAL, "%s: page_size 16, 32, 64, 128 or 256 (%d)", who, page_size);
+    TW4_REQUIRE(count >= 0 && batch >= 1 && width >= 0 && n_free >= 0 && table_stride >= width, TW4_EINVAL,
+                "%s: bad sizes (%d of %d requests, width %d)", who, count, batch, width);
+    if (count == 0 || width == 0) return TW4_OK;
+    TW4_REQUIRE(ended && table && lens && taken && (free_pages || !n_free), TW4_EINVAL, "%s: null pointer", who);
+    if (whole)
+        release_kernel<true><<<1, kThreads, 0, st>>>(ended, count, table, table_stride, width, lens, batch, free_pages, n_free, taken, shift);
+    else
+        release_kernel<false><<<1, kThreads, 0, st>>>(ended, count, table, table_stride, width, lens, batch, free_pages, n_free, taken, shift);
+    TW4_LAUNCH_CHECK("release_pages: launch");
+    return TW4_OK;
+}
+
 extern "C" int tw4_release_pages(const int32_t* ended, int count, int32_t* table, int64_t table_stride, int width,
                                  int32_t* lens, int batch, int32_t* free_pages, int n_free, int32_t* taken, int page_size,
                                  void* stream) {
-    const int shift = page_shift(page_size);
-    TW4_REQUIRE(shift >= 0, TW4_EINVAL, "release_pages: page_size 16, 32, 64, 128 or 256 (%d)", page_size);
-    TW4_REQUIRE(count >= 0 && batch >= 1 && width >= 0 && n_free >= 0 && table_stride >= width, TW4_EINVAL,
-                "release_pages: bad sizes (%d of %d requests, width %d)", count, batch, width);
-    if (count == 0 || width == 0) return TW4_OK;
-    TW4_REQUIRE(ended && table && lens && taken && (free_pages || !n_free), TW4_EINVAL, "release_pages: null pointer");
-    release_kernel<<<1, kThreads, 0, static_cast<hipStream_t>(stream)>>>(ended, count, table, table_stride, width, lens, batch,
-                                                                         free_pages, n_free, taken, shift);
-    TW4_LAUNCH_CHECK("release_pages: launch");
-    return TW4_OK;
+    return release("release_pages", false, ended, count, table, table_stride, width, lens, batch, free_pages, n_free, taken, page_size,
+                   static_cast<hipStream_t>(stream));
+}
+
+extern "C" int tw4_release_lanes(const int32_t* ended, int count, int32_t* table, int64_t table_stride, int width,
+                                 int32_t* lens, int batch, int32_t* free_pages, int n_free, int32_t* taken, int page_size,
+                                 void* stream) {
+    return release("release_lanes", true, ended, count, table, table_stride, width, lens, batch, free_pages, n_free, taken, page_size,
+                   static_cast<hipStream_t>(stream));
 }

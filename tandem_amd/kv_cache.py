@@ -3,7 +3,7 @@ list of the free ones, a table of each request's pages, and the positions and sl
 alone. Nothing is read back: a step, with its pages, can be captured in a HIP graph and replayed.
 
     plan_pages         pages, positions and slots of one step (tw4_plan_pages; a PagedKVCache's own, tw4_plan_step)
-    release_pages      pages of ended requests back to the list (tw4_release_pages)
+    release_pages      pages of ended requests back to the list (tw4_release_pages; a PagedKVCache's own, tw4_release_lanes)
     PagedKVCache       keys and values of every layer, the table and the lists
     PagedBatch         one step over a cache, as tandem_amd.model's attention takes it
 """
@@ -99,18 +99,23 @@ def plan_pages(context_lens: torch.Tensor, query_lens: torch.Tensor, page_table:
 def release_pages(ended: torch.Tensor, context_lens: torch.Tensor, page_table: torch.Tensor, free_pages: torch.Tensor,
                   taken: torch.Tensor, page_size: int) -> None:
     """The pages of the requests ``ended`` (int32 [n], indices into page_table's rows; others are passed over) go back to the
-    list: taken[0] falls by their number and they are the next to be given. Their rows become -1 and their lengths 0, all in place."""
+    list: taken[0] falls by their number and they are the next to be given. Their rows become -1 and their lengths 0, all in place. A
+    request's pages are those of its length: entries behind it are not looked at."""
+    _release("release_pages", w4_hip.library().tw4_release_pages, ended, context_lens, page_table, free_pages, taken, page_size)
+
+
+def _release(who: str, entry, ended: torch.Tensor, context_lens: torch.Tensor, page_table: torch.Tensor, free_pages: torch.Tensor,
+             taken: torch.Tensor, page_size: int) -> None:
     if ended.dim() != 1:
-        raise RuntimeError(f"release_pages: ended must be one list (got {list(ended.shape)})")
+        raise RuntimeError(f"{who}: ended must be one list (got {list(ended.shape)})")
     batch, width, stride, n_free, index = _checked(
-        "release_pages", layout(page_table), layout(free_pages), page_size, 0, ("ended", layout(ended), ended.shape[0]),
+        who, layout(page_table), layout(free_pages), page_size, 0, ("ended", layout(ended), ended.shape[0]),
         ("context_lens", layout(context_lens), None), ("taken", layout(taken), 1))
     if ended.shape[0] == 0:
         return
     with w4_hip.on_device(index):
-        w4_hip.check(w4_hip.library().tw4_release_pages(
-            ended.data_ptr(), ended.shape[0], page_table.data_ptr(), stride, width, context_lens.data_ptr(), batch,
-            free_pages.data_ptr(), n_free, taken.data_ptr(), page_size, w4_hip.raw_stream(index)))
+        w4_hip.check(entry(ended.data_ptr(), ended.shape[0], page_table.data_ptr(), stride, width, context_lens.data_ptr(), batch,
+                           free_pages.data_ptr(), n_free, taken.data_ptr(), page_size, w4_hip.raw_stream(index)))
 
 
 @dataclass(frozen=True)
@@ -132,7 +137,11 @@ class PagedBatch:
 class PagedKVCache:
     """Keys and values [layers, pages, KV heads, page size, head_dim] for up to max_requests requests of up to max_seq_len tokens.
     A request has a lane (a row of the table) from its first token until release. Lanes 0 .. B - 1 take part in a step of B;
-    those with no new token sit it out. One stream at a time works on a cache, as on any tensor it writes."""
+    those with no new token sit it out. One stream at a time works on a cache, as on any tensor it writes.
+
+    context_lens [max_requests] may be lowered in place between steps (drafted tokens that were not accepted; tokens of a step that the list
+    had too few pages for, down to the last whole page that is there): the lane keeps the pages behind its length for the
+    tokens to come."""
 
     def __init__(self, layers: int, kv_heads: int, head_dim: int, num_pages: int, max_requests: int, max_seq_len: int,
                  page_size: int = 16, rope_theta: float = 1e6, dtype: torch.dtype = torch.float16,
@@ -194,4 +203,5 @@ class PagedKVCache:
     def release(self, lanes: Sequence[int] | torch.Tensor) -> None:
         """The lanes' requests have ended: their pages are free again."""
         ended = torch.as_tensor(lanes, dtype=torch.int32).to(self.page_table.device)
-        release_pages(ended, self.context_lens, self.page_table, self.free_pages, self.taken, self.page_size)
+        _release("PagedKVCache.release", w4_hip.library().tw4_release_lanes, ended, self.context_lens, self.page_table, self.free_pages,
+                 self.taken, self.page_size)

@@ -78,6 +78,7 @@ _SIGNATURES = {
     "tw4_plan_pages": ([_P, _P, _P, _I64, _I, _P, _I, _P, _P, _I, _P, _P, _P, _P, _P, _I, _I, _P], _I),
     "tw4_plan_step": ([_P, _P, _P, _I64, _I, _P, _I, _P, _I, _P, _P, _P, _P, _P, _I, _I, _P], _I),
     "tw4_release_pages": ([_P, _I, _P, _I64, _I, _P, _I, _P, _I, _P, _I, _P], _I),
+    "tw4_release_lanes": ([_P, _I, _P, _I64, _I, _P, _I, _P, _I, _P, _I, _P], _I),
     "tw4_paged_attention_plan": ([_I] * 9 + [ctypes.POINTER(_I)], _I),
     "tw4_paged_attention": ([_P, _I64, _I64, _P, _P, _I64, _I64, _I64, _I, _I, _P, _I64, _I, _P, _P, _P, _P, _I64, _P, _I64,
                              _I, _I, _I, _I, _I, ctypes.c_float, _I, _I, _I, _P], _I),

@@ -226,3 +226,76 @@ def test_step_refuses_bad_arguments():
         args[at] = value
         assert lib.tw4_plan_step(*args, None) == w4_hip.TW4_EINVAL, (at, value)
         assert needle in lib.tw4_last_error().decode() and "plan_step" in lib.tw4_last_error().decode(), (at, value)
+
+
+def _whole(cache, lanes, pages):
+    """Every page is in the list or in one row of the table."""
+    table = cache.page_table.tolist()
+    left = cache.free_pages.tolist()[int(cache.taken):]
+    assert sorted([p for r in table[:lanes] for p in r if p >= 0] + left) == list(range(pages))
+
+
+@pytest.mark.gpu
+def test_lengths_taken_back_keep_their_pages():
+    """Drafted tokens that are not accepted: the lane's length is lowered, its pages stay with it, the next tokens take them, and release
+    returns all."""
+    cache = kv_cache.PagedKVCache(1, 1, 64, num_pages=40, max_requests=3, max_seq_len=200)
+    cache.plan(_int([15, 16, 3]), 34)
+    rng = random.Random(6)
+    lens = [15, 16, 3]
+    for step in range(30):
+        new = [rng.choice((0, 1, 5, 40)) for _ in range(3)]
+        new = [n if lens[i] + n <= 190 else 0 for i, n in enumerate(new)]
+        before = [r[:] for r in cache.page_table.tolist()]
+        batch = cache.plan(_int(new), sum(new))
+        table = cache.page_table.tolist()
+        lacking = sum(1 for i in range(3) for p in range(-(-lens[i] // 16), -(-(lens[i] + new[i]) // 16)) if before[i][p] < 0)
+        assert batch.counts.tolist() == [sum(new), lacking, 0, 0]
+        assert all(b in (-1, a) for old, now in zip(before, table) for b, a in zip(old, now))
+        lens = [x + n for x, n in zip(lens, new)]
+        assert batch.slots.tolist() == [table[i][j // 16] * 16 + j % 16 for i in range(3) for j in range(lens[i] - new[i], lens[i])]
+        _whole(cache, 3, 40)
+        back = [rng.randint(0, n) for n in new]  # not accepted
+        cache.context_lens -= _int(back)
+        lens = [x - n for x, n in zip(lens, back)]
+        if step % 7 == 6:
+            cache.release([step % 3])
+            lens[step % 3] = 0
+            assert set(cache.page_table.tolist()[step % 3]) == {-1}
+            _whole(cache, 3, 40)
+    cache.release([0, 1, 2])
+    assert int(cache.taken) == 0 and sorted(cache.free_pages.tolist()) == list(range(40))
+    assert cache.context_lens.tolist() == [0, 0, 0]
+
+
+@pytest.mark.gpu
+def test_many_pages_kept_and_given_in_one_step():
+    """More new places of the table than the workgroup has threads, kept and missing ones in turn."""
+    cache = kv_cache.PagedKVCache(1, 1, 64, num_pages=6000, max_requests=5, max_seq_len=16 * 900)
+    for steps in ([100, 14000, 1, 0, 9000], [5000, 1, 14000, 14000, 0]):
+        cache.plan(_int(steps), sum(steps))
+        cache.context_lens.clamp_(max=1)
+    batch = cache.plan(_int([14000] * 5), 70000)
+    assert batch.counts.tolist() == [70000, 5 * 876 - (313 + 875 + 876 + 875 + 563), 0, 0]  # ceil(14001 / 16) = 876 a lane
+    _whole(cache, 5, 6000)
+    slots, table = batch.slots.tolist(), cache.page_table.tolist()
+    assert slots == [table[i][j // 16] * 16 + j % 16 for i in range(5) for j in range(1, 14001)]
+    cache.release([4, 2, 0, 1, 3])
+    assert int(cache.taken) == 0 and sorted(cache.free_pages.tolist()) == list(range(6000))
+
+
+@pytest.mark.gpu
+def test_tokens_without_a_page_can_be_brought_again():
+    """A step that the list had too few pages for: the lane's length is taken back to the last page there is, another lane is released, and
+    the tokens come again."""
+    cache = kv_cache.PagedKVCache(1, 1, 64, num_pages=4, max_requests=2, max_seq_len=96)
+    cache.plan(_int([40, 10]), 50)
+    batch = cache.plan(_int([30, 0]), 30)
+    assert batch.counts.tolist() == [30, 0, 2, 0] and cache.page_table.tolist()[0][:5] == [0, 1, 2, -1, -1]
+    assert batch.slots.tolist() == [*range(40, 48)] + [-1] * 22
+    cache.context_lens[0] = 48
+    cache.release([1])
+    batch = cache.plan(_int([16, 0]), 16)
+    assert batch.counts.tolist() == [16, 1, 0, 0] and batch.slots.tolist() == [*range(48, 64)]
+    cache.release([0])
+    assert int(cache.taken) == 0 and sorted(cache.free_pages.tolist()) == list(range(4))
