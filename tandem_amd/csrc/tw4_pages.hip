@@ -89,7 +89,8 @@ __device__ __forceinline__ void scan2(int& x, int& y, int& tx, int& ty, int (*pa
 }
 
 // STEP: the table is a cache's own, so an entry behind a request's length is a page it already has (its length was taken back): it stays, and
-// only entries that are none (-1) take pages, in the order of their places.
+// only entries that are none (-1) take pages, in the order of their places. Tokens behind row a.tokens - 1 are not computed in this step,
+// so starts and lengths end there too: they come again, and find the pages they were given.
 template <bool STEP>
 __global__ void __launch_bounds__(kThreads) pages_kernel(PageArgs a, int rows) {
     __shared__ int part[kThreads / 64][2];
@@ -116,15 +117,21 @@ __global__ void __launch_bounds__(kThreads) pages_kernel(PageArgs a, int rows) {
         const int i = base + j;
         if (i < a.batch) {
             starts[i] = sum_n, first[i] = sum_need;
-            a.starts[i] = sum_n;
-            a.lens[i] = context[i] + n[j];  // the lengths' arrays may be one: read above, written here
-            if constexpr (STEP) a.advance[i] = context[i] + n[j];
+            // the lengths' arrays may be one: read above, written here
+            if constexpr (STEP) {
+                const int from = min(sum_n, a.tokens), to = min(sum_n + n[j], a.tokens);
+                a.starts[i] = from;
+                a.lens[i] = a.advance[i] = context[i] + (to - from);
+            } else {
+                a.starts[i] = sum_n;
+                a.lens[i] = context[i] + n[j];
+            }
             sum_n += n[j], sum_need += need[j];
         }
     }
     if (tid == 0) {
         starts[a.batch] = total, first[a.batch] = pages;
-        a.starts[a.batch] = total;
+        a.starts[a.batch] = STEP ? min(total, a.tokens) : total;
     }
     __syncthreads();
     int missing = 0;  // of the places so far; without STEP all are

@@ -72,7 +72,8 @@ def plan_pages(context_lens: torch.Tensor, query_lens: torch.Tensor, page_table:
 
     int32 GPU tensors; lengths below zero count as zero, and each new length and all new tokens together are below 2^31. seq_lens_out (context_lens
     itself, to advance it) and taken_out (taken itself) are written instead of new tensors. Nothing is read back; the caller that
-    wants to know whether the pages sufficed reads counts[2]."""
+    wants to know whether the pages sufficed reads counts[2]. Tokens past num_tokens (counts[3]) have pages, and count in seq_lens and query_start, but no
+    position or slot."""
     outs = () if seq_lens_out is None else (("seq_lens_out", layout(seq_lens_out), None),)
     if taken_out is not None:
         outs += (("taken_out", layout(taken_out), 1),)
@@ -177,7 +178,9 @@ class PagedKVCache:
     def plan(self, query_lens: torch.Tensor, num_tokens: int, max_query_len: int | None = None,
              max_seq_len: int | None = None) -> PagedBatch:
         """Takes pages for query_lens[i] new tokens of lane i (int32 [B], B <= max_requests) and advances the lanes' lengths; the
-        step's tokens are num_tokens rows, lane by lane (rows behind the last are computed for nothing). max_query_len,
+        step's tokens are num_tokens rows, lane by lane (rows behind the last are computed for nothing). Tokens that have no row, past
+        num_tokens, are not in the step: query_start and the lengths stop at those that are, counts[3] says how many are left, and they
+        are to come again. max_query_len,
         max_seq_len: bounds the host knows, for the division of the work."""
         if query_lens.dim() != 1 or not 1 <= query_lens.numel() <= self.max_requests:
             raise RuntimeError(f"PagedKVCache.plan: query_lens [1 .. {self.max_requests}] expected (got {tuple(query_lens.shape)})")

@@ -244,3 +244,29 @@ def test_two_runners_side_by_side(monkeypatch):
     torch.cuda.synchronize()
     for outs in got:
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@pytest.mark.gpu
+def test_prompts_in_steps_of_too_few_rows_match_oracle(monkeypatch):
+    """Two prompts brought whole to every step of 16 rows: each step computes what fits, and the rest comes again."""
+    model, w = _model(monkeypatch, 16)
+    cache = PagedKVCache.for_model(CFG, num_pages=20, max_requests=2, max_seq_len=96)
+    cache.keys.fill_(float("nan"))
+    cache.values.fill_(float("nan"))
+    rng = np.random.default_rng(3)
+    seqs = [rng.integers(0, CFG.vocab_size, n).tolist() for n in (21, 18)]
+    want = [_oracle(w, s) for s in seqs]
+    done = [0, 0]
+    while done != [21, 18]:
+        new = [len(s) - d for s, d in zip(seqs, done)]
+        rest = ([x for s, d in zip(seqs, done) for x in s[d:]] + [0] * 16)[:16]
+        with torch.inference_mode():
+            batch = cache.plan(_int(new), 16)
+            starts = batch.query_start.tolist()
+            assert starts[-1] == min(sum(new), 16)
+            logits = model.compute_logits(model(torch.tensor(rest, device="cuda"), batch))
+        for lane, (a, b) in enumerate(zip(starts, starts[1:])):
+            if b > a:
+                one_token._close(logits[a:b], want[lane][done[lane]:done[lane] + b - a], 0.02, (done, lane))
+            done[lane] += b - a
+        assert cache.context_lens.tolist() == done

@@ -299,3 +299,26 @@ def test_tokens_without_a_page_can_be_brought_again():
     assert batch.counts.tolist() == [16, 1, 0, 0] and batch.slots.tolist() == [*range(48, 64)]
     cache.release([0])
     assert int(cache.taken) == 0 and sorted(cache.free_pages.tolist()) == list(range(4))
+
+
+@pytest.mark.gpu
+def test_a_step_with_too_few_rows_advances_by_those_it_has():
+    """Tokens that no row is left for are counted, and come again in a later step: a lane's length has those only that were computed."""
+    cache = kv_cache.PagedKVCache(1, 1, 64, num_pages=16, max_requests=4, max_seq_len=96)
+    batch = cache.plan(_int([5, 40, 7, 0]), 20)
+    assert batch.counts.tolist() == [52, 5, 0, 32]
+    assert batch.query_start.tolist() == [0, 5, 20, 20, 20] and batch.seq_lens.tolist() == [5, 15, 0, 0]
+    assert cache.context_lens.tolist() == [5, 15, 0, 0] and batch.positions.tolist() == [*range(5), *range(15)]
+    batch = cache.plan(_int([0, 25, 7, 0]), 33)
+    assert batch.counts.tolist() == [32, 0, 0, 0] and batch.seq_lens.tolist() == [5, 40, 7, 0]
+    table = cache.page_table.tolist()
+    assert batch.slots.tolist() == [table[1][j // 16] * 16 + j % 16 for j in range(15, 40)] + [table[2][0] * 16 + j for j in range(7)] + [-1]
+    batch = cache.plan(_int([3, 2, 1, 1]), 0)
+    assert batch.counts.tolist() == [7, 1, 0, 7] and batch.query_start.tolist() == [0] * 5 and cache.context_lens.tolist() == [5, 40, 7, 0]
+    _whole(cache, 4, 16)
+    # more rows than one workgroup places
+    cache = kv_cache.PagedKVCache(1, 1, 64, num_pages=2000, max_requests=3, max_seq_len=9000)
+    cache.plan(_int([1, 2, 3]), 6)
+    batch = cache.plan(_int([6000, 5000, 100]), 9001)
+    assert batch.query_start.tolist() == [0, 6000, 9001, 9001] and batch.seq_lens.tolist() == [6001, 3003, 3]
+    assert batch.positions.tolist() == [*range(1, 6001), *range(2, 3003)] and min(batch.slots.tolist()) >= 0
