@@ -8,8 +8,8 @@
 A head x of D values becomes y = x rsqrt(mean(x^2) + eps) weight (no weight: y = x), and then, with the angle a_i of its
 token's position, (y[i] cos a_i - y[i + D/2] sin a_i, y[i + D/2] cos a_i + y[i] sin a_i): the halves of a head rotate
 against each other, as in the Qwen3 and Llama checkpoints of Hugging Face. fp32 arithmetic, one rounding. float16 and
-bfloat16, heads of 64 or 128 values. Inference only: a projection or a cache that autograd follows is refused, and the weights are
-taken as values, as in layers/norm.py.
+bfloat16, heads of 64 or 128 values. Inference only: a projection or a cache that a gradient, tangent or transform follows is refused, and the
+weights and the table are taken as values, as in layers/norm.py.
 """
 
 from __future__ import annotations
@@ -101,7 +101,7 @@ def _run(who: str, qkv, positions, table, num_heads: int, num_kv_heads: int, q_w
                                              None if q_weight is None else layout(q_weight),
                                              None if k_weight is None else layout(k_weight), None if k is None else layout(k),
                                              None if v is None else layout(v), None if slots is None else layout(slots))
-    if not w4_hip.plain(qkv) or (slots is not None and torch.is_grad_enabled() and (k.requires_grad or v.requires_grad)):
+    if not (w4_hip.plain(qkv) and (slots is None or (w4_hip.plain(k) and w4_hip.plain(v)))):
         raise RuntimeError(f"{who}: inference only, no gradient, transform or tracer can follow qkv or the caches")
     tokens = qkv.shape[0]
     q = qkv.new_empty((tokens, num_heads, d))

@@ -457,3 +457,22 @@ def test_rows_of_a_step_cut_short_see_no_later_key(rows, splits):
         assert ((got.double() - want[:cut]).abs() <= tol[:cut]).all(), cut
         got = paged_attention(q[:cut], k, v, table, lens, starts)
         assert ((got.double() - want[:cut]).abs() <= tol[:cut]).all(), cut
+
+
+@pytest.mark.gpu
+def test_caches_and_out_that_a_gradient_or_tangent_follows_are_refused():
+    q, k, v, table, lens, starts = args = build([33], [2], 4, 2, 64, torch.float16, 16, seed=33)
+    want = paged_attention(*args)
+    with torch.autograd.forward_ad.dual_level():
+        for name, x in (("q", q), ("k_cache", k), ("v_cache", v), ("out", torch.empty_like(q))):
+            dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+            with pytest.raises(RuntimeError, match="inference only"):
+                paged_attention(**{**dict(q=q, k_cache=k, v_cache=v, page_table=table, seq_lens=lens, query_start=starts), name: dual})
+        assert torch.equal(paged_attention(*args), want)
+    out = torch.empty_like(q).requires_grad_()
+    with pytest.raises(RuntimeError, match="inference only"):
+        paged_attention(*args, out=out)
+    with torch.no_grad():
+        assert torch.equal(paged_attention(q, k.requires_grad_(), v, table, lens, starts, out=out), want)
+    k.requires_grad_(False)
+    assert torch.equal(paged_attention(q, torch.nn.Parameter(k, requires_grad=False), v, table, lens, starts), want)

@@ -181,3 +181,19 @@ def test_refusals():
     assert (rotary.norm_rope(one, pos[:1], table, heads, kv)[0] == 0).all()
     q, k = rotary.norm_rope(qkv[:0], pos[:0], table, heads, kv)
     assert q.shape == (0, heads, d) and k.shape == (0, kv, d)
+
+
+@pytest.mark.gpu
+def test_caches_that_a_tangent_follows_are_refused():
+    d, heads, kv = 64, 4, 2
+    table = rotary.rotary_table(8, d, 1e4, "cuda")
+    qkv = torch.zeros(2, 8 * d, dtype=torch.float16, device="cuda")
+    pos = torch.arange(2, dtype=torch.int32, device="cuda")
+    k, v = (torch.zeros(2, kv, 16, d, dtype=torch.float16, device="cuda") for _ in range(2))
+    with torch.autograd.forward_ad.dual_level():
+        for at in range(2):
+            caches = [k, v]
+            caches[at] = torch.autograd.forward_ad.make_dual(caches[at], torch.ones_like(k))
+            with pytest.raises(RuntimeError, match="inference only"):
+                rotary.norm_rope_cache(qkv, pos, table, heads, kv, *caches, pos)
+        rotary.norm_rope_cache(qkv, pos, table, heads, kv, k, v, pos)
