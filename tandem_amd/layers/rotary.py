@@ -110,6 +110,8 @@ def _run(who: str, qkv, positions, table, num_heads: int, num_kv_heads: int, q_w
     if tokens:
         xp, tp, kp, vp = qkv.data_ptr(), table.data_ptr(), k.data_ptr(), 0 if v is None else v.data_ptr()
         qw, kw = 0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr()
+        if kp == vp:
+            raise RuntimeError(f"{who}: keys and values need memory of their own")
         if (xp | tp | kp | vp | qw | kw) % 16:
             raise RuntimeError(f"{who}: qkv, the table, weights and caches must be 16-byte aligned")
         with w4_hip.on_device(index):
@@ -133,7 +135,8 @@ def norm_rope_cache(qkv: torch.Tensor, positions: torch.Tensor, table: torch.Ten
                     k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor, q_weight: torch.Tensor | None = None,
                     k_weight: torch.Tensor | None = None, eps: float = 1e-6) -> torch.Tensor:
     """norm_rope whose keys, and the values as they are, go into the caches [pages, KV heads, page size, head_dim]: token t's
-    at slots[t] = page * page size + offset (int32 [T]; outside of the cache: nowhere). Slots are distinct; of two tokens
+    at slots[t] = page * page size + offset (int32 [T]; outside of the cache: nowhere). The two caches share no place (one tensor may hold
+    both, as views). Slots are distinct; of two tokens
     with one slot either may win. Returns the queries [T, heads, head_dim]."""
     return _run("norm_rope_cache", qkv, positions, table, num_heads, num_kv_heads, q_weight, k_weight, eps, k_cache,
                 v_cache, slots)[0]

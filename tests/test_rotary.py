@@ -197,3 +197,16 @@ def test_caches_that_a_tangent_follows_are_refused():
             with pytest.raises(RuntimeError, match="inference only"):
                 rotary.norm_rope_cache(qkv, pos, table, heads, kv, *caches, pos)
         rotary.norm_rope_cache(qkv, pos, table, heads, kv, k, v, pos)
+
+
+@pytest.mark.gpu
+def test_one_cache_for_keys_and_values_is_refused():
+    d, heads, kv = 64, 4, 2
+    table = rotary.rotary_table(8, d, 1e4, "cuda")
+    qkv = torch.zeros(2, 8 * d, dtype=torch.float16, device="cuda")
+    pos = torch.arange(2, dtype=torch.int32, device="cuda")
+    k = torch.zeros(2, kv, 16, d, dtype=torch.float16, device="cuda")
+    with pytest.raises(RuntimeError, match="memory of their own"):
+        rotary.norm_rope_cache(qkv, pos, table, heads, kv, k, k, pos)
+    both = torch.zeros(2, 2, kv, 16, d, dtype=torch.float16, device="cuda")  # keys and values in one tensor: two places each
+    rotary.norm_rope_cache(qkv, pos, table, heads, kv, both[:, 0], both[:, 1], pos)
