@@ -78,7 +78,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         layout(q), layout(k_cache), layout(v_cache), layout(page_table), layout(seq_lens),
         None if query_start is None else layout(query_start), None if out is None else layout(out),
         max_query_len, None if max_seq_len is None else (max_seq_len + 127) // 128 * 128, scale)
-    if not (w4_hip.plain(q) and w4_hip.plain(k_cache) and w4_hip.plain(v_cache) and (out is None or w4_hip.plain(out))):
+    if not w4_hip.all_plain(q, k_cache, v_cache, *(() if out is None else (out,))):
         raise RuntimeError("paged_attention: inference only, no gradient, transform or tracer can follow q, the caches or out")
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)  # 1 us less than torch.empty of a device

@@ -101,7 +101,7 @@ def _run(who: str, qkv, positions, table, num_heads: int, num_kv_heads: int, q_w
                                              None if q_weight is None else layout(q_weight),
                                              None if k_weight is None else layout(k_weight), None if k is None else layout(k),
                                              None if v is None else layout(v), None if slots is None else layout(slots))
-    if not (w4_hip.plain(qkv) and (slots is None or (w4_hip.plain(k) and w4_hip.plain(v)))):
+    if not (w4_hip.plain(qkv) if slots is None else w4_hip.all_plain(qkv, k, v)):
         raise RuntimeError(f"{who}: inference only, no gradient, transform or tracer can follow qkv or the caches")
     tokens = qkv.shape[0]
     q = qkv.new_empty((tokens, num_heads, d))

@@ -517,6 +517,19 @@ def plain(x: torch.Tensor) -> bool:
             and (forward_ad._current_level < 0 or forward_ad.unpack_dual(x).tangent is None))
 
 
+def all_plain(*tensors: torch.Tensor) -> bool:
+    """``plain`` of each, what is the same for all looked at once: an eager call is bound by the host."""
+    if _functorch.peek_interpreter_stack() is not None or forward_ad._current_level >= 0:
+        return all(map(plain, tensors))
+    if _is_tracing() or _len_torch_dispatch_stack():
+        return False
+    grad = torch.is_grad_enabled()
+    for x in tensors:
+        if type(x) not in _TENSORS or (grad and x.requires_grad):
+            return False
+    return True
+
+
 def intercepted(product: bool = True) -> bool:
     """Whether a torch operator called here would come out otherwise than by its arguments: autocast to another type than
     float16 gives a product another dtype, a torch function mode sees or replaces it (a default device does neither), a

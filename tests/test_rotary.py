@@ -210,3 +210,38 @@ def test_one_cache_for_keys_and_values_is_refused():
         rotary.norm_rope_cache(qkv, pos, table, heads, kv, k, k, pos)
     both = torch.zeros(2, 2, kv, 16, d, dtype=torch.float16, device="cuda")  # keys and values in one tensor: two places each
     rotary.norm_rope_cache(qkv, pos, table, heads, kv, both[:, 0], both[:, 1], pos)
+
+
+def test_all_plain_is_plain_of_each():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.autograd import forward_ad
+    from torch.func import vmap
+
+    class Own(torch.Tensor):
+        pass
+
+    x, y, p, own = torch.zeros(3), torch.ones(3, requires_grad=True), torch.nn.Parameter(torch.zeros(3), requires_grad=False), Own([1.0])
+
+    def agree(*extra):
+        pool = [x, y, p, own, *extra]
+        for a in pool:
+            for b in pool:
+                assert w4_hip.all_plain(x, a, b) == all(map(w4_hip.plain, (x, a, b)))
+        assert w4_hip.all_plain(x, p) == (w4_hip.plain(x) and w4_hip.plain(p))
+
+    agree()
+    assert w4_hip.all_plain(x, p) and not w4_hip.all_plain(x, y) and not w4_hip.all_plain(own, x)
+    for mode in (torch.no_grad(), torch.inference_mode(), FakeTensorMode()):
+        with mode:
+            agree()
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(torch.zeros(3), torch.ones(3))
+        agree(dual)
+        assert w4_hip.all_plain(x, p) and not w4_hip.all_plain(x, dual)
+
+    def wrapped(t):
+        agree(t)
+        assert w4_hip.all_plain(x, p) and not w4_hip.all_plain(x, t)
+        return t
+
+    vmap(wrapped)(torch.zeros(2, 3))
