@@ -172,6 +172,11 @@ class PagedKVCache:
         """A cache of float16 for a DecoderModel of this configuration."""
         if config.rope_type != "default":
             raise NotImplementedError(f"rope_scaling of type {config.rope_type!r}: only plain rotary positions are supported")
+        if config.sliding_window is not None and config.sliding_window < max_seq_len:
+            raise NotImplementedError(f"sliding_window {config.sliding_window}: only attention over all keys is supported (a cache of no more "
+                                      f"than that per request is; got max_seq_len {max_seq_len})")
+        if config.other_attention:
+            raise NotImplementedError(f"attention with {', '.join(config.other_attention)} is not supported")
         return cls(config.num_layers, config.num_kv_heads, config.head_dim, num_pages, max_requests, max_seq_len, page_size,
                    config.rope_theta, torch.float16, device)
 

@@ -59,22 +59,37 @@ class DecoderConfig:
     rope_theta: float = 1e6
     qk_norm: bool = False
     rope_type: str = "default"
+    sliding_window: Optional[int] = None  # keys a token sees, its own among them, in some layer; None: all
+    other_attention: tuple[str, ...] = ()  # fields of config.json that ask for more than this attention computes
 
     @classmethod
     def from_hf(cls, d: dict[str, Any]) -> "DecoderConfig":
         """The fields of a Hugging Face config.json (python/tandem/model_config.py). Without a model_type: Qwen3, whose
         queries and keys are normalised head by head."""
         heads = int(d["num_attention_heads"])
-        qwen3 = d.get("model_type", "qwen3") == "qwen3"
+        kind, layers = str(d.get("model_type", "qwen3")), d.get("layer_types") or ()
+        qwen3 = kind == "qwen3"
         rope = d.get("rope_parameters") or d.get("rope_scaling") or {}
+        head_dim = int(d.get("head_dim") or d["hidden_size"] // heads)
+        # Qwen's configurations name a window that is off unless asked for, and then in the layers from max_window_layers on
+        slides = d.get("use_sliding_window", not kind.startswith("qwen")) and int(d.get("max_window_layers") or 0) < int(d["num_hidden_layers"])
+        window = d.get("sliding_window") if ("sliding_attention" in layers if layers else slides) else None
+        scale = head_dim ** -0.5
+        other = {"partial_rotary_factor": any(float(f.get("partial_rotary_factor") or 1.0) != 1.0 for f in (d, rope)),
+                 "attn_logit_softcapping": d.get("attn_logit_softcapping"),
+                 "attention_bias": d.get("attention_bias", kind == "qwen2"),  # Qwen2's qkv biases are not optional
+                 "query_pre_attn_scalar": abs(float(d.get("query_pre_attn_scalar") or head_dim) ** -0.5 / scale - 1) > 1e-6,
+                 "attention_multiplier": abs(float(d.get("attention_multiplier") or scale) / scale - 1) > 1e-6,
+                 "layer_types": any(x not in ("full_attention", "sliding_attention") for x in layers),
+                 "rope_parameters": any(isinstance(x, dict) for x in rope.values())}  # positions of their own for some layers
         return cls(hidden_size=int(d["hidden_size"]), intermediate_size=int(d["intermediate_size"]),
                    num_heads=heads, num_kv_heads=int(d.get("num_key_value_heads", heads)),
-                   head_dim=int(d.get("head_dim") or d["hidden_size"] // heads),
-                   num_layers=int(d["num_hidden_layers"]), vocab_size=int(d["vocab_size"]),
+                   head_dim=head_dim, num_layers=int(d["num_hidden_layers"]), vocab_size=int(d["vocab_size"]),
                    rms_norm_eps=float(d.get("rms_norm_eps", 1e-6)),
                    tie_word_embeddings=bool(d.get("tie_word_embeddings", False)),
                    rope_theta=float(d.get("rope_theta") or rope.get("rope_theta") or (1e6 if qwen3 else 1e4)), qk_norm=qwen3,
-                   rope_type=str(rope.get("rope_type") or rope.get("type") or "default"))
+                   rope_type=str(rope.get("rope_type") or rope.get("type") or "default"),
+                   sliding_window=None if window is None else int(window), other_attention=tuple(k for k, v in other.items() if v))
 
 
 QWEN3_8B = DecoderConfig(4096, 12288, 32, 8, 128, 36, 151936, qk_norm=True)

@@ -270,3 +270,32 @@ def test_prompts_in_steps_of_too_few_rows_match_oracle(monkeypatch):
                 one_token._close(logits[a:b], want[lane][done[lane]:done[lane] + b - a], 0.02, (done, lane))
             done[lane] += b - a
         assert cache.context_lens.tolist() == done
+
+
+def test_attention_that_the_model_does_not_compute_is_refused():
+    """Fields of config.json that ask for another attention than the cache's: at position 0 they do not matter, past it they do."""
+    hf = {"hidden_size": 4096, "intermediate_size": 14336, "num_attention_heads": 32, "num_key_value_heads": 8, "num_hidden_layers": 32,
+          "vocab_size": 32000, "rms_norm_eps": 1e-5, "model_type": "mistral", "rope_theta": 1e4}
+    small = dict(num_pages=2, max_requests=1, device="cpu")
+    for change, needle in (({"sliding_window": 4096}, "sliding_window"), ({"partial_rotary_factor": 0.5}, "partial_rotary_factor"),
+                           ({"rope_parameters": {"rope_type": "default", "rope_theta": 1e4, "partial_rotary_factor": 0.25}}, "partial_rotary_factor"),
+                           ({"attn_logit_softcapping": 50.0}, "attn_logit_softcapping"), ({"attention_bias": True}, "attention_bias"),
+                           ({"model_type": "qwen2"}, "attention_bias"), ({"query_pre_attn_scalar": 256}, "query_pre_attn_scalar"),
+                           ({"attention_multiplier": 0.5}, "attention_multiplier"),
+                           ({"model_type": "qwen3", "sliding_window": 4096, "use_sliding_window": True, "max_window_layers": 8}, "sliding_window"),
+                           ({"sliding_window": 4096, "layer_types": ["full_attention"] * 31 + ["sliding_attention"]}, "sliding_window"),
+                           ({"layer_types": ["full_attention"] * 31 + ["linear_attention"]}, "layer_types"),
+                           ({"rope_parameters": {"full_attention": {"rope_theta": 1e6}, "sliding_attention": {"rope_theta": 1e4}}}, "rope_parameters")):
+        cfg = tmodel.DecoderConfig.from_hf({**hf, **change})  # the one-token step takes it as before
+        with pytest.raises(NotImplementedError, match=needle):
+            PagedKVCache.for_model(cfg, max_seq_len=4097, **small)
+    layers = dict(small, max_seq_len=4097)
+    for change in ({}, {"sliding_window": None}, {"sliding_window": 5000}, {"sliding_window": 4096, "use_sliding_window": False},
+                   {"model_type": "qwen3", "sliding_window": 4096, "use_sliding_window": True, "max_window_layers": 32},
+                   {"sliding_window": 4096, "layer_types": ["full_attention"] * 32}, {"attn_logit_softcapping": None},
+                   {"partial_rotary_factor": 1.0}, {"query_pre_attn_scalar": 128}, {"attention_bias": False},
+                   {"attention_multiplier": 128 ** -0.5}):
+        cfg = tmodel.DecoderConfig.from_hf({**hf, **change, "num_hidden_layers": 32})
+        PagedKVCache.for_model(dataclasses.replace(cfg, num_layers=1), **layers)
+    # a cache that no request can outgrow the window of
+    PagedKVCache.for_model(dataclasses.replace(tmodel.DecoderConfig.from_hf({**hf, "sliding_window": 4096}), num_layers=1), **dict(small, max_seq_len=4096))
