@@ -278,8 +278,8 @@ static int release(const char* who, bool whole, const int32_t* ended, int count,
     TW4_REQUIRE(shift >= 0, TW4_EINVAL, "%s: page_size 16, 32, 64, 128 or 256 (%d)", who, page_size);
     TW4_REQUIRE(count >= 0 && batch >= 1 && width >= 0 && n_free >= 0 && table_stride >= width, TW4_EINVAL,
                 "%s: bad sizes (%d of %d requests, width %d)", who, count, batch, width);
-    if (count == 0 || width == 0) return TW4_OK;
-    TW4_REQUIRE(ended && table && lens && taken && (free_pages || !n_free), TW4_EINVAL, "%s: null pointer", who);
+    if (count == 0) return TW4_OK;
+    TW4_REQUIRE(ended && (table || !width) && lens && taken && (free_pages || !n_free), TW4_EINVAL, "%s: null pointer", who);
     if (whole)
         release_kernel<true><<<1, kThreads, 0, st>>>(ended, count, table, table_stride, width, lens, batch, free_pages, n_free, taken, shift);
     else

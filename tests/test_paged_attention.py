@@ -476,3 +476,30 @@ def test_caches_and_out_that_a_gradient_or_tangent_follows_are_refused():
         assert torch.equal(paged_attention(q, k.requires_grad_(), v, table, lens, starts, out=out), want)
     k.requires_grad_(False)
     assert torch.equal(paged_attention(q, torch.nn.Parameter(k, requires_grad=False), v, table, lens, starts), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("splits", [1, 3, 7])
+@pytest.mark.parametrize("rows", [16, 32, 128])
+@pytest.mark.parametrize("dtype,page,d", [(torch.float16, 16, 128), (torch.bfloat16, 64, 64), (torch.bfloat16, 16, 128), (torch.float16, 64, 64)])
+def test_entries_that_are_no_page_in_every_tile_and_split(dtype, page, d, rows, splits):
+    """Holes at the start, in the middle and at the end of long contexts, whole tiles of keys and parts of them; page 0, which is read in
+    their place, is NaN."""
+    q, k, v, table, lens, starts = build([1500, 700, 0, 900], [140, 3, 70, 1], 8, 2, d, dtype, page, seed=41)
+    pages = k.shape[0]
+    k, v = (torch.cat([torch.full_like(c[:1], float("nan")), c]) for c in (k, v))
+    table = torch.where(table >= 0, table + 1, table)
+    whole = (q, k, v, table, lens, starts)
+    bad = (-1, pages + 1, 2 ** 31 - 1, -2 ** 31)
+    last = [-(-int(x) // page) - 1 for x in lens]
+    for holes in ([(0, 0)], [(0, last[0])], [(0, last[0] // 2), (0, last[0] // 2 + 1), (1, 2), (2, 0), (3, last[3])],
+                  [(0, 3), (0, last[0] - 1), (1, last[1]), (1, 0), (3, 1), (3, 4)], [(1, i) for i in range(last[1] + 1)]):
+        cut = table.clone()
+        for n, (i, j) in enumerate(holes):
+            cut[i, j] = bad[n % 4]
+        args = (q, k, v, cut, lens, starts)
+        want, tol = exact(*args)
+        got = _direct(args, rows, splits)
+        assert torch.isfinite(got).all() and ((got.double() - want).abs() <= tol).all(), holes
+    want, tol = exact(*whole)
+    assert ((_direct(whole, rows, splits).double() - want).abs() <= tol).all()
