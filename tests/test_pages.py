@@ -322,3 +322,10 @@ def test_a_step_with_too_few_rows_advances_by_those_it_has():
     batch = cache.plan(_int([6000, 5000, 100]), 9001)
     assert batch.query_start.tolist() == [0, 6000, 9001, 9001] and batch.seq_lens.tolist() == [6001, 3003, 3]
     assert batch.positions.tolist() == [*range(1, 6001), *range(2, 3003)] and min(batch.slots.tolist()) >= 0
+
+
+@pytest.mark.gpu
+def test_release_without_table_columns():
+    lens, taken = _int([5, 3]), _int([2])
+    kv_cache.release_pages(_int([1, 7]), lens, torch.empty((2, 0), dtype=torch.int32, device="cuda"), _int([4, 5]), taken, 16)
+    assert lens.tolist() == [5, 0] and taken.tolist() == [2]
