@@ -6,7 +6,7 @@
 //   first_i = taken + sum over j < i of (pages_j(len_j) - pages_j(c_j))
 //   table[i][pages_i(c_i) + j] = free[first_i + j]    for its j-th new page (-1 past the end of the list)
 //   position of row t of request i = c_i + t - start_i
-//   slot = table[i][position / P] P + position % P    (-1: no page, or a row behind the last request)
+//   slot = table[i][position / P] P + position % P    (-1: no page, one past 2^31 slots, or a row behind the last request)
 //   taken <- min(first_last, length of the list)
 //
 // It moves a few KB and is bound by a launch and three dependent round trips to memory (lengths, the list's entries, the table's): one
@@ -60,7 +60,7 @@ __device__ __forceinline__ void place_row(const PageArgs& a, const int32_t* star
         pos = context(i) + (t - starts[i]);
         const int page = pos >> a.shift;
         const int id = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.width) ? a.table[i * a.table_stride + page] : -1;
-        if (id >= 0) slot = (id << a.shift) + (pos & ((1 << a.shift) - 1));
+        if (id >= 0 && id <= 0x7FFFFFFF >> a.shift) slot = (id << a.shift) + (pos & ((1 << a.shift) - 1));
     }
     a.positions[t] = pos;
     a.slots[t] = slot;

@@ -329,3 +329,14 @@ def test_release_without_table_columns():
     lens, taken = _int([5, 3]), _int([2])
     kv_cache.release_pages(_int([1, 7]), lens, torch.empty((2, 0), dtype=torch.int32, device="cuda"), _int([4, 5]), taken, 16)
     assert lens.tolist() == [5, 0] and taken.tolist() == [2]
+
+
+@pytest.mark.gpu
+def test_pages_past_all_slots_give_none():
+    """A page number whose slots have no int32 gives no slot, not another page's."""
+    for page, shift in ((16, 4), (256, 8)):
+        table = _int([[-1], [-1], [-1]])
+        free = _int([(1 << (32 - shift)) + 3, (1 << (31 - shift)) - 1, 1 << (31 - shift)])
+        plan = kv_cache.plan_pages(_int([0, 0, 0]), _int([2, 2, 2]), table, free, _int([0]), page, 6)
+        top = ((1 << (31 - shift)) - 1) * page
+        assert plan.slots.tolist() == [-1, -1, top, top + 1, -1, -1] and table.flatten().tolist() == free.tolist()
