@@ -14,6 +14,8 @@ A = sum_j w_j |v_j|:
 from __future__ import annotations
 
 import ctypes
+import json
+import os
 import random
 
 import pytest
@@ -503,3 +505,20 @@ def test_entries_that_are_no_page_in_every_tile_and_split(dtype, page, d, rows, 
         assert torch.isfinite(got).all() and ((got.double() - want).abs() <= tol).all(), holes
     want, tol = exact(*whole)
     assert ((_direct(whole, rows, splits).double() - want).abs() <= tol).all()
+
+
+def test_plan_against_the_timed_choices():
+    """The choice of tile and splits beside every one that was timed (profiles/paged_attention_rule_sweep.jsonl: us of a call in a graph for
+    each "rows,splits", MI355X): the fitted calls and those left out of the fit."""
+    with open(os.path.join(os.path.dirname(__file__), "..", "profiles", "paged_attention_rule_sweep.jsonl"), encoding="utf-8") as f:
+        calls = [json.loads(line) for line in f]
+    for fitted, least in ((True, 290), (False, 70)):
+        ratios = []
+        for c in calls:
+            rows, splits, _, _ = _plan(c["tokens"], c["batch"], c["heads"], c["kv_heads"], c["head_dim"], c["max_query"],
+                                       (c["max_keys"] + 127) // 128 * 128, int(c["single"]))
+            chosen = c["us"].get(f"{rows},{splits}")  # a number of splits that fills the CUs exactly was not timed everywhere
+            if c["fitted"] == fitted and chosen is not None:
+                ratios.append(chosen / min(c["us"].values()))
+        assert len(ratios) >= least and sum(ratios) / len(ratios) < 1.02 and max(ratios) < 1.25, (fitted, len(ratios))
+        print(fitted, len(ratios), sum(ratios) / len(ratios), max(ratios))
