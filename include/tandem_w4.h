@@ -309,7 +309,8 @@ int tw4_plan_pages(const int32_t* context, const int32_t* fresh, int32_t* table,
 /* tw4_plan_pages for a cache that keeps its requests' lengths from step to step: context and taken are advanced in place, and lens
  * (another array) are the step's own, which later steps leave as they are. The table's entries behind a request's length are its pages or
  * -1: where context was taken back (tokens that were not accepted) the pages stay in their places, and only entries that are -1 take
- * new ones. New tokens past `tokens` are counted in counts[3] and given pages, but starts, lens and context stop at those that have a row. */
+ * new ones. New tokens past `tokens` are counted in counts[3] and given pages, but starts, lens and context stop at those that have a
+ * row. */
 int tw4_plan_step(int32_t* context, const int32_t* fresh, int32_t* table, int64_t table_stride, int width, const int32_t* free_pages,
                   int n_free, int32_t* taken, int page_size, int32_t* starts, int32_t* lens, int32_t* positions, int32_t* slots,
                   int32_t* counts, int batch, int tokens, void* stream);

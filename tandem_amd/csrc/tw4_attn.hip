@@ -22,8 +22,8 @@
 // transposed; both a block ahead. It is bound by reading K and V: 3 requests of 40002 keys, 16 + 8 heads of 128, 75-77 us (6.4-6.6 TB/s; a plain
 // read reaches 7.1), 32 of 1 to 8192 keys, 32 + 8 heads, 91-94 (5.8-6.0). Measured and not kept: V by ordinary loads 113 us at 32 requests against 92, K
 // through LDS as well 100, three wavefronts per SIMD (they spill) 95. With few rows in flight the keys are split over up to `splits`
-// workgroups; the last to arrive joins their results in order: one request of 1024 keys 9.6 us, most of it ten dependent round trips to memory
-// (lengths, table, keys, the partial results' way out and in, the counter), of 32001 keys 31.
+// workgroups; the last to arrive joins their results in order: one request of 1024 keys 9.4-9.6 us, most of it seven dependent round trips
+// to memory (length, table, keys, store of the partial result, counter, load of all of them, store of the row), of 32001 keys 31.
 //
 // Tiles of 128 rows (chunks of prompts): the chunk kernel below. Its K and V are read by 128 rows at a time from LDS.
 #include <algorithm>
@@ -901,14 +901,14 @@ int attn_launch(const AttnArgs& a, int rows, unsigned units, hipStream_t st) {
 
 using namespace tw4;
 
-// Microseconds of a call with tiles of kRows[i] rows and `splits` splits, as fitted to 300 calls of all sizes with each tile and 1 to
-// 128 splits (batches 1 to 200, 1 to 2000 new tokens, 0 to 100000 keys, heads of 64 and 128). A workgroup takes `start`, its keys' latency,
-// and, with splits, the store of its part and the last one's reading of all; two workgroups share a CU, so beyond 2 cus of them the
-// keys' throughput counts. What the rule picks took 1.011 times the fastest tile and split on average, 1.20 at most (4 chunks of 65 tokens:
-// 12.0 us with 16 rows, 10.0 with 128); on 75 calls it was not fitted to 1.017, 1.19 at most (5 chunks of 188 tokens of 7 heads behind 1908
-// keys: 33.2 us with 3 splits, 27.8 with one). Without it: tiles by rows alone (16, 32, or 128 past 32 rows) and splits for two
-// workgroups per CU took 1.3 on average, 5.8 at most (7 new tokens of 24 heads over 7638 keys: 119 us with tiles of 128 rows and 60
-// splits, 20.4 with 16 rows and 12).
+// Microseconds of a call with tiles of kRows[i] rows and `splits` splits, as fitted to 300 calls of all sizes with each tile and 1 to 128
+// splits (batches 1 to 200, 1 to 2000 new tokens, 0 to 100000 keys, heads of 64 and 128). A workgroup takes `start`, its keys' latency,
+// and, with splits, the store of its part and the last one's reading of all; two workgroups share a CU, so beyond 2 cus of them the keys'
+// throughput counts. What the rule picks took 1.013 times the fastest tile and split on average, 1.18 at most (4 chunks of 65 tokens: 11.8
+// us with 16 rows, 10.0 with 128); on 75 calls it was not fitted to 1.017, 1.18 at most (5 chunks of up to 188 tokens of 7 heads behind up
+// to 1908 keys: 32.9 us with 3 splits, 27.8 with one); profiles/paged_attention_rule_sweep.jsonl has them all. Without it: tiles by rows
+// alone (16, 32, or 128 past 32 rows) and splits for two workgroups per CU took 1.3 on average, 5.8 at most (7 new tokens of 24 heads over
+// 7638 keys: 119 us with tiles of 128 rows and 60 splits, 20.4 with 16 rows and 12).
 constexpr int kRows[3] = {16, 32, 128};
 double cost_us(int i, int64_t units, int splits, int group, int head_dim, int max_keys, int single, int cus) {
     constexpr double kStart[3] = {6.097, 7.606, 7.066}, kLatency[3] = {0.0089, 0.0092, 0.0165}, kRate[3] = {0.0185, 0.0165, 0.0443},

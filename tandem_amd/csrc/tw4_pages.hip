@@ -88,9 +88,10 @@ __device__ __forceinline__ void scan2(int& x, int& y, int& tx, int& ty, int (*pa
     y = by + sy - y;
 }
 
-// STEP: the table is a cache's own, so an entry behind a request's length is a page it already has (its length was taken back): it stays, and
-// only entries that are none (-1) take pages, in the order of their places. Tokens behind row a.tokens - 1 are not computed in this step,
-// so starts and lengths end there too: they come again, and find the pages they were given.
+// STEP: the table is a cache's own, so an entry behind a request's length is a page it already has (its length was taken back): it
+// stays, and only entries that are none (-1) take pages, in the order of their places. Tokens behind row a.tokens - 1 are not computed in
+// this step, so starts and lengths end there too: they come again, and find the pages they were given. One request in decode takes 3.0-3.2 us,
+// 0.1 more than without STEP, 64 prompts of 40 tokens 0.5 more: a round trip to the entries and a scan of what they lack.
 template <bool STEP>
 __global__ void __launch_bounds__(kThreads) pages_kernel(PageArgs a, int rows) {
     __shared__ int part[kThreads / 64][2];
@@ -186,8 +187,9 @@ __global__ void __launch_bounds__(256) rows_kernel(PageArgs a) {
 
 // The pages of the listed requests go back to the front of what is left of the free list, each request's (1024 of them at a time) before
 // those of the one before it;
-// their rows of the table become -1 and their lengths 0. WHOLE: every page of the row, not those of the request's length only. One
-// workgroup: it runs when requests end.
+// their rows of the table become -1 and their lengths 0. WHOLE: every page of the row, not those of the request's length only.
+// It is bound by two barriers and a round trip to memory for each 1024 columns of each request, one after another: with 512 columns one
+// request 1.7 us, 8 6.6, 64 47-49; with 2501 3.2, 19 and 142. One workgroup all the same: it runs when requests end, not in every step.
 template <bool WHOLE>
 __global__ void __launch_bounds__(kThreads) release_kernel(const int32_t* ended, int count, int32_t* table, int64_t table_stride,
                                                            int width, int32_t* lens, int batch, int32_t* free_pages, int n_free,

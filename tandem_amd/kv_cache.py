@@ -72,8 +72,8 @@ def plan_pages(context_lens: torch.Tensor, query_lens: torch.Tensor, page_table:
 
     int32 GPU tensors; lengths below zero count as zero, and each new length and all new tokens together are below 2^31. seq_lens_out (context_lens
     itself, to advance it) and taken_out (taken itself) are written instead of new tensors. Nothing is read back; the caller that
-    wants to know whether the pages sufficed reads counts[2]. Tokens past num_tokens (counts[3]) have pages, and count in seq_lens and query_start, but no
-    position or slot."""
+    wants to know whether the pages sufficed reads counts[2]. Tokens past num_tokens (counts[3]) have pages, and count in seq_lens and
+    query_start, but no position or slot."""
     outs = () if seq_lens_out is None else (("seq_lens_out", layout(seq_lens_out), None),)
     if taken_out is not None:
         outs += (("taken_out", layout(taken_out), 1),)
@@ -169,12 +169,13 @@ class PagedKVCache:
     @classmethod
     def for_model(cls, config: "DecoderConfig", num_pages: int, max_requests: int, max_seq_len: int, page_size: int = 16,
                   device: torch.device | str = "cuda") -> "PagedKVCache":
-        """A cache of float16 for a DecoderModel of this configuration."""
+        """A cache of float16 for a DecoderModel of this configuration. NotImplementedError where it asks for attention that the model
+        does not compute."""
         if config.rope_type != "default":
             raise NotImplementedError(f"rope_scaling of type {config.rope_type!r}: only plain rotary positions are supported")
         if config.sliding_window is not None and config.sliding_window < max_seq_len:
-            raise NotImplementedError(f"sliding_window {config.sliding_window}: only attention over all keys is supported (a cache of no more "
-                                      f"than that per request is; got max_seq_len {max_seq_len})")
+            raise NotImplementedError(f"sliding_window {config.sliding_window}: only attention over all keys is supported (a cache of no "
+                                      f"more than that per request is; got max_seq_len {max_seq_len})")
         if config.other_attention:
             raise NotImplementedError(f"attention with {', '.join(config.other_attention)} is not supported")
         return cls(config.num_layers, config.num_kv_heads, config.head_dim, num_pages, max_requests, max_seq_len, page_size,

@@ -68,8 +68,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 
     page_table int32 [B, pages per request] (any row stride), seq_lens int32 [B], query_start int32 [B + 1], ascending from 0.
     They are read on the GPU only, and nothing outside of the tensors is touched whatever they hold: keys of an entry that is no
-    page, or behind the table's width, are left out, and a row that sees no key is zero. Infinities and NaN of keys and values
-    reach the rows that see them and no others. Rows from query_start[B] on are left as they were in ``out``.
+    page, or behind the table's width, are left out, and a row that sees no key (or none with a score above -inf) is zero.
+    Infinities and NaN of keys and values reach the rows that see them and no others. Rows from query_start[B] on are left as they
+    were in ``out``.
 
     max_query_len, max_seq_len: bounds the host knows; they only choose how the work is divided (T and the table's width
     otherwise). Results do not depend on the order in which workgroups run. Inference only."""

@@ -8,8 +8,8 @@
 A head x of D values becomes y = x rsqrt(mean(x^2) + eps) weight (no weight: y = x), and then, with the angle a_i of its
 token's position, (y[i] cos a_i - y[i + D/2] sin a_i, y[i + D/2] cos a_i + y[i] sin a_i): the halves of a head rotate
 against each other, as in the Qwen3 and Llama checkpoints of Hugging Face. fp32 arithmetic, one rounding. float16 and
-bfloat16, heads of 64 or 128 values. Inference only: a projection or a cache that a gradient, tangent or transform follows is refused, and the
-weights and the table are taken as values, as in layers/norm.py.
+bfloat16, heads of 64 or 128 values. Inference only: a projection or a cache that a gradient, tangent or transform follows is
+refused, and the weights and the table are taken as values, as in layers/norm.py.
 """
 
 from __future__ import annotations
@@ -134,9 +134,9 @@ def norm_rope(qkv: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, n
 def norm_rope_cache(qkv: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, num_heads: int, num_kv_heads: int,
                     k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor, q_weight: torch.Tensor | None = None,
                     k_weight: torch.Tensor | None = None, eps: float = 1e-6) -> torch.Tensor:
-    """norm_rope whose keys, and the values as they are, go into the caches [pages, KV heads, page size, head_dim]: token t's
-    at slots[t] = page * page size + offset (int32 [T]; outside of the cache: nowhere). The two caches share no place (one tensor may hold
-    both, as views). Slots are distinct; of two tokens
-    with one slot either may win. Returns the queries [T, heads, head_dim]."""
+    """norm_rope whose keys, and the values as they are, go into the caches [pages, KV heads, page size, head_dim]: token t's at
+    slots[t] = page * page size + offset (int32 [T]; outside of the cache: nowhere). The two caches share no place (one tensor may
+    hold both, as views). Slots are distinct; of two tokens with one slot either may win, head by head. Returns the queries [T,
+    heads, head_dim]."""
     return _run("norm_rope_cache", qkv, positions, table, num_heads, num_kv_heads, q_weight, k_weight, eps, k_cache,
                 v_cache, slots)[0]

@@ -16,7 +16,7 @@ A model is called with token ids alone, or with a step over a paged cache (tande
     cache = PagedKVCache.for_model(cfg, num_pages=4096, max_requests=32, max_seq_len=8192)
     batch = cache.plan(query_lens, num_tokens)          # lanes' new tokens: prompts, chunks, single tokens, any mix
     hidden = model(input_ids, batch)                    # [num_tokens] ids, lane by lane
-    logits = model.compute_logits(hidden[batch.query_start[1:].long() - 1])   # each lane's last token
+    logits = model.compute_logits(hidden[batch.query_start[1:].long() - 1])   # last token of each lane that has one
 
 With it, each layer normalises (Qwen3) and rotates queries and keys into the cache in one kernel and attends over the lane's
 pages (python/tandem/layers/attention.py, triton_ops.py, flashinfer_attention.py). Without it, ``Attention.attend`` computes
@@ -72,7 +72,8 @@ class DecoderConfig:
         rope = d.get("rope_parameters") or d.get("rope_scaling") or {}
         head_dim = int(d.get("head_dim") or d["hidden_size"] // heads)
         # Qwen's configurations name a window that is off unless asked for, and then in the layers from max_window_layers on
-        slides = d.get("use_sliding_window", not kind.startswith("qwen")) and int(d.get("max_window_layers") or 0) < int(d["num_hidden_layers"])
+        slides = (d.get("use_sliding_window", not kind.startswith("qwen"))
+                  and int(d.get("max_window_layers") or 0) < int(d["num_hidden_layers"]))
         window = d.get("sliding_window") if ("sliding_attention" in layers if layers else slides) else None
         scale = head_dim ** -0.5
         other = {"partial_rotary_factor": any(float(f.get("partial_rotary_factor") or 1.0) != 1.0 for f in (d, rope)),
