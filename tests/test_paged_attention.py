@@ -521,4 +521,3 @@ def test_plan_against_the_timed_choices():
             if c["fitted"] == fitted and chosen is not None:
                 ratios.append(chosen / min(c["us"].values()))
         assert len(ratios) >= least and sum(ratios) / len(ratios) < 1.02 and max(ratios) < 1.25, (fitted, len(ratios))
-        print(fitted, len(ratios), sum(ratios) / len(ratios), max(ratios))

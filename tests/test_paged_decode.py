@@ -299,3 +299,36 @@ def test_attention_that_the_model_does_not_compute_is_refused():
         PagedKVCache.for_model(dataclasses.replace(cfg, num_layers=1), **layers)
     # a cache that no request can outgrow the window of
     PagedKVCache.for_model(dataclasses.replace(tmodel.DecoderConfig.from_hf({**hf, "sliding_window": 4096}), num_layers=1), **dict(small, max_seq_len=4096))
+
+
+@pytest.mark.gpu
+def test_drafted_tokens_taken_back_match_oracle(monkeypatch):
+    """Drafts scored in one pass, most of them taken back, single tokens in the captured step, drafts again: every row is the oracle's for
+    the tokens that stayed, and no page is lost."""
+    model, w = _model(monkeypatch, 17)
+    cache = PagedKVCache.for_model(CFG, num_pages=14, max_requests=2, max_seq_len=112)
+    rng = np.random.default_rng(4)
+    draw = lambda n: rng.integers(0, CFG.vocab_size, n).tolist()  # noqa: E731
+    seqs = [draw(14), draw(30)]
+    _step(model, cache, seqs)
+    runner = decode_graph.DecodeGraphRunner(model, max_bs=2, device=torch.device("cuda", 0), cache=cache)
+    for kept in ((1, 3), (0, 17), (20, 2)):
+        drafts = [draw(20), draw(18)]
+        logits = _step(model, cache, drafts)
+        at = 0
+        for lane, (draft, keep) in enumerate(zip(drafts, kept)):
+            one_token._close(logits[at:at + len(draft)], _oracle(w, seqs[lane] + draft)[-len(draft):], 0.02, (kept, lane))
+            at += len(draft)
+            seqs[lane] += draft[:keep]
+        cache.context_lens -= _int([20 - kept[0], 18 - kept[1]])
+        assert cache.context_lens.tolist() == [len(s) for s in seqs]
+        for _ in range(2):
+            ids = draw(2)
+            got = runner.run(ids).clone()
+            for lane, x in enumerate(ids):
+                seqs[lane].append(x)
+                one_token._close(got[lane:lane + 1], _oracle(w, seqs[lane])[-1:], 0.02, (kept, lane))
+        held = [p for r in cache.page_table.tolist() for p in r if p >= 0]
+        assert sorted(held + cache.free_pages.tolist()[int(cache.taken):]) == list(range(14))
+    cache.release([1, 0])
+    assert int(cache.taken) == 0 and sorted(cache.free_pages.tolist()) == list(range(14))
