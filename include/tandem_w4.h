@@ -362,6 +362,26 @@ int tw4_rms_norm(const uint16_t* x, const uint16_t* weight, uint16_t* y, int M, 
 int tw4_add_rms_norm(uint16_t* x, uint16_t* residual, const uint16_t* weight, int M, int K,
                      float eps, void* stream);
 
+/* Rows of activations in 8-bit integers with a scale for each row. x [M, K] of fp16 (bf16 = 1: bfloat16), rows x_stride values
+ * apart -> codes int8 [M, K], scales float32 [M]: scale = max|x| / 127, code = 127 x / max|x| rounded to nearest, halves to even,
+ * exactly. A row with an infinity or NaN has scale NaN and codes 0; one whose largest magnitude is below 2^-100 has scale 0 and codes
+ * 0. K % 16 == 0, K <= TW4_ROWS8_MAX, rows and codes 16-byte aligned. No reference counterpart. */
+#define TW4_ROWS8_MAX 32768
+int tw4_quantize_int8(const uint16_t* x, int64_t x_stride, int8_t* codes, float* scales, int M, int K, int bf16, void* stream);
+
+/* tw4_rms_norm (residual NULL) or tw4_add_rms_norm (residual <- the type's rounding of s = x + residual, x is left as it is) with
+ * its output y = s rsqrt(mean(s^2) + eps) weight, unrounded, in 8-bit integers: scale = max|y| / 127, code = 127 t / max|t| rounded as in
+ * tw4_quantize_int8, t = s weight, of whose exact values the codes are exactly rounded. Infinities, NaN and small rows as there, by t. */
+int tw4_rms_norm_int8(const uint16_t* x, int64_t x_stride, uint16_t* residual, int64_t r_stride, const uint16_t* weight,
+                      float eps, int8_t* codes, float* scales, int M, int K, int bf16, void* stream);
+
+/* Product of 8-bit integers: y[m, n] = x_scale[m] w_scale[n] sum_k x[m, k] w[n, k], x int8 [M, K] and w int8 [N, K] with rows
+ * x_stride and w_stride bytes apart (16-byte aligned, less than 2^22 apart), x_scale float32 [M], w_scale float32 [N]; y of fp16 (bf16 = 1:
+ * bfloat16), rounded once. act = 1: w's rows are [gate | up] (N even) and y [M, N / 2] = silu(gate) up. K % 16 == 0, K < 2^17 (the sum
+ * is exact in 32 bits), M <= 2^20, N <= 2^24. No reference counterpart. */
+int tw4_gemm_int8(const int8_t* x, int64_t x_stride, const float* x_scale, const int8_t* w, int64_t w_stride,
+                  const float* w_scale, uint16_t* y, int M, int N, int K, int act, int bf16, void* stream);
+
 /* Streaming-read probe: reads `bytes` (a multiple of 16) from the device buffer `src` with 16-byte
  * non-temporal loads (1 KB per wavefront instruction, `inflight` = 1, 2, 4 or 8 issued per lane
  * before any is used) over `workgroups`

@@ -1,5 +1,5 @@
 """Projection factory of the decoder layers: a plain nn.Linear for an unquantized checkpoint, a
-W4Linear for an AutoAWQ one. Same two entry points and signatures as
+W4Linear for an AutoAWQ one, a W8Linear for one in 8-bit integers. Same two entry points and signatures as
 python/tandem/layers/linear.py:10-31 (make_linear, finalize_quantized)."""
 
 from __future__ import annotations
@@ -13,11 +13,15 @@ def make_linear(in_features: int, out_features: int, bias: bool = False, quant: 
     """The projection module for one weight. ``quant`` is None (dense float weights) or a
     quantization description with a ``group_size`` attribute (``tandem_amd.loader.QuantConfig``).
     A W4Linear is created empty: it holds only the AutoAWQ tensors the loader fills, never a dense
-    copy of the weight, and is usable once ``finalize_quantized`` has run. The W4A16 kernels have
-    no bias term, so a biased quantized projection is refused."""
+    copy of the weight, and is usable once ``finalize_quantized`` has run. A ``bits`` attribute of 8 makes
+    a W8Linear. The quantized kernels have no bias term, so a biased quantized projection is refused."""
     if quant is not None:
         if bias:
             raise NotImplementedError("quantized projections with a bias")
+        if getattr(quant, "bits", 4) == 8:
+            from tandem_amd.layers.w8 import W8Linear
+
+            return W8Linear(in_features, out_features)
         from tandem_amd.layers.awq import W4Linear
 
         return W4Linear(in_features, out_features, quant.group_size)

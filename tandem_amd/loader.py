@@ -1,10 +1,12 @@
-"""Put an AutoAWQ "gemm" checkpoint into a model built from W4Linear (and nn.Linear) projections.
+"""Put an AutoAWQ "gemm" checkpoint, or one in 8-bit integers, into a model built from W4Linear or W8Linear (and nn.Linear)
+projections.
 
 Behaviour kept from 12vivi/tandem (python/tandem/model_config.py:28-43 for ``QuantConfig``,
 python/tandem/models/loader.py:66-105 for ``load_weights``):
 
-- only 4-bit AWQ "gemm" checkpoints with zero points are accepted; anything else raises
-  NotImplementedError, and an absent quantization_config means an unquantized model;
+- 4-bit AWQ "gemm" checkpoints with zero points are accepted, and (beyond the reference) compressed-tensors checkpoints
+  in 8-bit integers with a scale for each output channel and activations quantised token by token; anything else
+  raises NotImplementedError, and an absent quantization_config means an unquantized model;
 - the model's fused projections take their halves from the checkpoint's separate ones
   (q / k / v -> qkv_proj, gate / up -> gate_up_proj), in that order along the output features;
 - a tensor the model has no use for is logged and skipped (a stored lm_head of a tied-embedding
@@ -38,11 +40,13 @@ from torch import nn
 logger = logging.getLogger(__name__)
 
 AWQ_TENSORS = ("qweight", "qzeros", "scales")
+W8_TENSORS = ("weight", "weight_scale")
 
 
 @dataclass(frozen=True)
 class QuantConfig:
-    """The ``quantization_config`` entry of a checkpoint's config.json, for weight-only AWQ."""
+    """The ``quantization_config`` entry of a checkpoint's config.json, for weight-only AWQ and int8 weights and activations (bits
+    8; group_size is then 0: a channel)."""
 
     method: str
     bits: int
@@ -55,6 +59,8 @@ class QuantConfig:
         raises NotImplementedError, naming what does not fit, for every other scheme."""
         if not d:
             return None
+        if d.get("quant_method") == "compressed-tensors":
+            return cls._int8(d)
         reasons = []
         if d.get("quant_method") != "awq":
             reasons.append(f"quant_method {d.get('quant_method')!r} (only 'awq')")
@@ -68,14 +74,50 @@ class QuantConfig:
             raise NotImplementedError(f"cannot load quantization_config {d}: " + "; ".join(reasons))
         return cls("awq", 4, int(d.get("group_size", 128)))
 
+    @classmethod
+    def _int8(cls, d: dict[str, Any]) -> "QuantConfig":
+        """compressed-tensors' "int-quantized" form of every Linear but the head: symmetric int8 weights with a scale for each
+        output channel, activations quantised to symmetric int8 token by token as they come."""
+        groups = d.get("config_groups")
+        groups = list(groups.values()) if isinstance(groups, dict) else []
+        group = groups[0] if len(groups) == 1 and isinstance(groups[0], dict) else {}
+        reasons = [] if group else [f"{len(groups)} config_groups (only one, for all projections)"]
+        if d.get("format") != "int-quantized":
+            reasons.append(f"format {d.get('format')!r} (only 'int-quantized')")
+        if group.get("format") not in (None, "int-quantized"):
+            reasons.append(f"a group's format {group.get('format')!r} (only 'int-quantized')")
+        if group and list(group.get("targets") or ()) != ["Linear"]:
+            reasons.append(f"targets {group.get('targets')!r} (only ['Linear'])")
+        if any(x != "lm_head" for x in d.get("ignore") or ()):
+            reasons.append(f"ignore {d.get('ignore')!r} (only the lm_head)")
+        if group and "lm_head" not in (d.get("ignore") or ()):
+            reasons.append("a quantized lm_head")
+        for name, wanted in (("weights", {"strategy": "channel", "dynamic": False}), ("input_activations", {"strategy": "token", "dynamic": True})):
+            args = group.get(name) or {}
+            for key, value in {"num_bits": 8, "type": "int", "symmetric": True, **wanted}.items():
+                if args.get(key, False if key == "dynamic" else None) != value:
+                    reasons.append(f"{name} with {key} {args.get(key)!r} (only {value!r})")
+            if args.get("actorder") not in (None, False):
+                reasons.append(f"{name} with actorder {args['actorder']!r}")
+        for name, asked in (("output_activations", group.get("output_activations")), ("kv_cache_scheme", d.get("kv_cache_scheme")),
+                            ("sparsity_config", (d.get("sparsity_config") or {}).get("format") not in (None, "dense")),
+                            ("transform_config", (d.get("transform_config") or {}).get("config_groups"))):
+            if asked:
+                reasons.append(name)
+        if d.get("quantization_status") not in (None, "compressed"):
+            reasons.append(f"quantization_status {d['quantization_status']!r} (only 'compressed')")
+        if reasons:
+            raise NotImplementedError(f"cannot load quantization_config {d}: " + "; ".join(reasons))
+        return cls("compressed-tensors", 8, 0)
+
 
 # Model tensors assembled from several checkpoint tensors: (model-name pattern, parts in stacking
 # order). The attention prefix may sit anywhere in the module tree; the MLP pattern names the
 # dense decoder MLP only (a mixture-of-experts layer's "mlp.experts.E.*" never matches).
 _FUSED = (
-    (re.compile(r"^(?P<pre>.+\.self_attn)\.qkv_proj\.(?P<t>weight|bias|qweight|qzeros|scales)$"),
+    (re.compile(r"^(?P<pre>.+\.self_attn)\.qkv_proj\.(?P<t>weight|weight_scale|bias|qweight|qzeros|scales)$"),
      ("q_proj", "k_proj", "v_proj")),
-    (re.compile(r"^(?P<pre>model\.layers\.\d+\.mlp)\.gate_up_proj\.(?P<t>weight|qweight|qzeros|scales)$"),
+    (re.compile(r"^(?P<pre>model\.layers\.\d+\.mlp)\.gate_up_proj\.(?P<t>weight|weight_scale|qweight|qzeros|scales)$"),
      ("gate_proj", "up_proj")),
 )
 # Checkpoint tensors that are never model state (buffers older exporters saved).
@@ -93,9 +135,9 @@ def fused_sources(target: str) -> Optional[tuple[list[str], int]]:
 
 
 def model_tensors(model: nn.Module) -> dict[str, torch.Tensor]:
-    """What a checkpoint fills: every parameter, and the AutoAWQ buffers W4Linear registers."""
+    """What a checkpoint fills: every parameter, and the buffers W4Linear (AutoAWQ) and W8Linear register."""
     out = dict(model.named_parameters())
-    out.update((n, b) for n, b in model.named_buffers() if n.rsplit(".", 1)[-1] in AWQ_TENSORS)
+    out.update((n, b) for n, b in model.named_buffers() if n.rsplit(".", 1)[-1] in AWQ_TENSORS + W8_TENSORS)
     return out
 
 
@@ -124,7 +166,7 @@ def _stacked_shape(shapes: list[tuple[int, ...]], axis: int) -> Optional[tuple[i
 
 
 def load_weights(model: nn.Module, model_path: str) -> None:
-    """Fill every parameter of ``model`` and the AutoAWQ buffers of its W4Linear layers from the
+    """Fill every parameter of ``model`` and the buffers of its W4Linear and W8Linear layers from the
     *.safetensors files in ``model_path`` (CPU tensors, cast to each target's dtype)."""
     from safetensors import safe_open
 
@@ -149,6 +191,8 @@ def load_weights(model: nn.Module, model_path: str) -> None:
             for name, (srcs, axis) in plans.items():
                 dst = targets[name]
                 parts = [where[s].get_tensor(s) for s in srcs]
+                if dst.dtype == torch.int8 and any(p.dtype != torch.int8 for p in parts):
+                    raise ValueError(f"{name}: int8 tensors expected, checkpoint {[str(p.dtype) for p in parts]}")
                 dst.copy_((parts[0] if len(parts) == 1 else torch.cat(parts, dim=axis)).to(dst.dtype))
         used = {s for srcs, _ in plans.values() for s in srcs}
         extra = sorted(n for n in where if n not in used and n != "lm_head.weight" and not n.endswith(_NOT_STATE))

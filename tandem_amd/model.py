@@ -23,11 +23,12 @@ pages (python/tandem/layers/attention.py, triton_ops.py, flashinfer_attention.py
 attention over a one-token context, the first decode position: softmax over a single key is 1, so each query head's output is the
 value row of its KV head (grouped-query attention), one small copy kernel. At position 0 that is what the cached form gives.
 
-Projections are W4Linear (AutoAWQ checkpoints) or nn.Linear (fp16 checkpoints); ``prepare`` moves
+Projections are W4Linear (AutoAWQ checkpoints), W8Linear (int8 checkpoints) or nn.Linear (fp16 checkpoints); ``prepare`` moves
 the model to the GPU, repacks the W4 layers and routes the fp16 projections and the logits head
 through layers/gemv16.py's table. Norms run on tw4_rms_norm / tw4_add_rms_norm, or inside the W4
 qkv_proj / gate_up_proj kernels where W4Linear.forward_norm fuses them (the decode GEMV at the
-batch sizes it runs: a norm kernel fewer before each, the same bits).
+batch sizes it runs: a norm kernel fewer before each, the same bits). A W8Linear's come out of the norm in 8 bits
+(tw4_rms_norm_int8).
 """
 
 from __future__ import annotations
@@ -43,6 +44,7 @@ from tandem_amd.kv_cache import PagedBatch
 from tandem_amd.layers import gemv16, norm, rotary, w4_hip
 from tandem_amd.layers.linear import finalize_quantized, make_linear
 from tandem_amd.layers.paged_attention import paged_attention
+from tandem_amd.layers.w8 import W8Linear
 
 
 @dataclass(frozen=True)
@@ -192,7 +194,7 @@ class DecoderLayer(nn.Module):
         step = () if batch is None else (batch, layer)
         n1, n2 = self.input_layernorm, self.post_attention_layernorm
         attn, mlp = self.self_attn, self.mlp
-        if hasattr(attn.qkv_proj, "forward_norm"):  # W4: the norm goes into the projection's prologue
+        if hasattr(attn.qkv_proj, "forward_norm"):  # W4: the norm goes into the projection's prologue; W8: it writes what that reads
             qkv, residual = attn.qkv_proj.forward_norm(hidden, residual, n1.weight, n1.eps)
             hidden = attn.o_proj(attn.attend(qkv, *step))
         else:
@@ -259,8 +261,9 @@ def prepare(model: DecoderModel, device: torch.device, device_name: Optional[str
 def init_random(model: DecoderModel, seed: int = 0) -> DecoderModel:
     """Synthetic weights of the architecture, generated on the model's device: AutoAWQ tensors with
     uniform int4 q and z and fp16 scales U[0.001, 0.02] (the reference tests' recipe), fp16
-    projections N(0, 0.02), embeddings N(0, 1), norm weights 1 + U(-0.1, 0.1). Head norms are drawn from a generator of their
-    own: the other weights of a seed are the same with and without them."""
+    projections N(0, 0.02), int8 ones of that size (scales of 0.02 / 36 for codes of deviation 36), embeddings N(0, 1), norm
+    weights 1 + U(-0.1, 0.1). Head norms are drawn from a generator of their own: the other weights of a seed are the same with and
+    without them."""
     dev = next(model.parameters()).device
     g = torch.Generator(device=dev).manual_seed(seed)
     heads = torch.Generator(device=dev).manual_seed(seed + 1)
@@ -269,6 +272,9 @@ def init_random(model: DecoderModel, seed: int = 0) -> DecoderModel:
             for t in (mod.qweight, mod.qzeros):
                 t.copy_(torch.randint(-2**31, 2**31 - 1, t.shape, device=dev, dtype=torch.int32, generator=g))
             mod.scales.copy_((torch.rand(mod.scales.shape, device=dev, generator=g) * 0.019 + 0.001).half())
+        elif isinstance(mod, W8Linear):
+            mod.weight.copy_((torch.randn(mod.weight.shape, device=dev, generator=g) * 36).round().clamp(-127, 127))
+            mod.weight_scale.copy_((torch.rand(mod.weight_scale.shape, device=dev, generator=g) * 0.4 + 0.8) * (0.02 / 36))
     for name, p in model.named_parameters():
         if name.endswith("embed_tokens.weight"):
             p.copy_(torch.randn(p.shape, device=dev, generator=g))

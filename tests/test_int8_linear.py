@@ -1,0 +1,260 @@
+"""Products of 8-bit integers (tw4_gemm_int8 behind layers/w8.py) against the formula in 64 bits.
+
+Tolerance. The sum of products is exact; made a float32 (2^-24 of it, nothing below 2^24), times one scale and the other: 3 roundings of 2^-24,
+and one to the type, half a step of it (fp16 2^-11, bf16 2^-8, and 2^-25 absolute where fp16 is subnormal). SwiGLU: gate and up
+have those 3 each; the gate's change the sigmoid by |g| 3 roundings at most; exp(-g) is off by its argument's roundings, 2 |g|, and 2
+of its own, addition, division and product by 3: (3 + 3 + 2 + 3 + 5 |g|) of 2^-24."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+from torch import nn
+
+from tandem_amd import model as tmodel
+from tandem_amd.layers import linear, norm, w4_hip, w8
+from tandem_amd.loader import QuantConfig
+
+HALF_STEP = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+INT8 = QuantConfig("compressed-tensors", 8, 0)
+
+
+# ------------------------------------------------------------------------------------------- CPU
+def test_argument_errors_return_before_launch():
+    lib, p, odd = w4_hip.library(), ctypes.c_void_p(4096), ctypes.c_void_p(4104)
+    #       x stride xs w stride ws y M N K act bf16
+    good = [p, 64, p, p, 64, p, p, 3, 5, 64, 0, 0]
+    for at, value, needle in ((0, None, "null"), (2, None, "null"), (3, None, "null"), (5, None, "null"), (6, None, "null"),
+                              (0, odd, "aligned"), (3, odd, "aligned"), (2, ctypes.c_void_p(4098), "aligned"),
+                              (6, ctypes.c_void_p(4097), "aligned"), (1, 48, "apart"), (1, 72, "apart"), (4, 48, "apart"), (4, 1 << 22, "apart"),
+                              (7, -1, "M"), (7, (1 << 20) + 1, "M"), (8, 0, "N"), (8, (1 << 24) + 1, "N"), (9, 72, "K"), (9, 0, "K"),
+                              (9, 1 << 17, "K"), (10, 2, "act"), (10, 1, "even")):
+        args = list(good)
+        args[at] = value
+        assert lib.tw4_gemm_int8(*args, None) == w4_hip.TW4_EINVAL, (at, value)
+        assert needle in lib.tw4_last_error().decode(), (at, value, lib.tw4_last_error())
+    good[7] = 0
+    assert lib.tw4_gemm_int8(*good, None) == w4_hip.TW4_OK
+
+
+def test_refusals_on_the_cpu():
+    x, s, w = torch.zeros(2, 64, dtype=torch.int8), torch.ones(2), torch.zeros(3, 64, dtype=torch.int8)
+    with pytest.raises(RuntimeError, match="GPU"):
+        w8.linear_int8(x, s, w, torch.ones(3))
+
+    def lay(shape, stride, dtype=torch.int8, index=0):
+        return torch.Size(shape), stride, dtype, index
+
+    def f32(*shape):
+        return lay(shape, (1,) * len(shape), torch.float32)
+
+    x, w = lay((2, 64), (64, 1)), lay((6, 64), (64, 1))
+    assert w8._checked(x, f32(2), w, f32(6, 1), True, torch.float16) == (64, 64, (2, 6, 64), 3, 0, 0)
+    assert w8._checked(lay((1, 64), (7, 1)), f32(1), w, f32(6), False, torch.bfloat16) == (64, 64, (1, 6, 64), 6, 1, 0)
+    for bad in ((x, f32(3), w, f32(6), False, torch.float16), (x, f32(2), w, f32(5), False, torch.float16),
+                (lay((2, 48), (64, 1)), f32(2), w, f32(6), False, torch.float16), (x, f32(2), w, f32(6), False, torch.float32),
+                (x, f32(2), lay((5, 64), (64, 1)), f32(5), True, torch.float16), (lay((2, 64), (72, 1)), f32(2), w, f32(6), False, torch.float16),
+                (x, f32(2), lay((6, 64), (1, 6)), f32(6), False, torch.float16), (x, f32(2), lay((6, 64), (64, 1), torch.uint8), f32(6), False, torch.float16),
+                (x, f32(2), lay((6, 64), (64, 1), torch.int8, 1), f32(6), False, torch.float16), (x, lay((2,), (1,), torch.float16), w, f32(6), False, torch.float16),
+                (x, lay((2,), (2,), torch.float32), w, f32(6), False, torch.float16), (lay((2, 1 << 17), (1 << 17, 1)), f32(2), lay((6, 1 << 17), (1 << 17, 1)), f32(6), False, torch.float16),
+                (lay((2, 64), (0, 1)), f32(2), w, f32(6), False, torch.float16), (lay((2, 64), (1 << 22, 1)), f32(2), w, f32(6), False, torch.float16)):
+        with pytest.raises(RuntimeError, match="^linear_int8: "):
+            w8._checked(*bad)
+
+
+def test_layer_without_a_gpu():
+    layer = linear.make_linear(64, 24, False, INT8)
+    assert isinstance(layer, w8.W8Linear) and layer.weight.shape == (24, 64) and layer.weight_scale.shape == (24, 1)
+    layer.weight.fill_(-128)
+    layer.weight_scale.copy_(torch.arange(24)[:, None] * 1e-9 + 1e-7)  # nothing float16 could hold
+    scale = layer.weight_scale.clone()
+    box = nn.ModuleList([layer, nn.Linear(4, 4)]).to(dtype=torch.float16)
+    assert box[1].weight.dtype == torch.float16 and layer.weight.dtype == torch.int8
+    assert layer.weight_scale.dtype == torch.float32 and torch.equal(layer.weight_scale, scale)
+    assert linear.finalize_quantized(box) == 0 and layer.enable_silu_mul()
+    with pytest.raises(NotImplementedError):
+        linear.make_linear(64, 24, True, INT8)
+    for bad in ((72, 8), (0, 8), (32784, 8), (64, 0)):
+        with pytest.raises(ValueError):
+            w8.W8Linear(*bad)
+    assert not w8.W8Linear(64, 23).enable_silu_mul()
+
+
+# ------------------------------------------------------------------------------------------- GPU
+def _operands(m, n, k, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randint(-127, 128, (m, k), device="cuda", dtype=torch.int8, generator=g)
+    w = torch.randint(-128, 128, (n, k), device="cuda", dtype=torch.int8, generator=g)
+    xs = (0.5 + torch.rand(m, device="cuda", generator=g)) * 0.02
+    ws = (0.5 + torch.rand(n, device="cuda", generator=g)) * 0.02 * k ** -0.5
+    return x, xs, w, ws
+
+
+def _check(y, x, xs, w, ws, silu_mul, dtype):
+    exact = torch.matmul(x.cpu().double(), w.cpu().double().t()) * xs.cpu().double()[:, None] * ws.cpu().double()
+    steps = 3.0
+    if silu_mul:
+        g, u = exact.chunk(2, dim=1)
+        exact, steps = g * torch.sigmoid(g) * u, 11 + 5 * g.abs()
+    assert y.dtype == dtype and y.shape == exact.shape
+    off = (y.cpu().double() - exact).abs()
+    allowed = (HALF_STEP[dtype] + steps * 2.0 ** -24 * 1.01) * exact.abs() + (2.0 ** -25 if dtype == torch.float16 else 2.0 ** -130)
+    assert bool((off <= allowed).all()), (float((off / exact.abs().clamp(min=1e-9)).max()), int((off > allowed).sum()))
+
+
+SHAPES = [(1, 1, 16), (1, 17, 48), (1, 256, 4096), (2, 6, 64), (3, 130, 2064), (4, 4096, 1024), (5, 100, 4096), (7, 33, 112), (8, 500, 1040),
+          (15, 64, 128), (16, 2048, 512), (17, 34, 80), (24, 1000, 4096), (31, 48, 16), (32, 512, 12288), (33, 258, 272), (48, 4096, 1024),
+          (63, 70, 336), (64, 1024, 2048), (65, 130, 528), (77, 1536, 1024), (100, 62, 4096), (127, 128, 64), (128, 256, 256), (129, 514, 640),
+          (200, 2000, 512), (255, 250, 1008), (256, 256, 4096), (257, 30, 2064), (300, 5002, 272), (512, 512, 512), (513, 1026, 144),
+          (700, 2, 4096), (1024, 1280, 1024), (1500, 766, 1040), (2049, 258, 128)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("silu_mul", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_linear(m, n, k, dtype, silu_mul):
+    x, xs, w, ws = _operands(m, n + (n % 2 if silu_mul else 0), k, seed=m + n + k)
+    kept = [t.clone() for t in (x, xs, w, ws)]
+    y = w8.linear_int8(x, xs, w, ws, silu_mul=silu_mul, dtype=dtype)
+    _check(y, x, xs, w, ws, silu_mul, dtype)
+    assert all(torch.equal(a, b) for a, b in zip(kept, (x, xs, w, ws)))
+    assert torch.equal(y, w8.linear_int8(x, xs[:, None], w, ws[:, None], silu_mul=silu_mul, dtype=dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("silu_mul", [False, True])
+@pytest.mark.parametrize("n,k", [(514, 1040), (4096, 4096), (96, 12288)])
+def test_rows_do_not_depend_on_the_batch(n, k, silu_mul):
+    """Sums are exact and the epilogue is a value's own: a token's result is the same bits in every batch and kernel."""
+    x, xs, w, ws = _operands(1100, n, k, seed=n)
+    want = w8.linear_int8(x, xs, w, ws, silu_mul=silu_mul)
+    for m in (1, 2, 5, 16, 17, 33, 64, 65, 100, 128, 200, 256, 300, 511, 600, 1025):
+        assert torch.equal(w8.linear_int8(x[-m:], xs[-m:], w, ws, silu_mul=silu_mul), want[-m:]), m
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n", [(1, 5), (16, 40), (70, 48), (300, 130)])
+def test_largest_sums(m, n):
+    """K = 131056 of -128 * -128: the largest sum 32 bits hold."""
+    k = (1 << 17) - 16
+    x = torch.full((m, k), -128, dtype=torch.int8, device="cuda")
+    w = torch.full((n, k), -128, dtype=torch.int8, device="cuda")
+    w[n // 2] = 127
+    one = torch.full((max(m, n),), 2.0 ** -16, device="cuda")
+    y = w8.linear_int8(x, one[:m], w, one[:n], dtype=torch.bfloat16)
+    want = torch.full((m, n), 128 * 128 * k * 2.0 ** -32, device="cuda", dtype=torch.float64)
+    want[:, n // 2] *= -127 / 128
+    assert torch.equal(y, want.to(torch.bfloat16))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(3, 130, 1040), (40, 254, 528), (150, 258, 784), (600, 514, 272)])
+@pytest.mark.parametrize("silu_mul", [False, True])
+def test_strides_scales_and_neighbours(m, n, k, silu_mul):
+    """Operands inside larger buffers whose other places hold codes that would show; infinite, NaN and zero scales stay in their
+    rows and columns."""
+    g = torch.Generator(device="cuda").manual_seed(m)
+    bx = torch.randint(-127, 128, (m + 2, k + 96), device="cuda", dtype=torch.int8, generator=g)
+    bw = torch.randint(-127, 128, (n + 2, k + 48), device="cuda", dtype=torch.int8, generator=g)
+    x, w = bx[1:-1, 32:32 + k], bw[1:-1, 16:16 + k]
+    _, xs, _, ws = _operands(m, n, 16, seed=m)
+    ws *= k ** -0.5
+    for dtype in (torch.float16, torch.bfloat16):
+        y = w8.linear_int8(x, xs, w, ws, silu_mul=silu_mul, dtype=dtype)
+        _check(y, x, xs, w, ws, silu_mul, dtype)
+        assert torch.equal(y, w8.linear_int8(x.contiguous(), xs, w.contiguous(), ws, silu_mul=silu_mul, dtype=dtype))
+    xs2, ws2 = xs.clone(), ws.clone()
+    xs2[m // 2], ws2[1] = float("nan"), float("nan")
+    xs2[0] = 0
+    y2 = w8.linear_int8(x, xs2, w, ws2, silu_mul=silu_mul, dtype=torch.bfloat16)
+    assert bool(y2[m // 2].isnan().all()) and bool(y2[:, 1].isnan().all())
+    keep = [i for i in range(m) if i not in (0, m // 2)]
+    cols = [j for j in range(y.shape[1]) if j != 1]
+    assert torch.equal(y2[keep][:, cols], y[keep][:, cols]) and (m // 2 == 0 or not bool(y2[0, cols].any()))
+
+
+@pytest.mark.gpu
+def test_refusals_and_empty():
+    x, xs, w, ws = _operands(4, 32, 64, seed=0)
+    assert w8.linear_int8(x[:0], xs[:0], w, ws).shape == (0, 32) and w8.linear_int8(x[:0], xs[:0], w, ws, silu_mul=True).shape == (0, 16)
+    buf = torch.zeros(64 * 4 + 8, dtype=torch.int8, device="cuda")
+    with pytest.raises(RuntimeError, match="aligned"):
+        w8.linear_int8(buf[8:].view(4, 64), xs, w, ws)
+    with pytest.raises(RuntimeError, match="inference only"):
+        w8.linear_int8(x, xs.clone().requires_grad_(), w, ws)
+
+
+@pytest.mark.gpu
+def test_streams_and_graphs():
+    """Calls on two streams at once, and the whole run norm -> product -> quantise -> product captured and replayed, each against the
+    eager result, with other work between the replays."""
+    layers = []
+    for i, (k, n) in enumerate(((1024, 4096), (2048, 1024))):
+        layer = w8.W8Linear(k, n).cuda()
+        _, _, w, ws = _operands(1, n, k, seed=i)
+        layer.weight.copy_(w)
+        layer.weight_scale.copy_(ws[:, None])
+        layers.append(layer)
+    layers[0].enable_silu_mul()
+    weight = (0.5 + torch.rand(1024, device="cuda")).half()
+
+    def step(x, r):
+        y, r = layers[0].forward_norm(x, r, weight, 1e-6)
+        return layers[1](y), r
+
+    for m in (1, 9, 40, 300):
+        xs = [torch.randn(m, 1024, device="cuda").half() for _ in range(4)]
+        rs = [torch.randn(m, 1024, device="cuda").half() for _ in range(4)]
+        want = [step(x, r.clone()) for x, r in zip(xs, rs)]
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        got = {}
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+        for i in range(4):
+            with torch.cuda.stream(streams[i % 2]):
+                got[i] = step(xs[i], rs[i].clone())
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for i in range(4) for a, b in zip(got[i], want[i]))
+        graphs = []
+        for j in range(2):
+            gx, gr = xs[0].clone(), rs[0].clone()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                out = step(gx, gr)
+            graphs.append((graph, gx, gr, out))
+        for i in (1, 3, 2, 0, 1):
+            for j, (graph, gx, gr, out) in enumerate(graphs):
+                at = (i + j) % 4
+                gx.copy_(xs[at])
+                gr.copy_(rs[at])
+                graph.replay()
+                step(xs[i], rs[i].clone())
+                torch.cuda.synchronize()
+                assert torch.equal(out[0], want[at][0]) and torch.equal(gr, want[at][1])
+
+
+@pytest.mark.gpu
+def test_layer_shapes_and_norm():
+    """W8Linear is its operators one behind the other, for rows and for more dimensions."""
+    layer = w8.W8Linear(512, 96).cuda()
+    _, _, w, ws = _operands(1, 96, 512, seed=3)
+    layer.weight.copy_(w)
+    layer.weight_scale.copy_(ws[:, None])
+    x, r = torch.randn(6, 512, device="cuda").half(), torch.randn(6, 512, device="cuda").half()
+    weight = (0.5 + torch.rand(512, device="cuda")).half()
+    for silu_mul in (False, True):
+        layer.silu_mul = silu_mul
+        y = layer(x)
+        assert torch.equal(y, w8.linear_int8(*w8.quantize_int8(x), w, ws, silu_mul=silu_mul))
+        assert torch.equal(layer(x.view(2, 3, 512)), y.view(2, 3, -1)) and torch.equal(layer(x[1]), y[1])
+        assert layer(x.bfloat16()).dtype == torch.bfloat16 and layer(x[:0]).shape == (0, y.shape[1])
+        y, same = layer.forward_norm(x, None, weight, 1e-6)
+        assert same is x and torch.equal(y, w8.linear_int8(*norm.rms_norm_int8(x, weight, 1e-6), w, ws, silu_mul=silu_mul))
+        r2 = r.clone()
+        codes, scales, r3 = norm.fused_add_rms_norm_int8(x, r.clone(), weight, 1e-6)
+        y, out = layer.forward_norm(x, r2, weight, 1e-6)
+        assert out is r2 and torch.equal(r2, r3) and torch.equal(y, w8.linear_int8(codes, scales, w, ws, silu_mul=silu_mul))
+    assert tmodel.GatedMLP(512, 256, INT8).fused_act
