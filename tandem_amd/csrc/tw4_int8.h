@@ -21,8 +21,11 @@ __device__ __forceinline__ void chunk_values(const u4& v, float (&f)[8]) {
     }
 }
 
+// The float32 is rounded before it is made a 16-bit value, in every kernel alike: left to itself the compiler folds the last product into
+// the conversion (v_fma_mixlo_f16, one rounding) in some of them, and a result would depend on the kernel that a batch takes.
 template <bool BF16>
 __device__ __forceinline__ uint32_t value16(float f) {
+    asm("" : "+v"(f));
     if constexpr (BF16)
         return bitcast<uint16_t>(static_cast<__bf16>(f));
     else
@@ -57,5 +60,29 @@ __device__ __forceinline__ void store_features(uint16_t* row, int n, int N, bool
             if (n + i < N) row[n + i] = static_cast<uint16_t>(value16<BF16>(v[i]));
     }
 }
+
+struct Gemm8Args {
+    const int8_t* x;
+    int64_t x_stride;
+    const float* x_scale;
+    const int8_t* w;
+    int64_t w_stride;
+    const float* w_scale;
+    uint16_t* y;
+    int M, N, K, act, bf16;
+    int *ws, *locks;  // splits > 1: partial sums and counters, as many as these
+    int64_t ws_words, n_locks;
+    hipStream_t st;
+};
+
+// The tiles of tw4_gemm8_lds.hip: kernel number, 16-token tiles and 16-row tiles of a wavefront, wavefronts along tokens and rows, slots
+// of the ring. Kernel 0 is the streaming one of tw4_gemm8.hip.
+#define TW4_GEMM8_LDS(X)                                                                                             \
+    X(1, 1, 2, 1, 2, 7) X(2, 1, 2, 1, 2, 3) X(3, 1, 2, 2, 2, 5) X(4, 2, 2, 2, 2, 4) X(5, 2, 2, 2, 4, 3) X(6, 4, 2, 2, 4, 3) \
+    X(7, 6, 2, 2, 2, 3) X(8, 4, 6, 2, 2, 2) X(9, 6, 4, 2, 2, 2) X(10, 4, 4, 2, 4, 3) X(11, 4, 4, 4, 2, 3) X(12, 8, 4, 2, 4, 2)
+constexpr int kGemm8Kernels = 13;
+
+int gemm8_stream(const Gemm8Args& a);                          // tw4_gemm8.hip
+int gemm8_lds(const Gemm8Args& a, int kernel, int splits);     // tw4_gemm8_lds.hip
 
 }  // namespace tw4

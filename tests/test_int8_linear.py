@@ -8,6 +8,9 @@ of its own, addition, division and product by 3: (3 + 3 + 2 + 3 + 5 |g|) of 2^-2
 from __future__ import annotations
 
 import ctypes
+import json
+import math
+import os
 
 import pytest
 import torch
@@ -24,22 +27,62 @@ INT8 = QuantConfig("compressed-tensors", 8, 0)
 # ------------------------------------------------------------------------------------------- CPU
 def test_argument_errors_return_before_launch():
     lib, p, odd = w4_hip.library(), ctypes.c_void_p(4096), ctypes.c_void_p(4104)
-    #       x stride xs w stride ws y M N K act bf16
-    good = [p, 64, p, p, 64, p, p, 3, 5, 64, 0, 0]
+    #       x stride xs w stride ws y ws words locks counters M N K act bf16 kernel splits
+    good = [p, 64, p, p, 64, p, p, None, 0, None, 0, 3, 5, 64, 0, 0, 3, 1]
     for at, value, needle in ((0, None, "null"), (2, None, "null"), (3, None, "null"), (5, None, "null"), (6, None, "null"),
                               (0, odd, "aligned"), (3, odd, "aligned"), (2, ctypes.c_void_p(4098), "aligned"),
                               (6, ctypes.c_void_p(4097), "aligned"), (1, 48, "apart"), (1, 72, "apart"), (4, 48, "apart"), (4, 1 << 22, "apart"),
-                              (7, -1, "M"), (7, (1 << 20) + 1, "M"), (8, 0, "N"), (8, (1 << 24) + 1, "N"), (9, 72, "K"), (9, 0, "K"),
-                              (9, 1 << 17, "K"), (10, 2, "act"), (10, 1, "even")):
+                              (11, -1, "M"), (11, (1 << 20) + 1, "M"), (12, 0, "N"), (12, (1 << 24) + 1, "N"), (13, 72, "K"), (13, 0, "K"),
+                              (13, 1 << 17, "K"), (14, 2, "act"), (14, 1, "even"), (16, -1, "kernel"), (16, 13, "kernel"), (17, 0, "splits"),
+                              (17, 2, "splits")):
         args = list(good)
         args[at] = value
-        assert lib.tw4_gemm_int8(*args, None) == w4_hip.TW4_EINVAL, (at, value)
+        assert lib.tw4_gemm_int8(*args, None) == (w4_hip.TW4_ECONFIG if at >= 16 else w4_hip.TW4_EINVAL), (at, value)
         assert needle in lib.tw4_last_error().decode(), (at, value, lib.tw4_last_error())
-    good[7] = 0
+    good[11] = 0
     assert lib.tw4_gemm_int8(*good, None) == w4_hip.TW4_OK
+    # splits that take a workspace: none, too few words, too few counters; kernels that do not take the call
+    for change, status, needle in (({13: 256, 1: 256, 4: 256, 17: 2}, w4_hip.TW4_EINVAL, "workspace"),
+                                   ({13: 256, 1: 256, 4: 256, 17: 2, 7: p, 8: 2 * 32 * 64 - 1, 9: p, 10: 1}, w4_hip.TW4_ESPACE, "partial sums"),
+                                   ({13: 256, 1: 256, 4: 256, 17: 2, 7: p, 8: 2 * 32 * 64, 9: p, 10: 0}, w4_hip.TW4_ESPACE, "counters"),
+                                   ({12: 6, 14: 1, 16: 0}, w4_hip.TW4_ECONFIG, "SwiGLU"), ({11: 17, 16: 1}, w4_hip.TW4_ECONFIG, "16 tokens"),
+                                   ({11: 17, 16: 2}, w4_hip.TW4_ECONFIG, "16 tokens")):
+        args = list(good)
+        args[11] = 3
+        for at, value in change.items():
+            args[at] = value
+        assert lib.tw4_gemm_int8(*args, None) == status, change
+        assert needle in lib.tw4_last_error().decode(), (change, lib.tw4_last_error())
 
 
-def test_refusals_on_the_cpu():
+def _plan(m, n, k, act, cus=256):
+    out = (ctypes.c_int * 4)()
+    w4_hip.check(w4_hip.library().tw4_gemm_int8_plan(m, n, k, act, cus, out))
+    return tuple(out)
+
+
+def test_plan():
+    """Every size has a kernel that takes it, within the workspace; and the choice on the sizes it was fitted to."""
+    for m in (1, 16, 17, 33, 200, 201, 1100, 5000, 1 << 20):
+        for n, k in ((1, 16), (2, 131056), (6144, 4096), (1 << 24, 16), (34816, 5120)):
+            for act in (0, 1) if n % 2 == 0 else (0,):
+                for cus in (1, 64, 256):
+                    kernel, splits, words, counters = _plan(m, n, k, act, cus)
+                    assert 0 <= kernel < 13 and 1 <= splits <= max(1, k // 128) and not (kernel == 0 and act) and not (kernel in (1, 2) and m > 16)
+                    assert words <= w4_hip.WORKSPACE_FLOATS and counters <= w4_hip.WORKSPACE_LOCKS and (splits > 1) == (words > 0)
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "profiles", "gemm_int8_rule_sweep.jsonl")
+    ratios = []
+    for line in open(path, encoding="utf-8"):
+        d = json.loads(line)
+        kernel, splits, _, _ = _plan(d["m"], d["n"], d["k"], d["act"])
+        us = d["us"][f"{kernel},{splits}"]
+        ratios.append(us / min(d["us"].values()))
+    assert len(ratios) > 500 and math.exp(sum(map(math.log, ratios)) / len(ratios)) < 1.02 and max(ratios) < 1.4
+    with pytest.raises(RuntimeError, match="plan"):
+        _plan(0, 4, 16, 0)
+
+
+def test_refusals_on_the_cpu(monkeypatch):
     x, s, w = torch.zeros(2, 64, dtype=torch.int8), torch.ones(2), torch.zeros(3, 64, dtype=torch.int8)
     with pytest.raises(RuntimeError, match="GPU"):
         w8.linear_int8(x, s, w, torch.ones(3))
@@ -51,8 +94,12 @@ def test_refusals_on_the_cpu():
         return lay(shape, (1,) * len(shape), torch.float32)
 
     x, w = lay((2, 64), (64, 1)), lay((6, 64), (64, 1))
-    assert w8._checked(x, f32(2), w, f32(6, 1), True, torch.float16) == (64, 64, (2, 6, 64), 3, 0, 0)
-    assert w8._checked(lay((1, 64), (7, 1)), f32(1), w, f32(6), False, torch.bfloat16) == (64, 64, (1, 6, 64), 6, 1, 0)
+    w8._checked.cache_clear()
+    monkeypatch.setattr(w8, "_cus", lambda index: 256)
+    got = w8._checked(x, f32(2), w, f32(6, 1), True, torch.float16)
+    assert got[:2] == (64, 64) and got[2][:5] == (2, 6, 64, 1, 0) and got[3:] == (3, 0) and got[2][5:] == _plan(2, 6, 64, 1)[:2]
+    got = w8._checked(lay((1, 64), (7, 1)), f32(1), w, f32(6), False, torch.bfloat16)
+    assert got[:2] == (64, 64) and got[2][:5] == (1, 6, 64, 0, 1) and got[3:] == (6, 0)
     for bad in ((x, f32(3), w, f32(6), False, torch.float16), (x, f32(2), w, f32(5), False, torch.float16),
                 (lay((2, 48), (64, 1)), f32(2), w, f32(6), False, torch.float16), (x, f32(2), w, f32(6), False, torch.float32),
                 (x, f32(2), lay((5, 64), (64, 1)), f32(5), True, torch.float16), (lay((2, 64), (72, 1)), f32(2), w, f32(6), False, torch.float16),
@@ -62,6 +109,7 @@ def test_refusals_on_the_cpu():
                 (lay((2, 64), (0, 1)), f32(2), w, f32(6), False, torch.float16), (lay((2, 64), (1 << 22, 1)), f32(2), w, f32(6), False, torch.float16)):
         with pytest.raises(RuntimeError, match="^linear_int8: "):
             w8._checked(*bad)
+    w8._checked.cache_clear()
 
 
 def test_layer_without_a_gpu():
@@ -122,6 +170,36 @@ def test_linear(m, n, k, dtype, silu_mul):
     _check(y, x, xs, w, ws, silu_mul, dtype)
     assert all(torch.equal(a, b) for a, b in zip(kept, (x, xs, w, ws)))
     assert torch.equal(y, w8.linear_int8(x, xs[:, None], w, ws[:, None], silu_mul=silu_mul, dtype=dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kernel", range(13))
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_every_kernel(kernel, dtype):
+    """Each kernel with each number of splits, tiles that are full and tiles that are not, outputs of any alignment: all the same
+    bits, nothing behind the output, counters back at zero."""
+    lib = w4_hip.library()
+    for m, n, k, act in ((1, 18, 16, 0), (5, 130, 144, 1), (16, 64, 2048, 0), (16, 515, 1040, 0), (17, 256, 400, 1), (150, 200, 640, 0), (193, 1030, 272, 1),
+                         (257, 385, 1296, 0), (260, 520, 1296, 1)):
+        if (kernel == 0 and act) or (kernel in (1, 2) and m > 16):
+            continue
+        x, xs, w, ws = _operands(m, n, k, seed=kernel + m)
+        out = n // 2 if act else n
+        want = None
+        for splits in sorted({s for s in (1, 2, 3, 5, 11) if s <= -(-k // 128) and (kernel or s == 1)}):
+            part, locks = w4_hip.stream_workspace(x.device)
+            for shift in (0, 1, 4):
+                buf = torch.full((m * out + 64,), 7.0, dtype=dtype, device="cuda")
+                y = buf[shift:shift + m * out].view(m, out)
+                w4_hip.check(lib.tw4_gemm_int8(x.data_ptr(), k, xs.data_ptr(), w.data_ptr(), k, ws.data_ptr(), y.data_ptr(), part.data_ptr(), part.numel(),
+                                               locks.data_ptr(), locks.numel(), m, n, k, act, int(dtype == torch.bfloat16), kernel, splits,
+                                               w4_hip.raw_stream(0)))
+                assert bool((buf[:shift] == 7).all()) and bool((buf[shift + m * out:] == 7).all())
+                if want is None:
+                    want = y.clone()
+                    _check(want, x, xs, w, ws, bool(act), dtype)
+                assert torch.equal(y, want), (m, n, k, act, splits, shift)
+                assert not bool(locks.any())
 
 
 @pytest.mark.gpu
