@@ -93,8 +93,9 @@ def _rows(m, k, dtype, seed, outliers=True):
     return x.to(dtype)
 
 
-WIDTHS = [16, 32, 48, 496, 512, 528, 1024, 2048, 2064, 2560, 4096, 4112, 5120, 8192, 8208, 12288, 16384, 16400, 28672, 32768]
-ROWS = [1, 2, 3, 5, 8, 63, 64, 65, 333, 1000]
+WIDTHS = [16, 32, 48, 496, 512, 528, 1024, 1040, 2048, 2064, 2560, 4096, 4112, 5120, 6160, 8192, 8208, 12288, 12304, 16384, 16400, 24576, 24592,
+          28672, 30720, 30736, 32768]
+ROWS = [1, 2, 3, 5, 8, 63, 64, 65, 255, 256, 333, 1023, 1024]
 
 
 @pytest.mark.gpu
