@@ -1,9 +1,9 @@
 // y[M, N] = x_scale[m] w_scale[n] sum_k x[m, k] w[n, k] of 8-bit integers, the sum exact in 32 bits, one rounding; or, with
 // act, y[M, N / 2] = silu(g) u of the rows w = [gate | up], g and u unrounded.
 //
-// The kernel for few tokens streams w through registers. A workgroup of 16 wavefronts takes 16 rows of w and 16 tokens. Units of 128 k
-// go to the wavefronts in turn, so that the workgroup reads each row in pieces of 2 KB; each wavefront has one unit in flight ahead of
-// the math. The wavefronts' sums are added in LDS.
+// The kernel for few tokens streams w through registers. A workgroup of 16 wavefronts takes `rows` rows of w, up to NT tiles of 16,
+// and 16 tokens; as many rows as give every CU the same work. Units of 128 k go to the wavefronts in turn, so that the workgroup reads
+// each row in pieces of 2 KB; each wavefront has one unit in flight ahead of the math. The wavefronts' sums are added in LDS.
 #include <math.h>
 
 #include "tw4_int8.h"
@@ -12,41 +12,51 @@ namespace tw4 {
 
 constexpr int kStreamWaves = 16;
 
+template <int NT>
 struct Stream8Regs {
-    u4 a[2], b[2];
+    u4 a[NT][2], b[2];
 };
 
-template <bool BF16>
+template <int NT, bool BF16>
 __global__ void __launch_bounds__(64 * kStreamWaves) gemm8_stream_kernel(const int8_t* __restrict__ x, uint32_t x_stride,
                                                                          const float* __restrict__ x_scale, const int8_t* __restrict__ w,
                                                                          uint32_t w_stride, const float* __restrict__ w_scale,
-                                                                         uint16_t* __restrict__ y, int M, int N, int K) {
-    __shared__ i4 part[kStreamWaves][64];
+                                                                         uint16_t* __restrict__ y, int M, int N, int K, int rows_each) {
+    __shared__ i4 part[kStreamWaves][NT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, q = lane >> 4;
-    const int n0 = 16 * blockIdx.x, m0 = 16 * blockIdx.y;
-    // rows past the end: the last one, not stored; k past the end: past the resources' records, zeros
-    const int rows = min(N - n0, 16), tokens = min(M - m0, 16);
+    const int n0 = rows_each * blockIdx.x, m0 = 16 * blockIdx.y;
+    // what lies past the rows, the tokens or K is past the resources' records: zeros, nothing read
+    const int rows = min(N - n0, rows_each), tokens = min(M - m0, 16);
     const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(w + static_cast<int64_t>(n0) * w_stride), 0,
                                                                         (rows - 1) * w_stride + K, kBufferFlags);
     const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(x + static_cast<int64_t>(m0) * x_stride), 0,
                                                                         (tokens - 1) * x_stride + K, kBufferFlags);
-    const uint32_t wo = static_cast<uint32_t>(min(r, rows - 1)) * w_stride + 16 * q, xo = static_cast<uint32_t>(min(r, tokens - 1)) * x_stride + 16 * q;
+    uint32_t wo[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) wo[t] = 16 * t + r < rows ? static_cast<uint32_t>(16 * t + r) * w_stride + 16 * q : 0x80000000u;
+    const uint32_t xo = r < tokens ? static_cast<uint32_t>(r) * x_stride + 16 * q : 0x80000000u;
     const int units = (K + 127) >> 7, steps = (units - wave + kStreamWaves - 1) / kStreamWaves;  // of this wavefront's units
-    const auto load = [&](Stream8Regs& v, int s) {
+    const auto load = [&](Stream8Regs<NT>& v, int s) {
         const int k = 128 * (s * kStreamWaves + wave);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const uint32_t past = k + 64 * h + 16 * q < K ? 0u : 0x80000000u;
-            v.a[h] = bitcast<u4>(__builtin_amdgcn_raw_buffer_load_b128(wr, (wo | past) + 64 * h, k, 2));  // non-temporal: read once
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+                v.a[t][h] = bitcast<u4>(__builtin_amdgcn_raw_buffer_load_b128(wr, (wo[t] | past) + 64 * h, k, 2));  // non-temporal: read once
             v.b[h] = bitcast<u4>(__builtin_amdgcn_raw_buffer_load_b128(xr, (xo | past) + 64 * h, k, 0));
         }
     };
-    i4 acc{0, 0, 0, 0};
-    const auto multiply = [&](const Stream8Regs& v) {
+    i4 acc[NT];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) acc = mfma_i8(v.a[h], v.b[h], acc);
+    for (int t = 0; t < NT; ++t) acc[t] = i4{0, 0, 0, 0};
+    const auto multiply = [&](const Stream8Regs<NT>& v) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) acc[t] = mfma_i8(v.a[t][h], v.b[h], acc[t]);
     };
-    Stream8Regs v0, v1;
+    Stream8Regs<NT> v0, v1;
     if (steps > 0) load(v0, 0);
     for (int s = 0; s < steps; s += 2) {
         if (s + 1 < steps) load(v1, s + 1);
@@ -57,29 +67,40 @@ __global__ void __launch_bounds__(64 * kStreamWaves) gemm8_stream_kernel(const i
         __builtin_amdgcn_sched_barrier(0);
         multiply(v1);
     }
-    part[wave][lane] = acc;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) part[wave][t][lane] = acc[t];
     __syncthreads();
-    if (wave != 0) return;
-    const int m = m0 + r, n = n0 + 4 * q;
+    if (wave >= NT) return;  // wavefront t adds tile t
+    const int m = m0 + r, at = 16 * wave + 4 * q, n = n0 + at;
     const float xs = x_scale[min(m, M - 1)];
     float s[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) s[i] = w_scale[min(n + i, N - 1)];
+    i4 sum{0, 0, 0, 0};
 #pragma unroll
-    for (int v = 1; v < kStreamWaves; ++v) acc += part[v][lane];
+    for (int v = 0; v < kStreamWaves; ++v) sum += part[v][wave][lane];
     if (m >= M) return;
-    float o[4];
+    uint16_t* row = y + static_cast<int64_t>(m) * N + n;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = static_cast<float>(acc[i]) * xs * s[i];
-    store_features<BF16>(y + static_cast<int64_t>(m) * N, n, N, (N & 3) == 0 && (reinterpret_cast<uintptr_t>(y) & 7) == 0, o);
+    for (int i = 0; i < 4; ++i)
+        if (at + i < rows) row[i] = static_cast<uint16_t>(value16<BF16>(static_cast<float>(sum[i]) * xs * s[i]));
 }
 
-int gemm8_stream(const Gemm8Args& a) {
+// Rows of w per workgroup of the streaming kernel: what gives every CU one workgroup, where that is 4 to 32 rows, else 16. M = 1, us, with
+// 16 rows each: K 4096 x N 6144 7.4 (8.2), K 9728 x N 2560 7.9 (9.9), K 8192 x N 512 6.1 (7.7), K 2064 x N 5001 5.3 (6.0).
+static int stream8_rows(int N, int cus) {
+    const int each = (N + cus - 1) / cus;
+    return each > 32 ? 16 : each < 4 ? 4 : each;
+}
+
+int gemm8_stream(const Gemm8Args& a, int rows) {
     TW4_REQUIRE(!a.act, TW4_ECONFIG, "gemm_int8: no SwiGLU in the streaming kernel");
-    const dim3 grid(static_cast<unsigned>((a.N + 15) / 16), static_cast<unsigned>((a.M + 15) / 16));
-    const auto kernel = a.bf16 ? gemm8_stream_kernel<true> : gemm8_stream_kernel<false>;
+    const dim3 grid(static_cast<unsigned>((a.N + rows - 1) / rows), static_cast<unsigned>((a.M + 15) / 16));
+    TW4_REQUIRE(grid.y < 1 << 16, TW4_ECONFIG, "gemm_int8: M < 2^20 for the streaming kernel (M %d)", a.M);
+    const auto kernel = rows <= 16 ? (a.bf16 ? gemm8_stream_kernel<1, true> : gemm8_stream_kernel<1, false>)
+                                   : (a.bf16 ? gemm8_stream_kernel<2, true> : gemm8_stream_kernel<2, false>);
     kernel<<<grid, 64 * kStreamWaves, 0, a.st>>>(a.x, static_cast<uint32_t>(a.x_stride), a.x_scale, a.w, static_cast<uint32_t>(a.w_stride),
-                                                 a.w_scale, a.y, a.M, a.N, a.K);
+                                                 a.w_scale, a.y, a.M, a.N, a.K, rows);
     TW4_LAUNCH_CHECK("gemm_int8: launch");
     return TW4_OK;
 }
@@ -93,7 +114,7 @@ int gemm8_stream(const Gemm8Args& a) {
 //   beside all this the bytes: what is read and written once at a rate of its own.
 // Coefficients in microseconds on MI355X (256 CUs), a row for one tile of tokens (w read once, not kept) and one for more, from least
 // squares on relative errors over 520 sizes (20 K x N, M = 1 .. 8192, w streamed from HBM) x up to 60 kernels and splits each
-// (profiles/gemm_int8_rule_sweep.jsonl). The choice is 1.2 % slower than the fastest that was timed on average, 31 % at
+// (profiles/gemm_int8_rule_sweep.jsonl). The choice is 0.9 % slower than the fastest that was timed on average, 27 % at
 // most.
 struct Gemm8Cost {
     double start, round, stage, share, split, part, rate, step, cu;
@@ -103,39 +124,39 @@ struct Gemm8Row {
     Gemm8Cost one, more;
 };
 constexpr Gemm8Row kGemm8Rows[kGemm8Kernels] = {
-    {16, 16, 2, 1, 48, {1.432, 0.03182, 1.396, 0.4754, 1, 0.2, 3.759, 0.3, 0.3415},
-     {1.432, 0.03182, 1.396, 0.4754, 1, 0.2, 3.759, 0.3, 0.3415}},
-    {16, 64, 2, 1, 16, {1.043, 2.466, 0.1504, 1.253, 0.606, 0.828, 5.535, 0.3353, 0.3957},
-     {1.043, 2.466, 0.1504, 1.253, 0.606, 0.828, 5.535, 0.3353, 0.3957}},
-    {16, 64, 5, 1, 16, {1.753, 1.157, 0.3101, 0.2732, 0.6548, 0.8535, 5.033, 0.3633, 0.03282},
-     {1.753, 1.157, 0.3101, 0.2732, 0.6548, 0.8535, 5.033, 0.3633, 0.03282}},
-    {32, 64, 2, 1, 200, {1.374, 2.106, 0.178, 1.243, 0.7155, 0.4386, 5.725, 0.3136, 0.2173},
-     {1.465, 1.774, 0.1462, 0.8874, 0.8115, 0.3415, 3.743, 0.3517, 0.3565}},
-    {64, 64, 2, 17, 1100, {1.316, 2.308, 0.2421, 1.137, 0.7823, 0.2945, 5.818, 0.3858, 0.1972},
-     {1.425, 2.263, 0.153, 0.9155, 0.7636, 0.2411, 3.299, 0.394, 0.6335}},
-    {64, 128, 2, 17, 1600, {1.698, 1.962, 0.4409, 1.302, 0.7004, 0.288, 4.981, 0.4271, 0.06092},
-     {1.631, 2.242, 0.2836, 0.766, 0.4939, 0.263, 3.182, 0.3965, 0.4844}},
-    {128, 128, 1, 48, 2048, {0.5382, 4.068, 0.4841, 0.5, 0.7206, 0.1981, 4.563, 0.6378, 0.3615},
-     {1.192, 3.459, 0.3894, 0.5, 0.6309, 0.2254, 3.111, 0.5572, 0.414}},
-    {192, 64, 1, 100, 4096, {1.106, 3.245, 0.4275, 0.5, 0.843, 0.2283, 3.84, 0.7679, 0.3268},
-     {1.597, 3.72, 0.3053, 0.5, 0.8003, 0.1767, 2.906, 0.8219, 0.5293}},
-    {128, 192, 2, 65, 1 << 20, {1.757, 4.944, 0.9339, 0.7345, 0.9842, 0.1316, 4.726, 1.397, 0.2274},
-     {0.2578, 6.523, 0.7848, 0.2714, 1.554, 0.1234, 2.781, 1.293, 0.2602}},
-    {192, 128, 2, 129, 1 << 20, {2.609, 2.363, 0.9088, 0.5419, 1.25, 0.2082, 4.277, 1.31, 0.1995},
-     {0.8359, 5.816, 0.7369, 0.3387, 1.259, 0.15, 3.08, 1.241, 0.2547}},
-    {128, 256, 1, 65, 1 << 20, {2.144, 4.186, 0.7909, 0.5, 1.299, 0.1618, 5.488, 0.876, 0.4925},
-     {0.5045, 6.247, 0.6347, 0.5, 0.5077, 0.1863, 3.056, 1.051, 0.3332}},
-    {256, 128, 1, 96, 1 << 20, {1.602, 4.435, 0.6056, 0.5, 0.5437, 0.1833, 4.045, 1.124, 0.5252},
-     {1.175, 6.368, 0.4713, 0.5, 0.3402, 0.1605, 4.646, 1.083, 0.7362}},
-    {256, 256, 1, 160, 1 << 20, {2.665, 4.276, 1.438, 0.5, 2.693, 0.1677, 4.321, 3.593, 0.4025},
-     {0.5145, 9.145, 1.201, 0.5, 1.468, 0.1513, 3.119, 3.448, 0.2847}},
+    {16, 16, 2, 1, 48, {1.923, 0.03967, 0.9524, 0.6954, 1, 0.2, 3.844, 0.3, 0.4964},
+     {1.923, 0.03967, 0.9524, 0.6954, 1, 0.2, 3.844, 0.3, 0.4964}},
+    {16, 64, 2, 1, 16, {0.9438, 2.471, 0.1525, 1.247, 0.6929, 0.8009, 5.48, 0.343, 0.3957},
+     {0.9438, 2.471, 0.1525, 1.247, 0.6929, 0.8009, 5.48, 0.343, 0.3957}},
+    {16, 64, 5, 1, 16, {1.91, 0.7856, 0.315, 0.2706, 0.7488, 0.8844, 5.065, 0.3724, 0.0323},
+     {1.91, 0.7856, 0.315, 0.2706, 0.7488, 0.8844, 5.065, 0.3724, 0.0323}},
+    {32, 64, 2, 1, 200, {1.383, 1.998, 0.1806, 1.215, 0.7839, 0.4486, 5.724, 0.3276, 0.22},
+     {1.433, 1.758, 0.1464, 0.889, 0.8775, 0.3399, 3.759, 0.3614, 0.3588}},
+    {64, 64, 2, 17, 1100, {1.359, 2.185, 0.2413, 1.118, 0.8995, 0.2992, 5.873, 0.3927, 0.2173},
+     {1.436, 2.141, 0.1547, 0.9047, 0.8219, 0.2479, 3.299, 0.4126, 0.628}},
+    {64, 128, 2, 17, 1600, {1.829, 1.624, 0.4425, 1.293, 0.9017, 0.2933, 5.003, 0.4268, 0.06747},
+     {1.619, 1.944, 0.2851, 0.7456, 0.6628, 0.265, 3.152, 0.4203, 0.5004}},
+    {128, 128, 1, 48, 2048, {0.7097, 3.826, 0.4999, 0.5, 0.9821, 0.1839, 4.606, 0.6007, 0.2654},
+     {1.237, 3.283, 0.3967, 0.5, 0.7107, 0.2046, 3.22, 0.5711, 0.3912}},
+    {192, 64, 1, 100, 4096, {1.082, 3.236, 0.425, 0.5, 0.9128, 0.2265, 3.92, 0.7776, 0.333},
+     {1.463, 3.563, 0.314, 0.5, 0.6986, 0.1831, 2.826, 0.87, 0.4798}},
+    {128, 192, 2, 65, 1 << 20, {1.728, 5.211, 0.9317, 0.7278, 0.9274, 0.1301, 4.614, 1.419, 0.2164},
+     {0.2758, 6.246, 0.7895, 0.2625, 1.447, 0.1268, 2.763, 1.373, 0.2609}},
+    {192, 128, 2, 129, 1 << 20, {2.827, 2.28, 0.9054, 0.5603, 1.304, 0.2044, 4.273, 1.321, 0.1978},
+     {0.8714, 5.576, 0.7378, 0.3379, 0.9419, 0.1609, 3.116, 1.322, 0.2601}},
+    {128, 256, 1, 65, 1 << 20, {2.206, 4.075, 0.7777, 0.5, 1.661, 0.116, 8.225, 0.9003, 0.6474},
+     {0.5667, 5.809, 0.652, 0.5, 0.9784, 0.1613, 3.133, 1.021, 0.304}},
+    {256, 128, 1, 96, 1 << 20, {1.781, 4.141, 0.6212, 0.5, 1.04, 0.1552, 4.122, 1.065, 0.4548},
+     {1.097, 6.024, 0.4873, 0.5, 0.415, 0.1522, 5.312, 1.086, 0.6831}},
+    {256, 256, 1, 160, 1 << 20, {2.813, 4.153, 1.452, 0.5, 2.865, 0.1676, 4.844, 3.68, 0.3836},
+     {0.4742, 8.871, 1.219, 0.5, 1.493, 0.1593, 3.09, 3.594, 0.2595}},
 };
 
 static double gemm8_cost(int kernel, int M, int out, int N, int K, int act, int splits, int cus) {
     const Gemm8Row& t = kGemm8Rows[kernel];
     const int64_t mb = (M + t.bm - 1) / t.bm;
     const Gemm8Cost& c = mb > 1 ? t.more : t.one;
-    const int features = act ? t.bn / 2 : t.bn;
+    const int features = kernel == 0 ? stream8_rows(N, cus) : act ? t.bn / 2 : t.bn;
     const double units = static_cast<double>(mb * ((out + features - 1) / features)) * splits;
     const int all = (K + 127) / 128, ways = kernel ? splits : kStreamWaves, stages = (all + ways - 1) / ways;
     const double n = ceil(units / cus), full = floor(n / t.occ), rest = n - full * t.occ;
@@ -163,7 +184,7 @@ static void gemm8_plan(int M, int N, int K, int act, int cus, int* out) {
             const double us = gemm8_cost(k, M, features, N, K, act, s, cus);
             if (us >= best) continue;
             best = us;
-            out[0] = k, out[1] = s, out[2] = s > 1 ? static_cast<int>(words) : 0, out[3] = s > 1 ? static_cast<int>(tiles) : 0;
+            out[0] = k, out[1] = k ? s : stream8_rows(N, cus), out[2] = s > 1 ? static_cast<int>(words) : 0, out[3] = s > 1 ? static_cast<int>(tiles) : 0;
         }
     }
 }
@@ -203,10 +224,10 @@ extern "C" int tw4_gemm_int8(const int8_t* x, int64_t x_stride, const float* x_s
                 TW4_EINVAL, "gemm_int8: rows at least K and less than 2^22 apart, 16-byte aligned (strides %lld, %lld)",
                 static_cast<long long>(x_stride), static_cast<long long>(w_stride));
     TW4_REQUIRE(kernel >= 0 && kernel < kGemm8Kernels, TW4_ECONFIG, "gemm_int8: kernel %d", kernel);
-    TW4_REQUIRE(splits >= 1 && splits <= (K + 127) / 128 && (kernel || splits == 1), TW4_ECONFIG,
-                "gemm_int8: 1 .. K / 128 splits, 1 for kernel 0 (kernel %d, splits %d, K %d)", kernel, splits, K);
+    TW4_REQUIRE(splits >= 1 && splits <= (kernel ? (K + 127) / 128 : 32), TW4_ECONFIG,
+                "gemm_int8: 1 .. K / 128 splits, 1 .. 32 rows of kernel 0 (kernel %d, splits %d, K %d)", kernel, splits, K);
     if (M == 0) return TW4_OK;
     const Gemm8Args a{x, x_stride, x_scale, w, w_stride, w_scale, y, M, N, K, act, bf16, ws, locks, ws_words, n_locks,
                       static_cast<hipStream_t>(stream)};
-    return kernel ? gemm8_lds(a, kernel, splits) : gemm8_stream(a);
+    return kernel ? gemm8_lds(a, kernel, splits) : gemm8_stream(a, splits);
 }

@@ -23,6 +23,19 @@ __device__ __forceinline__ void wave_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// ROWS x COLUMNS 16-bit values in LDS (rows PITCH bytes apart) to global rows `out` values apart, V values (a T) a lane and store; only
+// the first `rows` and `columns` (a multiple of V, or none).
+template <int V, int ROWS, int COLUMNS, int PITCH, class T>
+__device__ __forceinline__ void store_rows(uint16_t* __restrict__ to, int out, const char* from, int rows, int columns, int lane) {
+    constexpr int PER_ROW = COLUMNS / V, ALL = ROWS * PER_ROW;
+#pragma unroll 8
+    for (int i = 0; i < (ALL + 63) / 64; ++i) {
+        const int at = 64 * i + lane, row = at / PER_ROW, c = V * (at % PER_ROW);
+        if ((ALL % 64 == 0 || at < ALL) && row < rows && c < columns)
+            *reinterpret_cast<T*>(to + static_cast<int64_t>(row) * out + c) = *reinterpret_cast<const T*>(from + row * PITCH + 2 * c);
+    }
+}
+
 #define TW4_STEP_FENCE __builtin_amdgcn_sched_barrier(0)
 
 template <int TM_, int TN_, int WM_, int WN_, int R_, bool NT_ = false>
@@ -246,7 +259,7 @@ gemm8_lds_kernel(const int8_t* __restrict__ x, uint32_t x_stride, const float* _
     // results.
     constexpr int TILES = ACT ? TN / 2 : TN;
     constexpr int PART = C::LDS_BYTES / C::WAVES / 16 * 16, SCALES = 64 * (TM + TN);  // bytes
-    constexpr int ROW = 32 * TILES + 16, CHUNKS = 2 * TILES;  // a token's results, 16 bytes behind them against bank conflicts; 16-byte chunks
+    constexpr int ROW = 32 * TILES + 16;  // a token's results, 16 bytes behind them against bank conflicts
     constexpr int FIT = (PART - SCALES) / (16 * ROW);
     constexpr int TB = FIT >= TM ? TM : FIT >= TM / 2 && TM % 2 == 0 ? TM / 2 : 1;
     static_assert(FIT >= 1 && TM % TB == 0, "one token tile at least");
@@ -291,44 +304,33 @@ gemm8_lds_kernel(const int8_t* __restrict__ x, uint32_t x_stride, const float* _
             for (int i = 0; i < 4; ++i) v[i] = silu(v[i]) * (static_cast<float>(acc[t + TILES][b][i]) * xs * u[i]);
         }
     };
-    if ((out & 7) == 0 && (reinterpret_cast<uintptr_t>(y) & 15) == 0) {
-        // through LDS, so that a store instruction writes whole rows of the wavefront's features
+    // Results go through LDS, so that a store instruction writes whole rows of the wavefront's features: 8 values a lane where rows are
+    // that aligned, else 2 or 1.
+    const int width = (out & 7) == 0 && (reinterpret_cast<uintptr_t>(y) & 15) == 0  ? 8
+                      : (out & 1) == 0 && (reinterpret_cast<uintptr_t>(y) & 3) == 0 ? 2
+                                                                                     : 1;
 #pragma unroll
-        for (int b0 = 0; b0 < TM; b0 += TB) {
+    for (int b0 = 0; b0 < TM; b0 += TB) {
 #pragma unroll
-            for (int b = b0; b < b0 + TB; ++b)
+        for (int b = b0; b < b0 + TB; ++b)
 #pragma unroll
-                for (int t = 0; t < TILES; ++t) {
-                    TW4_STEP_FENCE;  // one tile's values at a time: all of them at once do not fit the registers
-                    float v[4];
-                    values(t, b, v);
-                    *reinterpret_cast<u2*>(mine + (16 * (b - b0) + r) * ROW + 32 * t + 8 * q) =
-                        u2{value16<BF16>(v[0]) | value16<BF16>(v[1]) << 16, value16<BF16>(v[2]) | value16<BF16>(v[3]) << 16};
-                }
-            wave_fence();
-#pragma unroll
-            for (int i = 0; i < (16 * TB * CHUNKS + 63) / 64; ++i) {
-                const int at = 64 * i + lane, row = at / CHUNKS, c = at % CHUNKS;
-                const int m = m0 + 16 * (TM * wm + b0) + row, n = n0 + 16 * TILES * wn + 8 * c;
-                if ((16 * TB * CHUNKS % 64 == 0 || at < 16 * TB * CHUNKS) && m < M && n < out)
-                    *reinterpret_cast<u4*>(y + static_cast<int64_t>(m) * out + n) = *reinterpret_cast<const u4*>(mine + row * ROW + 16 * c);
+            for (int t = 0; t < TILES; ++t) {
+                TW4_STEP_FENCE;  // one tile's values at a time: all of them at once do not fit the registers
+                float v[4];
+                values(t, b, v);
+                *reinterpret_cast<u2*>(mine + (16 * (b - b0) + r) * ROW + 32 * t + 8 * q) =
+                    u2{value16<BF16>(v[0]) | value16<BF16>(v[1]) << 16, value16<BF16>(v[2]) | value16<BF16>(v[3]) << 16};
             }
-            wave_fence();
-        }
-        return;
-    }
-#pragma unroll
-    for (int t = 0; t < TILES; ++t) {
-        const int n = n0 + 16 * (TILES * wn + t) + 4 * q;
-#pragma unroll
-        for (int b = 0; b < TM; ++b) {
-            const int m = m0 + 16 * (TM * wm + b) + r;
-            if (m >= M) continue;
-            TW4_STEP_FENCE;
-            float o[4];
-            values(t, b, o);
-            store_features<BF16>(y + static_cast<int64_t>(m) * out, n, out, false, o);
-        }
+        wave_fence();
+        uint16_t* to = y + static_cast<int64_t>(m0 + 16 * (TM * wm + b0)) * out + n0 + 16 * TILES * wn;
+        const int rows = min(M - m0 - 16 * (TM * wm + b0), 16 * TB), columns = min(out - n0 - 16 * TILES * wn, 16 * TILES);
+        if (width == 8)
+            store_rows<8, 16 * TB, 16 * TILES, ROW, u4>(to, out, mine, rows, columns, lane);
+        else if (width == 2)
+            store_rows<2, 16 * TB, 16 * TILES, ROW, uint32_t>(to, out, mine, rows, columns, lane);
+        else
+            store_rows<1, 16 * TB, 16 * TILES, ROW, uint16_t>(to, out, mine, rows, columns, lane);
+        wave_fence();
     }
 }
 

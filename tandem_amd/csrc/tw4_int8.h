@@ -82,7 +82,7 @@ struct Gemm8Args {
     X(7, 6, 2, 2, 2, 3) X(8, 4, 6, 2, 2, 2) X(9, 6, 4, 2, 2, 2) X(10, 4, 4, 2, 4, 3) X(11, 4, 4, 4, 2, 3) X(12, 8, 4, 2, 4, 2)
 constexpr int kGemm8Kernels = 13;
 
-int gemm8_stream(const Gemm8Args& a);                          // tw4_gemm8.hip
-int gemm8_lds(const Gemm8Args& a, int kernel, int splits);     // tw4_gemm8_lds.hip
+int gemm8_stream(const Gemm8Args& a, int rows);             // tw4_gemm8.hip
+int gemm8_lds(const Gemm8Args& a, int kernel, int splits);  // tw4_gemm8_lds.hip
 
 }  // namespace tw4

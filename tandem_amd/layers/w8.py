@@ -49,7 +49,8 @@ def _cus(index: int) -> int:
 # As norm.check_rows: what depends on layouts alone, once for each combination of them.
 @functools.lru_cache(maxsize=1 << 14)
 def _checked(x: tuple, x_scale: tuple, weight: tuple, weight_scale: tuple, silu_mul: bool, dtype: torch.dtype) -> tuple:
-    """(row strides of x and of the weight, (M, N, K, act, type code, kernel, splits), output features, GPU)."""
+    """(row strides of x and of the weight, (M, N, K, act, type code, kernel, splits), whether those take a workspace,
+    output features, GPU)."""
     index = x[3]
     steps = []
     for name, t in (("x", x), ("weight", weight)):
@@ -72,7 +73,7 @@ def _checked(x: tuple, x_scale: tuple, weight: tuple, weight_scale: tuple, silu_
     plan = (ctypes.c_int * 4)(0, 1)
     if m:
         w4_hip.check(w4_hip.library().tw4_gemm_int8_plan(m, n, k, int(silu_mul), _cus(index), plan))
-    return *steps, (m, n, k, int(silu_mul), TYPES[dtype], plan[0], plan[1]), n // 2 if silu_mul else n, index
+    return *steps, (m, n, k, int(silu_mul), TYPES[dtype], plan[0], plan[1]), plan[2] > 0, n // 2 if silu_mul else n, index
 
 
 def linear_int8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, *,
@@ -81,8 +82,8 @@ def linear_int8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, we
     ``dtype``: y[m, n] = x_scale[m] * weight_scale[n] * sum_k x[m, k] weight[n, k], the sum exact, one rounding (tw4_gemm_int8).
     silu_mul: the weight's rows are [gate | up] and y [M, N / 2] = silu(gate) * up, gate and up in float32. K % 16 == 0, K < 2^17;
     any row strides of x and weight that are multiples of 16."""
-    step, w_step, sizes, features, index = _checked(layout(x), layout(x_scale), layout(weight), layout(weight_scale), bool(silu_mul),
-                                                    dtype)
+    step, w_step, sizes, split, features, index = _checked(layout(x), layout(x_scale), layout(weight), layout(weight_scale),
+                                                           bool(silu_mul), dtype)
     if not w4_hip.all_plain(x, x_scale, weight, weight_scale):
         raise RuntimeError("linear_int8: inference only, no gradient, transform or tracer can follow the operands")
     y = x.new_empty((sizes[0], features), dtype=dtype)
@@ -92,7 +93,7 @@ def linear_int8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, we
             raise RuntimeError("linear_int8: x and the weight must be 16-byte aligned")
         with w4_hip.on_device(index):
             wsp = locksp = words = counters = 0
-            if sizes[6] > 1:
+            if split:
                 ws, locks = w4_hip.stream_workspace(x.device)
                 wsp, locksp, words, counters = ws.data_ptr(), locks.data_ptr(), ws.numel(), locks.numel()
             w4_hip.check(w4_hip.library().tw4_gemm_int8(xp, step, x_scale.data_ptr(), wp, w_step, weight_scale.data_ptr(), y.data_ptr(),

@@ -68,16 +68,16 @@ def test_plan():
             for act in (0, 1) if n % 2 == 0 else (0,):
                 for cus in (1, 64, 256):
                     kernel, splits, words, counters = _plan(m, n, k, act, cus)
-                    assert 0 <= kernel < 13 and 1 <= splits <= max(1, k // 128) and not (kernel == 0 and act) and not (kernel in (1, 2) and m > 16)
-                    assert words <= w4_hip.WORKSPACE_FLOATS and counters <= w4_hip.WORKSPACE_LOCKS and (splits > 1) == (words > 0)
+                    assert 0 <= kernel < 13 and 1 <= splits <= (max(1, k // 128) if kernel else 32) and not (kernel == 0 and act) and not (kernel in (1, 2) and m > 16)
+                    assert words <= w4_hip.WORKSPACE_FLOATS and counters <= w4_hip.WORKSPACE_LOCKS and (kernel > 0 and splits > 1) == (words > 0)
     path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "profiles", "gemm_int8_rule_sweep.jsonl")
     ratios = []
     for line in open(path, encoding="utf-8"):
         d = json.loads(line)
         kernel, splits, _, _ = _plan(d["m"], d["n"], d["k"], d["act"])
-        us = d["us"][f"{kernel},{splits}"]
+        us = d["us"][f"{kernel},{splits if kernel else 1}"]
         ratios.append(us / min(d["us"].values()))
-    assert len(ratios) > 500 and math.exp(sum(map(math.log, ratios)) / len(ratios)) < 1.02 and max(ratios) < 1.4
+    assert len(ratios) > 500 and math.exp(sum(map(math.log, ratios)) / len(ratios)) < 1.015 and max(ratios) < 1.35
     with pytest.raises(RuntimeError, match="plan"):
         _plan(0, 4, 16, 0)
 
@@ -97,9 +97,9 @@ def test_refusals_on_the_cpu(monkeypatch):
     w8._checked.cache_clear()
     monkeypatch.setattr(w8, "_cus", lambda index: 256)
     got = w8._checked(x, f32(2), w, f32(6, 1), True, torch.float16)
-    assert got[:2] == (64, 64) and got[2][:5] == (2, 6, 64, 1, 0) and got[3:] == (3, 0) and got[2][5:] == _plan(2, 6, 64, 1)[:2]
+    assert got[:2] == (64, 64) and got[2][:5] == (2, 6, 64, 1, 0) and got[3:] == (False, 3, 0) and got[2][5:] == _plan(2, 6, 64, 1)[:2]
     got = w8._checked(lay((1, 64), (7, 1)), f32(1), w, f32(6), False, torch.bfloat16)
-    assert got[:2] == (64, 64) and got[2][:5] == (1, 6, 64, 0, 1) and got[3:] == (6, 0)
+    assert got[:2] == (64, 64) and got[2][:5] == (1, 6, 64, 0, 1) and got[3:] == (False, 6, 0)
     for bad in ((x, f32(3), w, f32(6), False, torch.float16), (x, f32(2), w, f32(5), False, torch.float16),
                 (lay((2, 48), (64, 1)), f32(2), w, f32(6), False, torch.float16), (x, f32(2), w, f32(6), False, torch.float32),
                 (x, f32(2), lay((5, 64), (64, 1)), f32(5), True, torch.float16), (lay((2, 64), (72, 1)), f32(2), w, f32(6), False, torch.float16),
@@ -176,7 +176,7 @@ def test_linear(m, n, k, dtype, silu_mul):
 @pytest.mark.parametrize("kernel", range(13))
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_every_kernel(kernel, dtype):
-    """Each kernel with each number of splits, tiles that are full and tiles that are not, outputs of any alignment: all the same
+    """Each kernel with several numbers of splits (the streaming one: of rows), tiles that are full and tiles that are not, outputs of any alignment: all the same
     bits, nothing behind the output, counters back at zero."""
     lib = w4_hip.library()
     for m, n, k, act in ((1, 18, 16, 0), (5, 130, 144, 1), (16, 64, 2048, 0), (16, 515, 1040, 0), (17, 256, 400, 1), (150, 200, 640, 0), (193, 1030, 272, 1),
@@ -186,7 +186,7 @@ def test_every_kernel(kernel, dtype):
         x, xs, w, ws = _operands(m, n, k, seed=kernel + m)
         out = n // 2 if act else n
         want = None
-        for splits in sorted({s for s in (1, 2, 3, 5, 11) if s <= -(-k // 128) and (kernel or s == 1)}):
+        for splits in sorted({s for s in (1, 2, 3, 5, 11) if s <= -(-k // 128)} if kernel else {1, 5, 16, 17, 32}):
             part, locks = w4_hip.stream_workspace(x.device)
             for shift in (0, 1, 4):
                 buf = torch.full((m * out + 64,), 7.0, dtype=dtype, device="cuda")
