@@ -114,7 +114,7 @@ int gemm8_stream(const Gemm8Args& a, int rows) {
 //   beside all this the bytes: what is read and written once at a rate of its own.
 // Coefficients in microseconds on MI355X (256 CUs), a row for one tile of tokens (w read once, not kept) and one for more, from least
 // squares on relative errors over 520 sizes (20 K x N, M = 1 .. 8192, w streamed from HBM) x up to 60 kernels and splits each
-// (profiles/gemm_int8_rule_sweep.jsonl). The choice is 0.9 % slower than the fastest that was timed on average, 27 % at
+// (profiles/gemm_int8_rule_sweep.jsonl). The choice is 0.9 % slower than the fastest that was timed on average, 20 % at
 // most.
 struct Gemm8Cost {
     double start, round, stage, share, split, part, rate, step, cu;
@@ -124,32 +124,32 @@ struct Gemm8Row {
     Gemm8Cost one, more;
 };
 constexpr Gemm8Row kGemm8Rows[kGemm8Kernels] = {
-    {16, 16, 2, 1, 48, {1.923, 0.03967, 0.9524, 0.6954, 1, 0.2, 3.844, 0.3, 0.4964},
-     {1.923, 0.03967, 0.9524, 0.6954, 1, 0.2, 3.844, 0.3, 0.4964}},
-    {16, 64, 2, 1, 16, {0.9438, 2.471, 0.1525, 1.247, 0.6929, 0.8009, 5.48, 0.343, 0.3957},
-     {0.9438, 2.471, 0.1525, 1.247, 0.6929, 0.8009, 5.48, 0.343, 0.3957}},
-    {16, 64, 5, 1, 16, {1.91, 0.7856, 0.315, 0.2706, 0.7488, 0.8844, 5.065, 0.3724, 0.0323},
-     {1.91, 0.7856, 0.315, 0.2706, 0.7488, 0.8844, 5.065, 0.3724, 0.0323}},
-    {32, 64, 2, 1, 200, {1.383, 1.998, 0.1806, 1.215, 0.7839, 0.4486, 5.724, 0.3276, 0.22},
-     {1.433, 1.758, 0.1464, 0.889, 0.8775, 0.3399, 3.759, 0.3614, 0.3588}},
-    {64, 64, 2, 17, 1100, {1.359, 2.185, 0.2413, 1.118, 0.8995, 0.2992, 5.873, 0.3927, 0.2173},
-     {1.436, 2.141, 0.1547, 0.9047, 0.8219, 0.2479, 3.299, 0.4126, 0.628}},
-    {64, 128, 2, 17, 1600, {1.829, 1.624, 0.4425, 1.293, 0.9017, 0.2933, 5.003, 0.4268, 0.06747},
-     {1.619, 1.944, 0.2851, 0.7456, 0.6628, 0.265, 3.152, 0.4203, 0.5004}},
-    {128, 128, 1, 48, 2048, {0.7097, 3.826, 0.4999, 0.5, 0.9821, 0.1839, 4.606, 0.6007, 0.2654},
-     {1.237, 3.283, 0.3967, 0.5, 0.7107, 0.2046, 3.22, 0.5711, 0.3912}},
-    {192, 64, 1, 100, 4096, {1.082, 3.236, 0.425, 0.5, 0.9128, 0.2265, 3.92, 0.7776, 0.333},
-     {1.463, 3.563, 0.314, 0.5, 0.6986, 0.1831, 2.826, 0.87, 0.4798}},
-    {128, 192, 2, 65, 1 << 20, {1.728, 5.211, 0.9317, 0.7278, 0.9274, 0.1301, 4.614, 1.419, 0.2164},
-     {0.2758, 6.246, 0.7895, 0.2625, 1.447, 0.1268, 2.763, 1.373, 0.2609}},
-    {192, 128, 2, 129, 1 << 20, {2.827, 2.28, 0.9054, 0.5603, 1.304, 0.2044, 4.273, 1.321, 0.1978},
-     {0.8714, 5.576, 0.7378, 0.3379, 0.9419, 0.1609, 3.116, 1.322, 0.2601}},
-    {128, 256, 1, 65, 1 << 20, {2.206, 4.075, 0.7777, 0.5, 1.661, 0.116, 8.225, 0.9003, 0.6474},
-     {0.5667, 5.809, 0.652, 0.5, 0.9784, 0.1613, 3.133, 1.021, 0.304}},
-    {256, 128, 1, 96, 1 << 20, {1.781, 4.141, 0.6212, 0.5, 1.04, 0.1552, 4.122, 1.065, 0.4548},
-     {1.097, 6.024, 0.4873, 0.5, 0.415, 0.1522, 5.312, 1.086, 0.6831}},
-    {256, 256, 1, 160, 1 << 20, {2.813, 4.153, 1.452, 0.5, 2.865, 0.1676, 4.844, 3.68, 0.3836},
-     {0.4742, 8.871, 1.219, 0.5, 1.493, 0.1593, 3.09, 3.594, 0.2595}},
+    {16, 16, 2, 1, 48, {2.006, 0.0404, 0.9011, 0.7127, 1, 0.2, 4.215, 0.3, 0.5808},
+     {2.006, 0.0404, 0.9011, 0.7127, 1, 0.2, 4.215, 0.3, 0.5808}},
+    {16, 64, 2, 1, 16, {1.075, 2.266, 0.1511, 1.197, 0.7192, 0.8719, 5.66, 0.3479, 0.4062},
+     {1.075, 2.266, 0.1511, 1.197, 0.7192, 0.8719, 5.66, 0.3479, 0.4062}},
+    {16, 64, 5, 1, 16, {1.953, 0.5751, 0.3161, 0.2639, 0.8462, 0.9349, 5.181, 0.373, 0.02961},
+     {1.953, 0.5751, 0.3161, 0.2639, 0.8462, 0.9349, 5.181, 0.373, 0.02961}},
+    {32, 64, 2, 1, 200, {1.401, 1.908, 0.1816, 1.213, 0.8341, 0.4644, 5.823, 0.3286, 0.2125},
+     {1.431, 1.725, 0.1484, 0.8889, 0.9028, 0.3455, 3.762, 0.3651, 0.3336}},
+    {64, 64, 2, 17, 1100, {1.272, 2.407, 0.2147, 1.198, 0.9773, 0.2784, 6.186, 0.3893, 0.3374},
+     {1.541, 2.178, 0.1584, 1.106, 0.8578, 0.2606, 3.462, 0.409, 0.4391}},
+    {64, 128, 1, 17, 1600, {0.6257, 3.355, 0.3741, 0.5, 1.021, 0.2248, 4.766, 0.4157, 0.2747},
+     {1.42, 2.543, 0.2623, 0.5, 0.7342, 0.2412, 3.277, 0.4192, 0.5235}},
+    {128, 128, 1, 48, 2048, {0.5995, 3.757, 0.4858, 0.5, 0.8329, 0.2038, 4.74, 0.6828, 0.3688},
+     {1.256, 3.112, 0.3904, 0.5, 0.6549, 0.2295, 3.025, 0.6031, 0.4285}},
+    {192, 64, 1, 100, 4096, {1.341, 2.825, 0.4221, 0.5, 0.9907, 0.2522, 4.439, 0.7727, 0.3601},
+     {1.433, 3.447, 0.3145, 0.5, 0.8059, 0.1902, 2.68, 0.8677, 0.4794}},
+    {128, 192, 2, 65, 1 << 20, {1.814, 4.734, 0.935, 0.6605, 1.004, 0.1143, 4.959, 1.509, 0.2237},
+     {0.1866, 6.255, 0.7796, 0.2627, 1.395, 0.1239, 2.824, 1.42, 0.2704}},
+    {192, 128, 2, 129, 1 << 20, {2.937, 1.886, 0.9098, 0.5362, 1.39, 0.2002, 4.871, 1.388, 0.1955},
+     {0.7776, 5.342, 0.7345, 0.3317, 1.109, 0.1562, 2.929, 1.366, 0.2663}},
+    {128, 256, 1, 65, 1 << 20, {2.105, 3.737, 0.7957, 0.5, 1.454, 0.1432, 6.805, 1.016, 0.5145},
+     {0.659, 5.642, 0.6385, 0.5, 0.5123, 0.1937, 3.156, 1.142, 0.3352}},
+    {256, 128, 1, 96, 1 << 20, {1.903, 3.708, 0.6029, 0.5, 0.6856, 0.1807, 4.557, 1.279, 0.5604},
+     {1.203, 5.711, 0.4825, 0.5, 0.3244, 0.1771, 3.293, 1.104, 0.694}},
+    {256, 256, 1, 160, 1 << 20, {2.705, 3.972, 1.437, 0.5, 3.409, 0.1492, 3.737, 3.916, 0.2705},
+     {0.5704, 8.532, 1.212, 0.5, 1.722, 0.1521, 2.879, 3.68, 0.2629}},
 };
 
 static double gemm8_cost(int kernel, int M, int out, int N, int K, int act, int splits, int cus) {

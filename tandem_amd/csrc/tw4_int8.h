@@ -82,7 +82,7 @@ struct Gemm8Args {
 // The tiles of tw4_gemm8_lds.hip: kernel number, 16-token tiles and 16-row tiles of a wavefront, wavefronts along tokens and rows, slots
 // of the ring. Kernel 0 is the streaming one of tw4_gemm8.hip.
 #define TW4_GEMM8_LDS(X)                                                                                             \
-    X(1, 1, 2, 1, 2, 7) X(2, 1, 2, 1, 2, 3) X(3, 1, 2, 2, 2, 5) X(4, 2, 2, 2, 2, 4) X(5, 2, 2, 2, 4, 3) X(6, 4, 2, 2, 4, 3) \
+    X(1, 1, 2, 1, 2, 7) X(2, 1, 2, 1, 2, 3) X(3, 1, 2, 2, 2, 5) X(4, 2, 2, 2, 2, 5) X(5, 2, 2, 2, 4, 6) X(6, 4, 2, 2, 4, 3) \
     X(7, 6, 2, 2, 2, 3) X(8, 4, 6, 2, 2, 2) X(9, 6, 4, 2, 2, 2) X(10, 4, 4, 2, 4, 3) X(11, 4, 4, 4, 2, 3) X(12, 8, 4, 2, 4, 2)
 constexpr int kGemm8Kernels = 13;
 
