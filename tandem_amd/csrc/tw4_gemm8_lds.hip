@@ -238,6 +238,11 @@ gemm8_lds_kernel(const int8_t* __restrict__ x, uint32_t x_stride, const float* _
     ring_barrier();
     gemm8_read<C, ACT>(regs.a[0], regs.b[0], base + ao, base + bo);
     int slot = 0;
+#pragma unroll
+    for (int t = 0; t < TN; ++t)
+#pragma unroll
+        for (int b = 0; b < TM; ++b) asm volatile("" : "+a"(acc[t][b]));
+    asm volatile("s_nop 4" ::: "memory");  // the zeros are written before the first product reads them
     for (int i = 0; i < stages; ++i) {
         const char* cur = base + slot * C::SLOT;
         const uint32_t cur_addr = ring_addr + slot * C::SLOT;
@@ -339,7 +344,7 @@ int gemm8_lds_launch(const Gemm8Args& a, int splits) {
     constexpr int FEATURES = ACT ? C::BN / 2 : C::BN;
     const int out = ACT ? a.N / 2 : a.N, mb = (a.M + C::BM - 1) / C::BM, nb = (out + FEATURES - 1) / FEATURES;
     const int64_t units = static_cast<int64_t>(mb) * nb * splits;
-    TW4_REQUIRE(units < int64_t(1) << 24, TW4_EINVAL, "gemm_int8: too many tiles (M %d, N %d)", a.M, a.N);
+    TW4_REQUIRE(units * C::THREADS < int64_t(1) << 32, TW4_EINVAL, "gemm_int8: too many tiles (M %d, N %d)", a.M, a.N);
     if (splits > 1) {
         const int64_t ints = units * C::BM * C::BN;
         TW4_REQUIRE(a.ws && a.locks, TW4_EINVAL, "gemm_int8: splits take a workspace");

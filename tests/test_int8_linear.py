@@ -45,6 +45,7 @@ def test_argument_errors_return_before_launch():
     for change, status, needle in (({13: 256, 1: 256, 4: 256, 17: 2}, w4_hip.TW4_EINVAL, "workspace"),
                                    ({13: 256, 1: 256, 4: 256, 17: 2, 7: p, 8: 2 * 32 * 64 - 1, 9: p, 10: 1}, w4_hip.TW4_ESPACE, "partial sums"),
                                    ({13: 256, 1: 256, 4: 256, 17: 2, 7: p, 8: 2 * 32 * 64, 9: p, 10: 0}, w4_hip.TW4_ESPACE, "counters"),
+                                   ({11: 1 << 20, 12: 1 << 20}, w4_hip.TW4_EINVAL, "too many"), ({11: 1 << 20, 16: 0}, w4_hip.TW4_ECONFIG, "streaming"),
                                    ({12: 6, 14: 1, 16: 0}, w4_hip.TW4_ECONFIG, "SwiGLU"), ({11: 17, 16: 1}, w4_hip.TW4_ECONFIG, "16 tokens"),
                                    ({11: 17, 16: 2}, w4_hip.TW4_ECONFIG, "16 tokens")):
         args = list(good)
@@ -252,6 +253,18 @@ def test_strides_scales_and_neighbours(m, n, k, silu_mul):
     keep = [i for i in range(m) if i not in (0, m // 2)]
     cols = [j for j in range(y.shape[1]) if j != 1]
     assert torch.equal(y2[keep][:, cols], y[keep][:, cols]) and (m // 2 == 0 or not bool(y2[0, cols].any()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(2, 1 << 20, 4112), (20, 1 << 20, 4112), (140, 1 << 20, 4112), (70001, 32768, 64), (300000, 16, 16384)])
+def test_past_32_bits(m, n, k):
+    """Weights, activations and results of more than 2^32 bytes: rows and columns at both ends and in between."""
+    x, xs, w, ws = _operands(m, n, k, seed=k)
+    y = w8.linear_int8(x, xs, w, ws)
+    rows = torch.tensor(sorted({0, 1, m // 2, m - 2, m - 1}), device="cuda")
+    for at in (0, n // 2 - 8, n - 16):
+        cols = slice(at, at + 16)
+        _check(y[rows, cols].contiguous(), x[rows], xs[rows], w[cols], ws[cols], False, torch.float16)
 
 
 @pytest.mark.gpu

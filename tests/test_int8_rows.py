@@ -26,7 +26,7 @@ def test_argument_errors_return_before_launch():
     good = [p, 64, p, p, 3, 64, 0]  # x stride codes scales M K bf16
     for at, value, needle in ((0, None, "null"), (2, None, "null"), (3, None, "null"), (0, odd, "aligned"), (2, odd, "aligned"),
                               (3, ctypes.c_void_p(4098), "aligned"), (1, 56, "apart"), (1, 68, "apart"), (4, -1, "M >= 0"), (5, 24, "K %"),
-                              (5, 0, "K %"), (5, 32784, "K %")):
+                              (5, 0, "K %"), (5, 32784, "K %"), (4, 1 << 26, "too many")):
         args = list(good)
         args[at] = value
         assert lib.tw4_quantize_int8(*args, None) == w4_hip.TW4_EINVAL, (at, value)
@@ -35,7 +35,7 @@ def test_argument_errors_return_before_launch():
     assert lib.tw4_quantize_int8(*good, None) == w4_hip.TW4_OK
     good = [p, 64, p, 64, p, 1e-6, p, p, 3, 64, 0]  # x stride residual stride weight eps codes scales M K bf16
     for at, value, needle in ((0, None, "null"), (4, None, "null"), (4, odd, "aligned"), (2, odd, "aligned"), (3, 56, "apart"),
-                              (3, 68, "apart"), (9, 40, "K %"), (8, -1, "M >= 0")):
+                              (3, 68, "apart"), (9, 40, "K %"), (8, -1, "M >= 0"), (8, 1 << 26, "too many")):
         args = list(good)
         args[at] = value
         assert lib.tw4_rms_norm_int8(*args, None) == w4_hip.TW4_EINVAL, (at, value)
@@ -222,3 +222,21 @@ def test_strides_and_shared_buffers(dtype):
         w8.quantize_int8(x.clone().requires_grad_())
     one = wide[3:4, 16:16 + k]
     assert torch.equal(w8.quantize_int8(one)[0], w8.quantize_int8(x)[0][3:4])
+
+
+@pytest.mark.gpu
+def test_past_32_bits():
+    """More than 2^32 bytes of values and of codes."""
+    m, k = 150001, 32768
+    x = torch.empty(m, k, dtype=torch.float16, device="cuda").normal_()
+    at = torch.tensor([0, 1, 65535, 65536, 131072, m - 1], device="cuda")
+    kept = x[at]
+    codes, scales = w8.quantize_int8(x)
+    want, top = _codes(kept.double())
+    assert torch.equal(codes[at], want) and bool(((scales[at].double() - top / 127).abs() <= 2 * STEP * top / 127).all())
+    del codes
+    w = (0.5 + torch.rand(k, device="cuda")).half()
+    r = torch.ones_like(x)
+    codes, _, _ = norm.fused_add_rms_norm_int8(x, r, w, EPS)
+    s = kept.float() + 1
+    assert torch.equal(codes[at], _codes(s.double() * w.double())[0]) and torch.equal(r[at], s.half())
