@@ -4,6 +4,9 @@
 // The kernel for few tokens streams w through registers. A workgroup of 16 wavefronts takes `rows` rows of w, up to NT tiles of 16,
 // and 16 tokens; as many rows as give every CU the same work. Units of 128 k go to the wavefronts in turn, so that the workgroup reads
 // each row in pieces of 2 KB; each wavefront has one unit in flight ahead of the math. The wavefronts' sums are added in LDS.
+// Bound by reading w behind a launch: K 4096 x N 6144 at M = 1 7.3 us (3.4 TB/s; 25 MB at 5.9 TB/s, what a plain read reaches, are 4.3, the
+// launch and the first and last round trips the rest), K 12288 x N 4096 12.3 (4.1 TB/s). 4 or 8 wavefronts per workgroup, or 2 units ahead:
+// within 5 %. Two 16-row tiles per workgroup where one fills the CUs: 20-60 % slower.
 #include <math.h>
 
 #include "tw4_int8.h"
