@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(64 * W) rows_int8_kernel(const u4* __restrict_
                                                                   int64_t r_step, const u4* __restrict__ w, float eps,
                                                                   u2* __restrict__ codes, float* __restrict__ scales, int chunks) {
     __shared__ double top_of[W];
-    __shared__ float sum_of[W], topf_of[W];
+    __shared__ float topf_of[W], group_of[NORM ? 4 * W * J : 1];  // group_of: sums of squares of 16 chunks
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t row = blockIdx.x;
     const u4* xr = x + row * x_step;
@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(64 * W) rows_int8_kernel(const u4* __restrict_
         }
     }
     float s[J][8], t[NORM ? J : 1][8];
-    float sum = 0.0f, topf = 0.0f, most[J];  // most: of a chunk
+    float topf = 0.0f, most[J];  // most: of a chunk
     const auto tf = [&](int j, int i) -> float { return NORM ? t[NORM ? j : 0][i] : s[j][i]; };
 #pragma unroll
     for (int j = 0; j < J; ++j) {
@@ -90,16 +90,16 @@ __global__ void __launch_bounds__(64 * W) rows_int8_kernel(const u4* __restrict_
         }
         most[j] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if constexpr (NORM) sum = __builtin_fmaf(s[j][i], s[j][i], sum);
-            most[j] = larger(most[j], fabsf(tf(j, i)));
-        }
+        for (int i = 0; i < 8; ++i) most[j] = larger(most[j], fabsf(tf(j, i)));
         topf = larger(topf, most[j]);
+        if constexpr (NORM) {
+            const float q = row16_sum(sumsq8(s[j]));
+            if ((lane & 15) == 0) group_of[4 * (W * j + wave) + (lane >> 4)] = q;
+        }
     }
     topf = wave_largest(topf);
     double top = static_cast<double>(topf);
     if constexpr (NORM) {
-        sum = wave_total(sum);
         // the exact largest is among those that round to topf
         double mine = 0.0;
 #pragma unroll
@@ -121,21 +121,22 @@ __global__ void __launch_bounds__(64 * W) rows_int8_kernel(const u4* __restrict_
         }
     }
     if constexpr (W > 1) {
-        if (lane == 0) top_of[wave] = top, topf_of[wave] = topf, sum_of[wave] = sum;
-        __syncthreads();
-        top = 0.0, topf = 0.0f, sum = 0.0f;
+        if (lane == 0) top_of[wave] = top, topf_of[wave] = topf;
+    }
+    __syncthreads();
+    if constexpr (W > 1) {
+        top = 0.0, topf = 0.0f;
 #pragma unroll
         for (int v = 0; v < W; ++v) {
             if constexpr (NORM) top = fmax(top, top_of[v]);
             topf = larger(topf, topf_of[v]);
-            if constexpr (NORM) sum += sum_of[v];
         }
         if constexpr (!NORM) top = static_cast<double>(topf);
     }
     const bool nan = !(topf < __builtin_inff()), none = nan || topf < kLeast;
-    if (lane == 0 && wave == 0) {
-        const float rstd = NORM ? rsqrtf(sum / static_cast<float>(8 * chunks) + eps) : 1.0f;
-        scales[row] = nan ? __builtin_nanf("") : none ? 0.0f : topf * rstd / 127.0f;
+    if (wave == 0) {  // rstd in the order of the other norms: the same bits whatever W and J
+        const float rstd = NORM ? norm_rstd(group_of, (chunks + 15) / 16, 8 * chunks, eps, lane) : 1.0f;
+        if (lane == 0) scales[row] = nan ? __builtin_nanf("") : none ? 0.0f : topf * rstd / 127.0f;
     }
     const float inv = 127.0f / topf;
     const uint32_t keep = none ? 0u : ~0u;

@@ -113,7 +113,7 @@ def _rms_norm_int8(who: str, x: torch.Tensor, residual: torch.Tensor | None, wei
     step, r_step, m, k, code, index = check_rows(who, layout(x), None if residual is None else layout(residual), layout(weight))
     if not (w4_hip.plain(x) if residual is None else w4_hip.all_plain(x, residual)):
         raise RuntimeError(f"{who}: inference only, no gradient, transform or tracer can follow x or the residual")
-    codes, scales = x.new_empty((m, k), dtype=torch.int8), x.new_empty((m,), dtype=torch.float32)
+    codes, scales = x.new_empty(m, k, dtype=torch.int8), x.new_empty(m, dtype=torch.float32)
     if m:
         xp, rp, wp = x.data_ptr(), 0 if residual is None else residual.data_ptr(), weight.data_ptr()
         if (xp | rp | wp) % 16:

@@ -31,7 +31,7 @@ def quantize_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     step, _, m, k, code, index = norm.check_rows("quantize_int8", layout(x), None, None)
     if not w4_hip.plain(x):
         raise RuntimeError("quantize_int8: inference only, no gradient, transform or tracer can follow x")
-    codes, scales = x.new_empty((m, k), dtype=torch.int8), x.new_empty((m,), dtype=torch.float32)
+    codes, scales = x.new_empty(m, k, dtype=torch.int8), x.new_empty(m, dtype=torch.float32)
     if m:
         xp = x.data_ptr()
         if xp % 16:
@@ -86,7 +86,7 @@ def linear_int8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, we
                                                            bool(silu_mul), dtype)
     if not w4_hip.all_plain(x, x_scale, weight, weight_scale):
         raise RuntimeError("linear_int8: inference only, no gradient, transform or tracer can follow the operands")
-    y = x.new_empty((sizes[0], features), dtype=dtype)
+    y = x.new_empty(sizes[0], features, dtype=dtype)
     if sizes[0]:
         xp, wp = x.data_ptr(), weight.data_ptr()
         if (xp | wp) % 16:

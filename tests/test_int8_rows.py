@@ -3,9 +3,9 @@
 Codes are exact. t = s * weight has 24 + 11 bits at most and 127 t 42, both exact in 64 bits; t / max|t| lies on a border between two
 codes or at least 2^-43 of itself beside it, so a quotient rounded to 53 bits decides every code as the exact one would.
 
-Scales. max|t| is rounded to float32, divided by 127: 2 roundings, 2^-24 each. With the norm: s is rounded, a lane adds up to 32 squares, 6
-steps add lanes and 16 wavefronts' sums are added, all positive, so that the sum is off by at most 2 + 32 + 6 + 16 = 56
-roundings and its root by 28; mean, eps, reciprocal root (2) and product are 5 more: 36 of 2^-24 in all."""
+Scales. max|t| is rounded to float32, divided by 127: 2 roundings, 2^-24 each. With the norm: s is rounded, a chunk adds 8 squares, 4
+steps add 16 chunks, a lane up to 4 of those sums and 6 steps the lanes, all positive, so that the sum is off by at most 2 + 8 + 4 +
+4 + 6 = 24 roundings and its root by 12; mean, eps, reciprocal root (2) and product are 5 more: 19 of 2^-24 in all; 36 are allowed."""
 
 from __future__ import annotations
 
@@ -136,6 +136,20 @@ def test_norm(k, dtype, add):
         full = x0.double() + r0.double() if add else x0.double()
         scale = top * torch.rsqrt((full * full).mean(-1) + EPS) / 127
         assert bool(((scales.double() - scale).abs() <= 36 * STEP * scale).all()) and torch.equal(x, x0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("k", WIDTHS)
+def test_rows_do_not_depend_on_the_batch(k, dtype):
+    """Codes and scales of a row are the same bits whatever the batch."""
+    m = 1030
+    x, r = _rows(m, k, dtype, seed=k), _rows(m, k, dtype, seed=k + 1)
+    w = (0.5 + torch.rand(k, device="cuda")).to(dtype)
+    want = norm.rms_norm_int8(x, w, EPS), norm.fused_add_rms_norm_int8(x, r.clone(), w, EPS), w8.quantize_int8(x)
+    for n in (1, 3, 255, 256, 1023):
+        got = norm.rms_norm_int8(x[-n:], w, EPS), norm.fused_add_rms_norm_int8(x[-n:], r[-n:].clone(), w, EPS), w8.quantize_int8(x[-n:])
+        assert all(torch.equal(a, b[-n:]) for g, v in zip(got, want) for a, b in zip(g, v)), n
 
 
 @pytest.mark.gpu
