@@ -391,6 +391,15 @@ int tw4_gemm_int8(const int8_t* x, int64_t x_stride, const float* x_scale, const
  * out[0 .. 4). Splits stay within TW4_AUTO_SPLIT_FLOATS and TW4_AUTO_SPLIT_COUNTERS. Host code. */
 int tw4_gemm_int8_plan(int M, int N, int K, int act, int cus, int* out);
 
+/* One token's projection in one kernel: x [K] of fp16 (bf16 = 1: bfloat16) put in 8 bits as tw4_quantize_int8 does (norm_weight NULL) or
+ * tw4_rms_norm_int8 (with residual [K]: of x + residual, which goes to residual_out, rounded; not in place), then tw4_gemm_int8's product
+ * with w [N, K] (act = 1: SwiGLU) -> y [N] or [N / 2]: the same bits as the two one behind the other. K <= TW4_TOKEN_INT8_MAX; cus: the
+ * device's CUs, and at most 32 outputs (16 with act = 1) for each of them. No reference counterpart. */
+#define TW4_TOKEN_INT8_MAX 16384
+int tw4_token_int8(const uint16_t* x, const uint16_t* residual, uint16_t* residual_out, const uint16_t* norm_weight, float eps,
+                   const int8_t* w, int64_t w_stride, const float* w_scale, uint16_t* y, int N, int K, int act, int bf16, int cus,
+                   void* stream);
+
 /* Streaming-read probe: reads `bytes` (a multiple of 16) from the device buffer `src` with 16-byte
  * non-temporal loads (1 KB per wavefront instruction, `inflight` = 1, 2, 4 or 8 issued per lane
  * before any is used) over `workgroups`

@@ -9,7 +9,7 @@
 // within 5 %. Two 16-row tiles per workgroup where one fills the CUs: 20-60 % slower.
 #include <math.h>
 
-#include "tw4_int8.h"
+#include "tw4_rows8.h"
 
 namespace tw4 {
 
@@ -87,6 +87,133 @@ __global__ void __launch_bounds__(64 * kStreamWaves) gemm8_stream_kernel(const i
 #pragma unroll
     for (int i = 0; i < 4; ++i)
         if (at + i < rows) row[i] = static_cast<uint16_t>(value16<BF16>(static_cast<float>(sum[i]) * xs * s[i]));
+}
+
+// One token, its row put in 8 bits on the way (the bits of the kernels that do it alone). The streaming kernel above; every workgroup makes the
+// whole row, in LDS, while its first rows of w are on the way: TILES tiles of 16 outputs, with SwiGLU one of gate rows and one of up rows.
+// Workgroup 0 writes the new residual, to memory of its own: others still read the old one.
+// Against the two kernels in a graph, us (weights from HBM; SwiGLU: the tiled kernel with K splits): row alone, norm, add + norm:
+//   K 4096 x N 6144   8.3, 8.5, 8.6 (9.2, 9.7, 9.7)     K 9728 x N 2560      8.6, 9.5, 9.6 (10.1, 11.4, 11.3)
+//   K 512 x N 1024    3.5, 4.6, 4.6 (4.5, 5.3, 5.0)     K 2064 x 2501 pairs  6.1, 6.7, 6.7 (9.5, 10.1, 10.2)
+// and 8 to 10 where a caller waits for the host (16.5 to 18). More outputs than one workgroup a CU holds lose, each round making the row again:
+//   K 8192 x N 10240  20.8, 25.8, 25.8 (18.2, 19, 19)   K 4096 x 14336 pairs  31, 35, 36 (25, 25, 25.5)
+// and so does SwiGLU in 32 pairs a workgroup (K 2560 x 6912 pairs 12.2, 12.1, 12.1 (10.1, 10.7, 10.8)), so that it is left at 16.
+template <int TILES, bool ACT, bool NORM, bool ADD, bool BF16, int J>
+__global__ void __launch_bounds__(64 * kStreamWaves) token8_kernel(const u4* __restrict__ x, const u4* __restrict__ r, u4* __restrict__ r_out,
+                                                                   const u4* __restrict__ norm_weight, float eps, const int8_t* __restrict__ w,
+                                                                   uint32_t w_stride, const float* __restrict__ w_scale,
+                                                                   uint16_t* __restrict__ y, int N, int K, int rows_each) {
+    constexpr int NT = ACT ? 2 * TILES : TILES;
+    constexpr bool late = NORM && NT * J > 2;  // 128 registers do not hold the row and both steps
+    __shared__ Row8Shared<NORM, kStreamWaves, J> shared;
+    __shared__ u2 codes[64 * kStreamWaves * J];
+    __shared__ i4 part[kStreamWaves][NT][64];
+    __shared__ float x_scale;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 15, q = lane >> 4;
+    const int out = ACT ? N >> 1 : N, n0 = rows_each * blockIdx.x, chunks = K >> 3;
+    Row8Loads<J> row;
+    row8_load<NORM, ADD, kStreamWaves, J>(row, x, r, norm_weight, chunks, wave, lane);
+    // what lies past the rows or K is past the resources' records: zeros, nothing read
+    const int rows = min(out - n0, rows_each), size = (rows - 1) * w_stride + K;
+    const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(w + static_cast<int64_t>(n0) * w_stride), 0, size, kBufferFlags);
+    const __amdgpu_buffer_rsrc_t ur =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(w + static_cast<int64_t>(ACT ? out + n0 : n0) * w_stride), 0, size, kBufferFlags);
+    uint32_t wo[TILES];
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) wo[t] = 16 * t + lr < rows ? static_cast<uint32_t>(16 * t + lr) * w_stride + 16 * q : 0x80000000u;
+    const int units = (K + 127) >> 7, steps = (units - wave + kStreamWaves - 1) / kStreamWaves;  // of this wavefront's units
+    const auto load = [&](u4 (&v)[NT][2], int s) {
+        const int k = 128 * (s * kStreamWaves + wave);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t past = k + 64 * h + 16 * q < K ? 0u : 0x80000000u;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+                v[t][h] = bitcast<u4>(__builtin_amdgcn_raw_buffer_load_b128(t < TILES ? wr : ur, (wo[t % TILES] | past) + 64 * h, k, 2));
+        }
+    };
+    i4 acc[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[t] = i4{0, 0, 0, 0};
+    const char* xc = reinterpret_cast<const char*>(codes) + 16 * q;  // every column is the token: one is stored
+    const auto multiply = [&](const u4 (&v)[NT][2], int s) {
+        const int k = 128 * (s * kStreamWaves + wave);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const u4 b = *reinterpret_cast<const u4*>(xc + k + 64 * h);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) acc[t] = mfma_i8(v[t][h], b, acc[t]);
+        }
+    };
+    u4 v0[NT][2], v1[NT][2];
+    if (steps > 0) load(v0, 0);
+    if (!late && steps > 1) load(v1, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    row8_quantize<NORM, ADD, BF16, kStreamWaves, J>(row, shared, blockIdx.x == 0 ? r_out : nullptr, codes, &x_scale, eps, chunks, wave, lane);
+    if (late && steps > 1) load(v1, 1);
+    __syncthreads();
+    for (int s = 0; s < steps; s += 2) {
+        multiply(v0, s);
+        if (s + 1 >= steps) break;
+        if (s + 2 < steps) load(v0, s + 2);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(v1, s + 1);
+        if (s + 3 < steps) load(v1, s + 3);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) part[wave][t][lane] = acc[t];
+    __syncthreads();
+    if (wave >= TILES || lr != 0) return;  // wavefront t adds tile t
+    const int at = 16 * wave + 4 * q, n = n0 + at;
+    i4 sum{0, 0, 0, 0}, up{0, 0, 0, 0};
+#pragma unroll 4
+    for (int v = 0; v < kStreamWaves; ++v) {
+        sum += part[v][wave][lane];
+        if constexpr (ACT) up += part[v][wave + TILES][lane];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (at + i >= rows) break;
+        float v = static_cast<float>(sum[i]) * x_scale * w_scale[n + i];
+        if constexpr (ACT) v = silu_rcp(v) * (static_cast<float>(up[i]) * x_scale * w_scale[out + n + i]);
+        y[n + i] = static_cast<uint16_t>(value16<BF16>(v));
+    }
+}
+
+struct Token8Args {
+    const u4 *x, *r;
+    u4* r_out;
+    const u4* norm_weight;
+    float eps;
+    const int8_t* w;
+    uint32_t w_stride;
+    const float* w_scale;
+    uint16_t* y;
+    int N, K, rows;
+    hipStream_t st;
+};
+
+template <int TILES, bool ACT, bool NORM, bool ADD, bool BF16>
+int token8_launch(const Token8Args& a) {
+    const int out = ACT ? a.N / 2 : a.N;
+    const unsigned grid = static_cast<unsigned>((out + a.rows - 1) / a.rows);
+    const auto kernel = a.K <= 512 * kStreamWaves ? token8_kernel<TILES, ACT, NORM, ADD, BF16, 1> : token8_kernel<TILES, ACT, NORM, ADD, BF16, 2>;
+    kernel<<<grid, 64 * kStreamWaves, 0, a.st>>>(a.x, a.r, a.r_out, a.norm_weight, a.eps, a.w, a.w_stride, a.w_scale, a.y, a.N, a.K, a.rows);
+    TW4_LAUNCH_CHECK("token_int8: launch");
+    return TW4_OK;
+}
+
+template <int TILES, bool ACT, bool BF16>
+int token8_norm(const Token8Args& a) {
+    if (!a.norm_weight) return token8_launch<TILES, ACT, false, false, BF16>(a);
+    return a.r ? token8_launch<TILES, ACT, true, true, BF16>(a) : token8_launch<TILES, ACT, true, false, BF16>(a);
+}
+
+template <bool BF16>
+int token8_any(const Token8Args& a, int act) {
+    if (act) return token8_norm<1, true, BF16>(a);
+    return a.rows <= 16 ? token8_norm<1, false, BF16>(a) : token8_norm<2, false, BF16>(a);
 }
 
 // Rows of w per workgroup of the streaming kernel: what gives every CU one workgroup, where that is 4 to 32 rows, else 16. M = 1, us, with
@@ -203,6 +330,34 @@ static int gemm8_check_sizes(int M, int N, int K, int act) {
 }  // namespace tw4
 
 using namespace tw4;
+
+extern "C" int tw4_token_int8(const uint16_t* x, const uint16_t* residual, uint16_t* residual_out, const uint16_t* norm_weight, float eps,
+                              const int8_t* w, int64_t w_stride, const float* w_scale, uint16_t* y, int N, int K, int act, int bf16, int cus,
+                              void* stream) {
+    TW4_REQUIRE(x && w && w_scale && y, TW4_EINVAL, "token_int8: null pointer");
+    TW4_REQUIRE(reinterpret_cast<uintptr_t>(x) % 16 == 0 && reinterpret_cast<uintptr_t>(w) % 16 == 0 &&
+                    reinterpret_cast<uintptr_t>(residual) % 16 == 0 && reinterpret_cast<uintptr_t>(residual_out) % 16 == 0 &&
+                    reinterpret_cast<uintptr_t>(norm_weight) % 16 == 0,
+                TW4_EINVAL, "token_int8: rows must be 16-byte aligned");
+    TW4_REQUIRE(reinterpret_cast<uintptr_t>(w_scale) % 4 == 0 && reinterpret_cast<uintptr_t>(y) % 2 == 0, TW4_EINVAL,
+                "token_int8: scales must be 4-byte aligned and y 2-byte");
+    TW4_REQUIRE(!residual == !residual_out && (!residual || norm_weight), TW4_EINVAL,
+                "token_int8: a residual comes with a norm weight and memory for the new one");
+    TW4_REQUIRE(residual_out != residual || !residual, TW4_EINVAL, "token_int8: the new residual needs memory of its own");
+    const int rc = gemm8_check_sizes(1, N, K, act);
+    if (rc) return rc;
+    TW4_REQUIRE(K <= TW4_TOKEN_INT8_MAX, TW4_EINVAL, "token_int8: K <= %d (K = %d)", TW4_TOKEN_INT8_MAX, K);
+    TW4_REQUIRE(w_stride >= K && w_stride % 16 == 0 && w_stride < 1 << 22, TW4_EINVAL,
+                "token_int8: rows at least K and less than 2^22 apart, 16-byte aligned (stride %lld)", static_cast<long long>(w_stride));
+    TW4_REQUIRE(cus >= 1, TW4_EINVAL, "token_int8: cus >= 1");
+    const int out = act ? N / 2 : N, rows = stream8_rows(out, cus);
+    TW4_REQUIRE((out + rows - 1) / rows <= cus && rows <= (act ? 16 : 32), TW4_ECONFIG,
+                "token_int8: at most 32 outputs, or 16 of SwiGLU, a CU (%d outputs, %d CUs)", out, cus);
+    const Token8Args a{reinterpret_cast<const u4*>(x), reinterpret_cast<const u4*>(residual), reinterpret_cast<u4*>(residual_out),
+                       reinterpret_cast<const u4*>(norm_weight), eps, w, static_cast<uint32_t>(w_stride), w_scale, y, N, K, rows,
+                       static_cast<hipStream_t>(stream)};
+    return bf16 ? token8_any<true>(a, act) : token8_any<false>(a, act);
+}
 
 extern "C" int tw4_gemm_int8_plan(int M, int N, int K, int act, int cus, int* out) {
     const int rc = gemm8_check_sizes(M, N, K, act);

@@ -17,161 +17,20 @@
 // (5.5), in 4 wavefronts of 2; 8 of 1 22.3, 26.7, 42.2; 2 of 4 21.1, 21.8, 44.0. M = 4096, K 12288: 27.9, 32.6, 69 in 8 of 3; 16 of 2 27.5,
 // 55, 82. Dividing every value in 64 bits took 54 us where 27.9 are now (M = 4096, K 12288, quantised). Four rows per
 // workgroup, a wavefront each, were slower than one at every width (K 512, M = 16384, add + norm 13.9 against 13.4).
-#include "tw4_int8.h"
+#include "tw4_rows8.h"
 
 namespace tw4 {
 
-constexpr float kLeast = 0x1p-100f;  // rows whose largest magnitude is below it count as zeros: 127 / max stays finite
-constexpr float kMagic = 12582912.0f;    // 1.5 2^23: a float32 of its binade counts by ones, so that adding it rounds, halves to even
-constexpr float kBorder = 0.5f - 3.1e-5f;
-
-// The larger of both, NaN if either is (v_maximum3_f32): an infinity or a NaN in a row comes out as its maximum.
-__device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
-
-// Largest of the 64 lanes' values.
-__device__ __forceinline__ float wave_largest(float v) {
-    v = larger(v, lane_xor1(v));
-    v = larger(v, lane_xor2(v));
-    v = larger(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xF, 0xF, false)));
-    v = larger(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x140, 0xF, 0xF, false)));
-    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = larger(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return larger(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-
-// The code of t (fl(t) tf) where r = tf fl(127 / fl(top)) is next to a border: the codes of r's size c and c + 1 are compared with t itself.
-__device__ __forceinline__ float border_code(float r, double t, double top) {
-    const float c = floorf(fabsf(r));
-    const double at = 254.0 * fabs(t), border = (2.0 * static_cast<double>(c) + 1.0) * top;
-    const bool odd = static_cast<int>(c) & 1;
-    const float n = at > border || (at == border && odd) ? c + 1.0f : c;
-    return copysignf(n, r);
-}
-
 template <bool NORM, bool ADD, bool BF16, int W, int J>
 __global__ void __launch_bounds__(64 * W) rows_int8_kernel(const u4* __restrict__ x, int64_t x_step, u4* __restrict__ r,
-                                                                  int64_t r_step, const u4* __restrict__ w, float eps,
-                                                                  u2* __restrict__ codes, float* __restrict__ scales, int chunks) {
-    __shared__ double top_of[W];
-    __shared__ float topf_of[W], group_of[NORM ? 4 * W * J : 1];  // group_of: sums of squares of 16 chunks
+                                                           int64_t r_step, const u4* __restrict__ w, float eps,
+                                                           u2* __restrict__ codes, float* __restrict__ scales, int chunks) {
+    __shared__ Row8Shared<NORM, W, J> shared;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t row = blockIdx.x;
-    const u4* xr = x + row * x_step;
-    u4* rr = r + row * r_step;
-    u4 xv[J], rv[J], wv[J];
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-        const int c = 64 * (W * j + wave) + lane;
-        xv[j] = rv[j] = wv[j] = u4{0, 0, 0, 0};
-        if (c < chunks) {
-            xv[j] = xr[c];
-            if constexpr (ADD) rv[j] = rr[c];
-            if constexpr (NORM) wv[j] = w[c];
-        }
-    }
-    float s[J][8], t[NORM ? J : 1][8];
-    float topf = 0.0f, most[J];  // most: of a chunk
-    const auto tf = [&](int j, int i) -> float { return NORM ? t[NORM ? j : 0][i] : s[j][i]; };
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-        chunk_values<BF16>(xv[j], s[j]);
-        if constexpr (ADD) {
-            float b[8];
-            chunk_values<BF16>(rv[j], b);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s[j][i] += b[i];
-        }
-        if constexpr (NORM) {
-            float g[8];
-            chunk_values<BF16>(wv[j], g);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) t[j][i] = s[j][i] * g[i];
-        }
-        most[j] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) most[j] = larger(most[j], fabsf(tf(j, i)));
-        topf = larger(topf, most[j]);
-        if constexpr (NORM) {
-            const float q = row16_sum(sumsq8(s[j]));
-            if ((lane & 15) == 0) group_of[4 * (W * j + wave) + (lane >> 4)] = q;
-        }
-    }
-    topf = wave_largest(topf);
-    double top = static_cast<double>(topf);
-    if constexpr (NORM) {
-        // the exact largest is among those that round to topf
-        double mine = 0.0;
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-            if (most[j] != topf) continue;
-            float g[8];
-            chunk_values<BF16>(wv[j], g);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (fabsf(t[j][i]) == topf) mine = fmax(mine, fabs(static_cast<double>(s[j][i]) * static_cast<double>(g[i])));
-        }
-        top = 0.0;
-        for (uint64_t lanes = __ballot(mine > 0.0); lanes; lanes &= lanes - 1) {  // one lane, nearly always
-            const int l = __builtin_ctzll(lanes);
-            const uint64_t bits = bitcast<uint64_t>(mine);
-            const uint64_t other = static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<int>(bits >> 32), l)) << 32 |
-                                   static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(bits), l));
-            top = fmax(top, bitcast<double>(other));
-        }
-    }
-    if constexpr (W > 1) {
-        if (lane == 0) top_of[wave] = top, topf_of[wave] = topf;
-    }
-    __syncthreads();
-    if constexpr (W > 1) {
-        top = 0.0, topf = 0.0f;
-#pragma unroll
-        for (int v = 0; v < W; ++v) {
-            if constexpr (NORM) top = fmax(top, top_of[v]);
-            topf = larger(topf, topf_of[v]);
-        }
-        if constexpr (!NORM) top = static_cast<double>(topf);
-    }
-    const bool nan = !(topf < __builtin_inff()), none = nan || topf < kLeast;
-    if (wave == 0) {  // rstd in the order of the other norms: the same bits whatever W and J
-        const float rstd = NORM ? norm_rstd(group_of, (chunks + 15) / 16, 8 * chunks, eps, lane) : 1.0f;
-        if (lane == 0) scales[row] = nan ? __builtin_nanf("") : none ? 0.0f : topf * rstd / 127.0f;
-    }
-    const float inv = 127.0f / topf;
-    const uint32_t keep = none ? 0u : ~0u;
-    u2* out = codes + row * chunks;
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-        const int c = 64 * (W * j + wave) + lane;
-        if (c >= chunks) continue;
-        if constexpr (ADD) rr[c] = values_chunk<BF16>(s[j]);
-        float n[8], far = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float v = tf(j, i) * inv;
-            n[i] = v + kMagic;
-            far = fmaxf(far, fabsf(v - (n[i] - kMagic)));
-        }
-        if (far > kBorder && !none) {
-            float g[8];
-            if constexpr (NORM) chunk_values<BF16>(wv[j], g);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float v = tf(j, i) * inv;
-                if (fabsf(v - (n[i] - kMagic)) > kBorder)
-                    n[i] = border_code(v, static_cast<double>(s[j][i]) * (NORM ? static_cast<double>(g[i]) : 1.0), top) + kMagic;
-            }
-        }
-        uint32_t q[2];  // the codes are the lowest bytes
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(n[4 * h + 1]), __float_as_uint(n[4 * h]), 0x0C0C0400);
-            const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(n[4 * h + 3]), __float_as_uint(n[4 * h + 2]), 0x04000C0C);
-            q[h] = (lo | hi) & keep;
-        }
-        out[c] = u2{q[0], q[1]};
-    }
+    Row8Loads<J> loads;
+    row8_load<NORM, ADD, W, J>(loads, x + row * x_step, r + row * r_step, w, chunks, wave, lane);
+    row8_quantize<NORM, ADD, BF16, W, J>(loads, shared, r + row * r_step, codes + row * chunks, scales + row, eps, chunks, wave, lane);
 }
 
 struct RowsArgs {

@@ -87,6 +87,7 @@ _SIGNATURES = {
     "tw4_quantize_int8": ([_P, _I64, _P, _P, _I, _I, _I, _P], _I),
     "tw4_rms_norm_int8": ([_P, _I64, _P, _I64, _P, ctypes.c_float, _P, _P, _I, _I, _I, _P], _I),
     "tw4_gemm_int8": ([_P, _I64, _P, _P, _I64, _P, _P, _P, _I64, _P, _I64, _I, _I, _I, _I, _I, _I, _I, _P], _I),
+    "tw4_token_int8": ([_P, _P, _P, _P, ctypes.c_float, _P, _I64, _P, _P, _I, _I, _I, _I, _I, _P], _I),
     "tw4_gemm_int8_plan": ([_I] * 5 + [ctypes.POINTER(_I)], _I),
 }
 

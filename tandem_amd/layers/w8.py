@@ -42,6 +42,7 @@ def quantize_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     return codes, scales
 
 
+@functools.lru_cache(maxsize=None)
 def _cus(index: int) -> int:
     return torch.cuda.get_device_properties(index).multi_processor_count
 
@@ -101,6 +102,41 @@ def linear_int8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, we
     return y
 
 
+MAX_TOKEN_K = 16384
+
+
+# As _checked. x's own stride is no matter: it is one row.
+@functools.lru_cache(maxsize=1 << 14)
+def _checked_token(x: tuple, residual: tuple | None, norm_weight: tuple | None, weight: tuple, weight_scale: tuple,
+                   silu_mul: bool) -> tuple:
+    """((N, K, act, type code, CUs), row stride of the weight, output features, GPU)."""
+    _, _, _, k, code, index = norm.check_rows("token_int8", x, residual, norm_weight)
+    one = ((1, k), (k, 1), torch.int8, index), ((1,), (1,), torch.float32, index)
+    _, w_step, (_, n, k, act, *_), _, features, _ = _checked(*one, weight, weight_scale, silu_mul, x[2])
+    return (n, k, act, code, _cus(index)), w_step, features, index
+
+
+def _token_int8(x: torch.Tensor, residual: torch.Tensor | None, norm_weight: torch.Tensor | None, eps: float, weight: torch.Tensor,
+                weight_scale: torch.Tensor, silu_mul: bool) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """linear_int8 of one row x [1, K] in 8 bits, K <= MAX_TOKEN_K, in one kernel: quantize_int8's codes, or with norm_weight rms_norm_int8's,
+    or with residual fused_add_rms_norm_int8's -> (y, x + residual in new memory). The bits of the two calls (tw4_token_int8)."""
+    sizes, w_step, features, index = _checked_token(layout(x), None if residual is None else layout(residual),
+                                                    None if norm_weight is None else layout(norm_weight), layout(weight),
+                                                    layout(weight_scale), silu_mul)
+    if not (w4_hip.all_plain(x, weight, weight_scale) if residual is None else w4_hip.all_plain(x, residual, weight, weight_scale)):
+        raise RuntimeError("token_int8: inference only, no gradient, transform or tracer can follow the operands")
+    y, total = x.new_empty(1, features), None if residual is None else x.new_empty(1, sizes[1])
+    xp, wp = x.data_ptr(), weight.data_ptr()
+    rp, tp = (0, 0) if residual is None else (residual.data_ptr(), total.data_ptr())
+    gp = 0 if norm_weight is None else norm_weight.data_ptr()
+    if (xp | wp | rp | gp) % 16:
+        raise RuntimeError("token_int8: x, the residual and the weights must be 16-byte aligned")
+    with w4_hip.on_device(index):
+        w4_hip.check(w4_hip.library().tw4_token_int8(xp, rp, tp, gp, eps, wp, w_step, weight_scale.data_ptr(), y.data_ptr(), *sizes,
+                                                     w4_hip.raw_stream(index)))
+    return y, total
+
+
 class W8Linear(nn.Module):
     """y = x @ W^T for a bias-free projection of an int8 checkpoint: ``weight`` int8 [N, K] and ``weight_scale`` float32 [N, 1], as
     such checkpoints store them (a fused qkv or gate_up holds its parts one behind the other). x is quantised token by token on
@@ -129,19 +165,30 @@ class W8Linear(nn.Module):
         self.silu_mul = self.out_features % 2 == 0
         return self.silu_mul
 
+    def _one_token(self, x: torch.Tensor) -> bool:
+        """Whether x's codes are made inside the product's kernel: one row, with as many outputs as one workgroup for each CU holds. Measured
+        on both sides in csrc/tw4_gemm8.hip."""
+        outputs, each = (self.out_features // 2, 16) if self.silu_mul else (self.out_features, 32)
+        return x.shape[0] == 1 and self.in_features <= MAX_TOKEN_K and x.is_cuda and outputs <= each * _cus(x.get_device())
+
     def _product(self, codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
         return linear_int8(codes, scales, self.weight, self.weight_scale, silu_mul=self.silu_mul, dtype=dtype)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        if x.dim() == 2:
-            return self._product(*quantize_int8(x), x.dtype)
-        y = self._product(*quantize_int8(x.reshape(-1, self.in_features)), x.dtype)
-        return y.view(*x.shape[:-1], y.shape[-1])
+        if x.dim() != 2:
+            y = self(x.reshape(-1, self.in_features))
+            return y.view(*x.shape[:-1], y.shape[-1])
+        if self._one_token(x):
+            return _token_int8(x, None, None, 0.0, self.weight, self.weight_scale, self.silu_mul)[0]
+        return self._product(*quantize_int8(x), x.dtype)
 
     def forward_norm(self, x: torch.Tensor, residual: torch.Tensor | None, norm_weight: torch.Tensor,
                      eps: float) -> tuple[torch.Tensor, torch.Tensor]:
-        """self(rms_norm(x + residual) * norm_weight), the norm's output in 8 bits as it is written, and the new residual (x itself
-        without one; else in place)."""
+        """self(rms_norm(x + residual) * norm_weight), the norm's output in 8 bits as it is written, and the new residual (x itself without
+        one). residual is consumed, as W4Linear's: one token gets the new one in fresh memory, more have it written in place."""
+        if x.dim() == 2 and self._one_token(x):
+            y, total = _token_int8(x, residual, norm_weight, eps, self.weight, self.weight_scale, self.silu_mul)
+            return y, x if residual is None else total
         if residual is None:
             return self._product(*norm.rms_norm_int8(x, norm_weight, eps), x.dtype), x
         codes, scales, residual = norm.fused_add_rms_norm_int8(x, residual, norm_weight, eps)

@@ -28,7 +28,7 @@ the model to the GPU, repacks the W4 layers and routes the fp16 projections and 
 through layers/gemv16.py's table. Norms run on tw4_rms_norm / tw4_add_rms_norm, or inside the W4
 qkv_proj / gate_up_proj kernels where W4Linear.forward_norm fuses them (the decode GEMV at the
 batch sizes it runs: a norm kernel fewer before each, the same bits). A W8Linear's come out of the norm in 8 bits
-(tw4_rms_norm_int8).
+(tw4_rms_norm_int8), or for one token inside the projection's kernel (tw4_token_int8).
 """
 
 from __future__ import annotations

@@ -56,6 +56,30 @@ def test_argument_errors_return_before_launch():
         assert needle in lib.tw4_last_error().decode(), (change, lib.tw4_last_error())
 
 
+def test_token_argument_errors_return_before_launch():
+    lib, p, odd, own = w4_hip.library(), ctypes.c_void_p(4096), ctypes.c_void_p(4104), ctypes.c_void_p(8192)
+    #       x residual new weight eps w stride ws y N K act bf16 cus
+    good = [p, p, own, p, 1e-6, p, 64, p, p, 6, 64, 0, 0, 256]
+    for at, value, needle in ((0, None, "null"), (5, None, "null"), (7, None, "null"), (8, None, "null"), (0, odd, "aligned"), (1, odd, "aligned"),
+                              (2, odd, "aligned"), (3, odd, "aligned"), (5, odd, "aligned"), (7, ctypes.c_void_p(4098), "aligned"),
+                              (8, ctypes.c_void_p(4097), "aligned"), (1, None, "residual"), (2, None, "residual"), (3, None, "residual"),
+                              (2, p, "its own"), (6, 48, "apart"), (6, 72, "apart"), (6, 1 << 22, "apart"), (9, 0, "N"), (9, (1 << 24) + 1, "N"),
+                              (10, 72, "K"), (10, 0, "K"), (10, 16400, "K"), (11, 2, "act"), (13, 0, "cus")):
+        args = list(good)
+        args[at] = value
+        if at == 10 and value:
+            args[6] = 1 << 15
+        assert lib.tw4_token_int8(*args, None) == w4_hip.TW4_EINVAL, (at, value)
+        assert needle in lib.tw4_last_error().decode(), (at, lib.tw4_last_error())
+    for n, act, cus in ((32 * 7 + 1, 0, 7), (2 * (16 * 7 + 1), 1, 7), (1 << 24, 0, 256)):
+        args = list(good)
+        args[9], args[11], args[13] = n, act, cus
+        assert lib.tw4_token_int8(*args, None) == w4_hip.TW4_ECONFIG and "CU" in lib.tw4_last_error().decode()
+    args = list(good)
+    args[9], args[11] = 5, 1
+    assert lib.tw4_token_int8(*args, None) == w4_hip.TW4_EINVAL and "even" in lib.tw4_last_error().decode()
+
+
 def _plan(m, n, k, act, cus=256):
     out = (ctypes.c_int * 4)()
     w4_hip.check(w4_hip.library().tw4_gemm_int8_plan(m, n, k, act, cus, out))
@@ -324,7 +348,7 @@ def test_streams_and_graphs():
                 graph.replay()
                 step(xs[i], rs[i].clone())
                 torch.cuda.synchronize()
-                assert torch.equal(out[0], want[at][0]) and torch.equal(gr, want[at][1])
+                assert torch.equal(out[0], want[at][0]) and torch.equal(out[1], want[at][1])
 
 
 @pytest.mark.gpu
@@ -349,3 +373,87 @@ def test_layer_shapes_and_norm():
         y, out = layer.forward_norm(x, r2, weight, 1e-6)
         assert out is r2 and torch.equal(r2, r3) and torch.equal(y, w8.linear_int8(codes, scales, w, ws, silu_mul=silu_mul))
     assert tmodel.GatedMLP(512, 256, INT8).fused_act
+
+
+def _pair(x, residual, weight, w, ws, silu_mul):
+    """What one token's kernel does, with the operators it stands for: (y, new residual)."""
+    if weight is None:
+        codes, scales = w8.quantize_int8(x)
+    elif residual is None:
+        codes, scales = norm.rms_norm_int8(x, weight, 1e-6)
+    else:
+        codes, scales, residual = norm.fused_add_rms_norm_int8(x, residual.clone(), weight, 1e-6)
+    return w8.linear_int8(codes, scales, w, ws, silu_mul=silu_mul, dtype=x.dtype), residual
+
+
+def _same_bits(a, b):
+    return torch.equal(a.view(torch.int16), b.view(torch.int16))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n,k", [(2, 16), (34, 48), (130, 1040), (333, 2576), (1024, 8192), (2502, 8208), (6128, 4096), (8192, 272), (96, 16384)])
+def test_one_token(n, k, dtype):
+    """W8Linear's one row, made in 8 bits inside the product's kernel: the bits of the operators one behind the other, rows of w any multiple
+    of 16 apart, x and the residual as they were, nothing written beside y."""
+    g = torch.Generator(device="cuda").manual_seed(n + k)
+    step = k + 48
+    w = torch.randint(-128, 128, (n, step), device="cuda", dtype=torch.int8, generator=g)[:, :k]
+    ws = (0.5 + torch.rand(n, device="cuda", generator=g)) * 0.02 * k ** -0.5
+    weight = (0.5 + torch.rand(k, device="cuda", generator=g)).to(dtype)
+    rows = torch.randn(6, k, device="cuda", generator=g).to(dtype)
+    rows[1, k // 2], rows[2, 0], rows[3] = float("inf"), float("nan"), 0
+    rows[4] *= 2.0 ** -9
+    residual = torch.randn(1, k, device="cuda", generator=g).to(dtype)
+    for silu_mul in ((False,) if n % 2 else (False, True)):
+        for i in range(6):
+            x, before, r = rows[i:i + 1], rows[i].clone(), residual.clone()
+            for args in ((None, None), (None, weight), (r, weight)):
+                y, total = w8._token_int8(x, args[0], args[1], 1e-6, w, ws, silu_mul)
+                want, want_r = _pair(x, *args, w, ws, silu_mul)
+                assert y.shape == want.shape and _same_bits(y, want), (i, silu_mul)
+                assert (total is None) == (args[0] is None) and (total is None or _same_bits(total, want_r))
+            assert _same_bits(rows[i], before) and torch.equal(r, residual)
+        out = n // 2 if silu_mul else n
+        y, total = torch.full((out + 64,), 3.0, device="cuda", dtype=dtype), torch.full((k + 64,), 3.0, device="cuda", dtype=dtype)
+        w4_hip.check(w4_hip.library().tw4_token_int8(
+            rows[0].data_ptr(), residual.data_ptr(), total.data_ptr(), weight.data_ptr(), 1e-6, w.data_ptr(), step, ws.data_ptr(),
+            y.data_ptr(), n, k, int(silu_mul), int(dtype == torch.bfloat16), 256, w4_hip.raw_stream(0)))
+        want, want_r = _pair(rows[:1], residual, weight, w, ws, silu_mul)
+        assert _same_bits(y[:out], want[0]) and _same_bits(total[:k], want_r[0])
+        assert bool((y[out:] == 3).all()) and bool((total[k:] == 3).all())
+
+
+@pytest.mark.gpu
+def test_one_token_layers():
+    """Which W8Linear calls take it, and that every one of them has the bits of the same row in a batch: outputs on both sides of one
+    workgroup a CU, K on both sides of its longest, one row of more than two dimensions, a row of odd stride."""
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+    for n, k, silu_mul, one in ((32 * cus, 64, False, True), (32 * cus + 2, 64, False, False), (32 * cus, 64, True, True),
+                                (32 * cus + 2, 64, True, False), (64, 16384, False, True), (64, 16400, False, False)):
+        layer = w8.W8Linear(k, n).cuda()
+        _, _, w, ws = _operands(1, n, k, seed=n + k)
+        layer.weight.copy_(w)
+        layer.weight_scale.copy_(ws[:, None])
+        layer.silu_mul = silu_mul
+        x, r = torch.randn(3, k, device="cuda").half(), torch.randn(3, k, device="cuda").half()
+        weight = (0.5 + torch.rand(k, device="cuda")).half()
+        assert layer._one_token(x[:1]) == one and not layer._one_token(x) and not layer._one_token(x[:0])
+        y, normed = layer(x), layer.forward_norm(x, None, weight, 1e-6)[0]
+        both, total = layer.forward_norm(x, r.clone(), weight, 1e-6)
+        for i in range(3):
+            assert torch.equal(layer(x[i:i + 1]), y[i:i + 1]) and torch.equal(layer(x[i].view(1, 1, k)), y[i].view(1, 1, -1))
+            got, same = layer.forward_norm(x[i:i + 1], None, weight, 1e-6)
+            assert torch.equal(got, normed[i:i + 1]) and same.data_ptr() == x[i].data_ptr()
+            got, out = layer.forward_norm(x[i:i + 1], r[i:i + 1].clone(), weight, 1e-6)
+            assert torch.equal(got, both[i:i + 1]) and torch.equal(out, total[i:i + 1])
+        odd = x[0].as_strided((1, k), (k + 1, 1))
+        assert torch.equal(layer(odd), y[:1])
+    layer = w8.W8Linear(64, 32).cuda()
+    x = torch.zeros(1, 64, device="cuda").half()
+    for bad in (x.float(), torch.zeros(1, 80, device="cuda").half(), torch.zeros(1, 72, device="cuda").half()[:, 4:68],
+                torch.zeros(64, 2, device="cuda").half().t()[:1], x.clone().requires_grad_()):
+        with pytest.raises(RuntimeError):
+            layer(bad)
+    with pytest.raises(RuntimeError, match="residual"):
+        layer.forward_norm(x, x.bfloat16(), torch.ones(64, device="cuda").half(), 1e-6)
