@@ -392,7 +392,7 @@ int tw4_gemm_int8(const int8_t* x, int64_t x_stride, const float* x_scale, const
 int tw4_gemm_int8_plan(int M, int N, int K, int act, int cus, int* out);
 
 /* One token's projection in one kernel: x [K] of fp16 (bf16 = 1: bfloat16) put in 8 bits as tw4_quantize_int8 does (norm_weight NULL) or
- * tw4_rms_norm_int8 (with residual [K]: of x + residual, which goes to residual_out, rounded; not in place), then tw4_gemm_int8's product
+ * tw4_rms_norm_int8 (with residual [K]: of x + residual, which goes to residual_out, rounded; neither x's memory nor residual's), then tw4_gemm_int8's product
  * with w [N, K] (act = 1: SwiGLU) -> y [N] or [N / 2]: the same bits as the two one behind the other. K <= TW4_TOKEN_INT8_MAX; cus: the
  * device's CUs, and at most 32 outputs (16 with act = 1) for each of them. No reference counterpart. */
 #define TW4_TOKEN_INT8_MAX 16384

@@ -343,7 +343,7 @@ extern "C" int tw4_token_int8(const uint16_t* x, const uint16_t* residual, uint1
                 "token_int8: scales must be 4-byte aligned and y 2-byte");
     TW4_REQUIRE(!residual == !residual_out && (!residual || norm_weight), TW4_EINVAL,
                 "token_int8: a residual comes with a norm weight and memory for the new one");
-    TW4_REQUIRE(residual_out != residual || !residual, TW4_EINVAL, "token_int8: the new residual needs memory of its own");
+    TW4_REQUIRE(!residual || (residual_out != residual && residual_out != x), TW4_EINVAL, "token_int8: the new residual needs memory of its own");
     const int rc = gemm8_check_sizes(1, N, K, act);
     if (rc) return rc;
     TW4_REQUIRE(K <= TW4_TOKEN_INT8_MAX, TW4_EINVAL, "token_int8: K <= %d (K = %d)", TW4_TOKEN_INT8_MAX, K);

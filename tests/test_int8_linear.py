@@ -63,7 +63,7 @@ def test_token_argument_errors_return_before_launch():
     for at, value, needle in ((0, None, "null"), (5, None, "null"), (7, None, "null"), (8, None, "null"), (0, odd, "aligned"), (1, odd, "aligned"),
                               (2, odd, "aligned"), (3, odd, "aligned"), (5, odd, "aligned"), (7, ctypes.c_void_p(4098), "aligned"),
                               (8, ctypes.c_void_p(4097), "aligned"), (1, None, "residual"), (2, None, "residual"), (3, None, "residual"),
-                              (2, p, "its own"), (6, 48, "apart"), (6, 72, "apart"), (6, 1 << 22, "apart"), (9, 0, "N"), (9, (1 << 24) + 1, "N"),
+                              (2, p, "its own"), (0, own, "its own"), (1, own, "its own"), (6, 48, "apart"), (6, 72, "apart"), (6, 1 << 22, "apart"), (9, 0, "N"), (9, (1 << 24) + 1, "N"),
                               (10, 72, "K"), (10, 0, "K"), (10, 16400, "K"), (11, 2, "act"), (13, 0, "cus")):
         args = list(good)
         args[at] = value
