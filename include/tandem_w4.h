@@ -371,7 +371,8 @@ int tw4_quantize_int8(const uint16_t* x, int64_t x_stride, int8_t* codes, float*
 
 /* tw4_rms_norm (residual NULL) or tw4_add_rms_norm (residual <- the type's rounding of s = x + residual, x is left as it is) with
  * its output y = s rsqrt(mean(s^2) + eps) weight, unrounded, in 8-bit integers: scale = max|y| / 127, code = 127 t / max|t| rounded as in
- * tw4_quantize_int8, t = s weight, of whose exact values the codes are exactly rounded. Infinities, NaN and small rows as there, by t. */
+ * tw4_quantize_int8, t = s weight, of whose exact values the codes are exactly rounded. Infinities, NaN and small rows as there, by t;
+ * scale NaN too where the sum of squares leaves float32. */
 int tw4_rms_norm_int8(const uint16_t* x, int64_t x_stride, uint16_t* residual, int64_t r_stride, const uint16_t* weight,
                       float eps, int8_t* codes, float* scales, int M, int K, int bf16, void* stream);
 

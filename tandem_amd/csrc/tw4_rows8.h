@@ -130,7 +130,8 @@ __device__ __forceinline__ void row8_quantize(const Row8Loads<J>& loads, Row8Sha
     const bool nan = !(topf < __builtin_inff()), none = nan || topf < kLeast;
     if (wave == 0) {  // rstd in the order of the other norms: the same bits whatever W and J
         const float rstd = NORM ? norm_rstd(sh.group_of, (chunks + 15) / 16, 8 * chunks, eps, lane) : 1.0f;
-        if (lane == 0) *scale = nan ? __builtin_nanf("") : none ? 0.0f : topf * rstd / 127.0f;
+        const bool lost = !(rstd > 0.0f && rstd < __builtin_inff());  // the squares' sum has left float32's range: not a scale of 0
+        if (lane == 0) *scale = nan || (lost && !none) ? __builtin_nanf("") : none ? 0.0f : topf * rstd / 127.0f;
     }
     const float inv = 127.0f / topf;
     const uint32_t keep = none ? 0u : ~0u;

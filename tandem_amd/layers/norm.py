@@ -132,7 +132,8 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float) -> tuple[to
     common to a row, so code = 127 t / max|t| with t = x * weight, and is exactly that, rounded to nearest, halves to even.
 
     A row that holds an infinity or a NaN (in x, the weight, or their product in float32) has scale NaN and codes 0, so that
-    its products are NaN; one with every |t| below 2^-100 has scale 0 and codes 0. Inference only."""
+    its products are NaN; one with every |t| below 2^-100 has scale 0 and codes 0. One whose sum of squares leaves float32 (bfloat16
+    from about 10^18 on; with eps 0, all below 10^-22) has scale NaN too. Inference only."""
     return _rms_norm_int8("rms_norm_int8", x, None, weight, eps)
 
 

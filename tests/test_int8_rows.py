@@ -211,6 +211,26 @@ def test_special_rows(k, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("k", [16, 528, 4096, 16384])
+def test_squares_past_float32(k):
+    """A norm whose sum of squares float32 does not hold has scale NaN, never 0; next to it, k squares of 2^(126 / 2) / sqrt(k), it is right."""
+    x, w = torch.ones(5, k, device="cuda", dtype=torch.bfloat16), torch.ones(k, device="cuda", dtype=torch.bfloat16)
+    x[0] *= 2.0 ** 65
+    x[1, k // 2] = -2.0 ** 100
+    x[2] *= 2.0 ** 63 * k ** -0.5
+    x[3] *= 2.0 ** -90
+    codes, scales = norm.rms_norm_int8(x, w, 0.0)
+    assert bool(scales[[0, 1, 3]].isnan().all())  # row 3: its squares are 0 and so is eps
+    assert bool((codes[[2, 4]] == 127).all())
+    assert bool(((scales[[2, 4]].double() * 127 - 1).abs() <= 36 * STEP).all())  # equal values: the norm is 1
+    codes, scales = norm.rms_norm_int8(x, w, EPS)
+    want = 2.0 ** -90 * EPS ** -0.5 / 127
+    assert abs(float(scales[3].double()) / want - 1) <= 36 * STEP and bool((codes[3] == 127).all())
+    y, _ = w8._token_int8(x[:1], None, w, EPS, torch.ones(4, k, device="cuda", dtype=torch.int8), torch.ones(4, device="cuda"), False)
+    assert bool(y.isnan().all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_strides_and_shared_buffers(dtype):
     """Rows inside wider ones; x and the residual beside each other in one buffer; what lies around them is left alone."""
