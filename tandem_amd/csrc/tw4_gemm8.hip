@@ -175,9 +175,12 @@ __global__ void __launch_bounds__(64 * kStreamWaves) token8_kernel(const u4* __r
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         if (at + i >= rows) break;
-        float v = static_cast<float>(sum[i]) * x_scale * w_scale[n + i];
-        if constexpr (ACT) v = silu_rcp(v) * (static_cast<float>(up[i]) * x_scale * w_scale[out + n + i]);
-        y[n + i] = static_cast<uint16_t>(value16<BF16>(v));
+        float v[1] = {static_cast<float>(sum[i]) * x_scale * w_scale[n + i]};
+        if constexpr (ACT) {
+            silu_values(v);
+            v[0] *= static_cast<float>(up[i]) * x_scale * w_scale[out + n + i];
+        }
+        y[n + i] = static_cast<uint16_t>(value16<BF16>(v[0]));
     }
 }
 

@@ -319,8 +319,9 @@ gemm8_lds_kernel(const int8_t* __restrict__ x, uint32_t x_stride, const float* _
         for (int i = 0; i < 4; ++i) v[i] = static_cast<float>(acc[t][b][i]) * xs * s[i];
         if constexpr (ACT) {
             const f4 u = *reinterpret_cast<const f4*>(scales + 16 * (TM + TILES + t) + 4 * q);
+            silu_values(v);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = silu_rcp(v[i]) * (static_cast<float>(acc[t + TILES][b][i]) * xs * u[i]);
+            for (int i = 0; i < 4; ++i) v[i] *= static_cast<float>(acc[t + TILES][b][i]) * xs * u[i];
         }
     };
     // Results go through LDS, so that a store instruction writes whole rows of the wavefront's features: 8 values a lane where rows are

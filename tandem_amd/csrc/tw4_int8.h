@@ -40,9 +40,33 @@ __device__ __forceinline__ u4 values_chunk(const float (&f)[8]) {
     return v;
 }
 
-// g / (1 + exp(-g)) by the reciprocal instruction (1 ulp; -0 from where exp(-g) passes 2^126, g < -87): a division takes ten
-// instructions. K 4096 x N 24576: M = 512 57.3 -> 55.9 us, 2048 191 -> 185; level at 8192, which the card's power bounds.
+// g / (1 + exp(-g)) by the reciprocal instruction (1 ulp), for g >= kSiluFar or NaN: a division takes ten instructions. K 4096 x N 24576:
+// M = 512 57.3 -> 55.9 us, 2048 191 -> 185; level at 8192, which the card's power bounds.
 __device__ __forceinline__ float silu_rcp(float g) { return g * __builtin_amdgcn_rcpf(1.0f + __expf(-g)); }
+
+// Below kSiluFar exp(-g) comes to pass 2^126, whose reciprocal that instruction flushes to 0, and float32 later on. 1 + exp(-g) is exp(-g) there, and g exp(g)
+// = (g exp(g / 2)) exp(g / 2) rounds once more than it has to, and to subnormal numbers only in its last product.
+constexpr float kSiluFar = -87.0f;
+__device__ __forceinline__ float silu_far(float g) {
+    const float e = __expf(0.5f * g);
+    return g * e * e;
+}
+
+// g[i] becomes silu(g[i]). Gates that far out are few or none: a wavefront without one jumps over their form (K 2560 x N 19456, M = 200 18.1 -> 18.4 us
+// for the look; M = 5 and 8192 level).
+template <int N>
+__device__ __forceinline__ void silu_values(float (&g)[N]) {
+    float least = g[0], s[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) least = fminf(least, g[i]), s[i] = silu_rcp(g[i]);
+    if (__builtin_expect(__ballot(least < kSiluFar) != 0, 0)) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (g[i] < kSiluFar) s[i] = silu_far(g[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) g[i] = s[i];
+}
 
 // D += A B on v_mfma_i32_16x16x64_i8: lane (q, r) = (lane / 16, lane % 16) gives row r of A and column r of B, 16 bytes each, at
 // the same 16 of the 64 k for both, and holds rows 4 q + i of column r of D. The sums are exact (K < 2^17).
