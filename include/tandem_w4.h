@@ -380,7 +380,8 @@ int tw4_rms_norm_int8(const uint16_t* x, int64_t x_stride, uint16_t* residual, i
  * x_stride and w_stride bytes apart (16-byte aligned, less than 2^22 apart), x_scale float32 [M], w_scale float32 [N]; y of fp16 (bf16 = 1:
  * bfloat16), rounded once. act = 1: w's rows are [gate | up] (N even) and y [M, N / 2] = silu(gate) up. K % 16 == 0, K < 2^17 (the sum
  * is exact in 32 bits), M <= 2^20, N <= 2^24. kernel, splits: from tw4_gemm_int8_plan; any kernel 0 .. TW4_GEMM_INT8_KERNELS - 1 gives the
- * same bits (0: act = 0, M <= 2^20 - 16; 1, 2: M <= 16), with 1 .. ceil(K / 128) K splits (kernel 0: 1 .. 32 rows of w per workgroup instead).
+ * same bits (0: act = 0, M <= 2^20 - 16; 1, 2: M <= 16), with 1 .. ceil(K / 128) K splits (kernel 0: 1 .. 32 rows of w per
+ * workgroup instead, in fewer than 2^22 workgroups).
  * More than one split takes ws and locks (zero before the first call, and after each; calls that share them must not overlap),
  * TW4_ESPACE if they are too small. No reference counterpart. */
 #define TW4_GEMM_INT8_KERNELS 13

@@ -230,6 +230,7 @@ int gemm8_stream(const Gemm8Args& a, int rows) {
     TW4_REQUIRE(!a.act, TW4_ECONFIG, "gemm_int8: no SwiGLU in the streaming kernel");
     const dim3 grid(static_cast<unsigned>((a.N + rows - 1) / rows), static_cast<unsigned>((a.M + 15) / 16));
     TW4_REQUIRE(grid.y < 1 << 16, TW4_ECONFIG, "gemm_int8: M <= 2^20 - 16 for the streaming kernel (M %d)", a.M);
+    TW4_REQUIRE(grid.x * (64LL * kStreamWaves) < 1LL << 32, TW4_ECONFIG, "gemm_int8: N = %d is too many rows of w for %d a workgroup", a.N, rows);
     const auto kernel = rows <= 16 ? (a.bf16 ? gemm8_stream_kernel<1, true> : gemm8_stream_kernel<1, false>)
                                    : (a.bf16 ? gemm8_stream_kernel<2, true> : gemm8_stream_kernel<2, false>);
     kernel<<<grid, 64 * kStreamWaves, 0, a.st>>>(a.x, static_cast<uint32_t>(a.x_stride), a.x_scale, a.w, static_cast<uint32_t>(a.w_stride),

@@ -29,6 +29,12 @@ def test_tokens_of_the_streaming_kernel(m):
     _refused(_product(m, 1, 16, 4), w4_hip.TW4_ECONFIG, "M <= 2^20 - 16")
 
 
+@pytest.mark.parametrize("n,rows", [(1 << 22, 1), (1 << 24, 1), (1 << 24, 4)])
+def test_workgroups_of_the_streaming_kernel(n, rows):
+    """2^22 workgroups of 1024 threads are past what a launch holds."""
+    _refused(_product(1, n, 16, rows), w4_hip.TW4_ECONFIG, "too many rows")
+
+
 # ------------------------------------------------------------------------------------------- GPU
 def _ones(*shape):
     return torch.ones(*shape, device="cuda")
@@ -41,5 +47,16 @@ def test_most_tokens_of_the_streaming_kernel():
     w = (torch.arange(n * k, device="cuda") % 7 - 3).to(torch.int8).view(n, k)
     xs, ws, y = _ones(m), _ones(n), torch.empty(m, n, dtype=torch.float16, device="cuda")
     w4_hip.check(_product(m, n, k, 4, *(t.data_ptr() for t in (x, xs, w, ws, y))))
+    torch.cuda.synchronize()
+    assert torch.equal(y.float(), torch.matmul(x.float(), w.float().t()).half().float())
+
+
+@pytest.mark.gpu
+def test_most_workgroups_of_the_streaming_kernel():
+    m, n, k = 1, (1 << 22) - 1, 16
+    x = (torch.arange(m * k, device="cuda") % 7 - 3).to(torch.int8).view(m, k)
+    w = (torch.arange(n * k, device="cuda") % 251 - 125).to(torch.int8).view(n, k)
+    xs, ws, y = _ones(m), _ones(n), torch.empty(m, n, dtype=torch.float16, device="cuda")
+    w4_hip.check(_product(m, n, k, 1, *(t.data_ptr() for t in (x, xs, w, ws, y))))
     torch.cuda.synchronize()
     assert torch.equal(y.float(), torch.matmul(x.float(), w.float().t()).half().float())
