@@ -372,7 +372,8 @@ int tw4_quantize_int8(const uint16_t* x, int64_t x_stride, int8_t* codes, float*
 /* tw4_rms_norm (residual NULL) or tw4_add_rms_norm (residual <- the type's rounding of s = x + residual, x is left as it is) with
  * its output y = s rsqrt(mean(s^2) + eps) weight, unrounded, in 8-bit integers: scale = max|y| / 127, code = 127 t / max|t| rounded as in
  * tw4_quantize_int8, t = s weight, of whose exact values the codes are exactly rounded. Infinities, NaN and small rows as there, by t;
- * scale NaN too where the sum of squares leaves float32. */
+ * scale NaN too where the sum of squares leaves float32. x and the residual share no byte (rows of one may lie between the other's, if
+ * both are as far apart): TW4_EINVAL. Codes, scales and the weight are memory of their own in all these calls. */
 int tw4_rms_norm_int8(const uint16_t* x, int64_t x_stride, uint16_t* residual, int64_t r_stride, const uint16_t* weight,
                       float eps, int8_t* codes, float* scales, int M, int K, int bf16, void* stream);
 
@@ -394,9 +395,10 @@ int tw4_gemm_int8(const int8_t* x, int64_t x_stride, const float* x_scale, const
 int tw4_gemm_int8_plan(int M, int N, int K, int act, int cus, int* out);
 
 /* One token's projection in one kernel: x [K] of fp16 (bf16 = 1: bfloat16) put in 8 bits as tw4_quantize_int8 does (norm_weight NULL) or
- * tw4_rms_norm_int8 (with residual [K]: of x + residual, which goes to residual_out, rounded; neither x's memory nor residual's), then tw4_gemm_int8's product
- * with w [N, K] (act = 1: SwiGLU) -> y [N] or [N / 2]: the same bits as the two one behind the other. K <= TW4_TOKEN_INT8_MAX; cus: the
- * device's CUs, and at most 32 outputs (16 with act = 1) for each of them. No reference counterpart. */
+ * tw4_rms_norm_int8 (with residual [K]: of x + residual, which goes to residual_out, rounded), then tw4_gemm_int8's product
+ * with w [N, K] (act = 1: SwiGLU) -> y [N] or [N / 2]: the same bits as the two one behind the other. residual_out and y share no byte
+ * with x, the residual, norm_weight or each other: TW4_EINVAL. K <= TW4_TOKEN_INT8_MAX; cus: the device's CUs, and at most 32 outputs
+ * (16 with act = 1) for each of them. No reference counterpart. */
 #define TW4_TOKEN_INT8_MAX 16384
 int tw4_token_int8(const uint16_t* x, const uint16_t* residual, uint16_t* residual_out, const uint16_t* norm_weight, float eps,
                    const int8_t* w, int64_t w_stride, const float* w_scale, uint16_t* y, int N, int K, int act, int bf16, int cus,

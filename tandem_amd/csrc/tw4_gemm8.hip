@@ -347,7 +347,6 @@ extern "C" int tw4_token_int8(const uint16_t* x, const uint16_t* residual, uint1
                 "token_int8: scales must be 4-byte aligned and y 2-byte");
     TW4_REQUIRE(!residual == !residual_out && (!residual || norm_weight), TW4_EINVAL,
                 "token_int8: a residual comes with a norm weight and memory for the new one");
-    TW4_REQUIRE(!residual || (residual_out != residual && residual_out != x), TW4_EINVAL, "token_int8: the new residual needs memory of its own");
     const int rc = gemm8_check_sizes(1, N, K, act);
     if (rc) return rc;
     TW4_REQUIRE(K <= TW4_TOKEN_INT8_MAX, TW4_EINVAL, "token_int8: K <= %d (K = %d)", TW4_TOKEN_INT8_MAX, K);
@@ -357,6 +356,11 @@ extern "C" int tw4_token_int8(const uint16_t* x, const uint16_t* residual, uint1
     const int out = act ? N / 2 : N, rows = stream8_rows(out, cus);
     TW4_REQUIRE((out + rows - 1) / rows <= cus && rows <= (act ? 16 : 32), TW4_ECONFIG,
                 "token_int8: at most 32 outputs, or 16 of SwiGLU, a CU (%d outputs, %d CUs)", out, cus);
+    const int64_t row = 2LL * K;  // bytes; some workgroups write while others still read
+    for (const uint16_t* p : {x, residual, norm_weight})
+        TW4_REQUIRE(!p || !residual_out || bytes_apart(p, row, residual_out, row), TW4_EINVAL, "token_int8: the new residual needs memory of its own");
+    for (const uint16_t* p : {x, residual, norm_weight, static_cast<const uint16_t*>(residual_out)})
+        TW4_REQUIRE(!p || bytes_apart(p, row, y, 2LL * out), TW4_EINVAL, "token_int8: y needs memory of its own");
     const Token8Args a{reinterpret_cast<const u4*>(x), reinterpret_cast<const u4*>(residual), reinterpret_cast<u4*>(residual_out),
                        reinterpret_cast<const u4*>(norm_weight), eps, w, static_cast<uint32_t>(w_stride), w_scale, y, N, K, rows,
                        static_cast<hipStream_t>(stream)};

@@ -89,6 +89,19 @@ __device__ __forceinline__ void store_features(uint16_t* row, int n, int N, bool
     }
 }
 
+// Whether so many bytes from a and from b on are apart (host).
+inline bool bytes_apart(const void* a, int64_t bytes_a, const void* b, int64_t bytes_b) {
+    return static_cast<const char*>(a) + bytes_a <= b || static_cast<const char*>(b) + bytes_b <= a;
+}
+
+// Whether rows of `width` bytes from a and b on, so many bytes apart, share no byte (host).
+inline bool rows_apart(const void* a, int64_t step_a, const void* b, int64_t step_b, int64_t rows, int64_t width) {
+    if (bytes_apart(a, (rows - 1) * step_a + width, b, (rows - 1) * step_b + width)) return true;
+    const int64_t off = static_cast<const char*>(b) - static_cast<const char*>(a);
+    const int64_t at = (off < 0 ? -off : off) % step_a;  // one's rows may lie between the other's, where both are as far apart
+    return step_a == step_b && width <= at && at <= step_a - width;
+}
+
 struct Gemm8Args {
     const int8_t* x;
     int64_t x_stride;

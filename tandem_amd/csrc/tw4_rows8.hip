@@ -49,6 +49,9 @@ struct RowsArgs {
 template <bool NORM, bool ADD, bool BF16, int W, int J>
 int rows_go(const RowsArgs& a) {
     TW4_REQUIRE(a.M * (64LL * W) < 1LL << 32, TW4_EINVAL, "%s: M = %d is too many rows of %d", NORM ? "rms_norm_int8" : "quantize_int8", a.M, 8 * a.chunks);
+    if constexpr (ADD)  // rows are read and written by different workgroups at once
+        TW4_REQUIRE(rows_apart(a.x, 16 * a.x_step, a.r, 16 * a.r_step, a.M, 16LL * a.chunks), TW4_EINVAL,
+                    "rms_norm_int8: the residual needs memory of its own");
     rows_int8_kernel<NORM, ADD, BF16, W, J>
         <<<static_cast<unsigned>(a.M), 64 * W, 0, a.st>>>(a.x, a.x_step, a.r, a.r_step, a.w, a.eps, a.codes, a.scales, a.chunks);
     hipError_t e = hipGetLastError();
