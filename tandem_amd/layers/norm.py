@@ -111,8 +111,8 @@ def _apart(a: int, step_a: int, b: int, step_b: int, rows: int, width: int) -> b
 def _rms_norm_int8(who: str, x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor,
                    eps: float) -> tuple[torch.Tensor, torch.Tensor]:
     step, r_step, m, k, code, index = check_rows(who, layout(x), None if residual is None else layout(residual), layout(weight))
-    if not (w4_hip.plain(x) if residual is None else w4_hip.all_plain(x, residual)):
-        raise RuntimeError(f"{who}: inference only, no gradient, transform or tracer can follow x or the residual")
+    if not (w4_hip.all_plain(x, weight) if residual is None else w4_hip.all_plain(x, residual, weight)):
+        raise RuntimeError(f"{who}: inference only, no gradient, transform or tracer can follow x, the residual or the weight")
     codes, scales = x.new_empty(m, k, dtype=torch.int8), x.new_empty(m, dtype=torch.float32)
     if m:
         xp, rp, wp = x.data_ptr(), 0 if residual is None else residual.data_ptr(), weight.data_ptr()
@@ -133,7 +133,8 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float) -> tuple[to
 
     A row that holds an infinity or a NaN (in x, the weight, or their product in float32) has scale NaN and codes 0, so that
     its products are NaN; one with every |t| below 2^-100 has scale 0 and codes 0. One whose sum of squares leaves float32 (bfloat16
-    from about 10^18 on; with eps 0, all below 10^-22) has scale NaN too. Inference only."""
+    from about 10^18 on; with eps 0, all below 10^-22) has scale NaN too. Inference only: an x, residual or weight that
+    a gradient, tangent or transform follows is refused."""
     return _rms_norm_int8("rms_norm_int8", x, None, weight, eps)
 
 

@@ -123,7 +123,8 @@ def _token_int8(x: torch.Tensor, residual: torch.Tensor | None, norm_weight: tor
     sizes, w_step, features, index = _checked_token(layout(x), None if residual is None else layout(residual),
                                                     None if norm_weight is None else layout(norm_weight), layout(weight),
                                                     layout(weight_scale), silu_mul)
-    if not (w4_hip.all_plain(x, weight, weight_scale) if residual is None else w4_hip.all_plain(x, residual, weight, weight_scale)):
+    operands = (x, weight, weight_scale) if norm_weight is None else (x, weight, weight_scale, norm_weight)
+    if not w4_hip.all_plain(*(operands if residual is None else (*operands, residual))):
         raise RuntimeError("token_int8: inference only, no gradient, transform or tracer can follow the operands")
     y, total = x.new_empty(1, features), None if residual is None else x.new_empty(1, sizes[1])
     xp, wp = x.data_ptr(), weight.data_ptr()

@@ -7,6 +7,7 @@ import ctypes
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from tandem_amd.layers import norm, w4_hip, w8
 
@@ -109,3 +110,37 @@ def test_memory_side_by_side():
     w4_hip.check(lib.tw4_token_int8(at[0], at[1], at[3], at[2], 1e-6, w.data_ptr(), k, ws.data_ptr(), at[4], n, k, 0, 0, 256, w4_hip.raw_stream(0)))
     assert torch.equal(row[3 * k:4 * k], want[2][0]) and torch.equal(row[4 * k:], w8.linear_int8(codes[:1], scales[:1], w, ws)[0])
     assert torch.equal(row[:2 * k], before[0]) and torch.equal(row[2 * k:3 * k], weight)
+
+
+class Own(torch.Tensor):
+    pass
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 3])
+def test_norm_weights_that_are_followed(m):
+    """A norm's weight that a gradient, a tangent, a transform or a type of its own follows is refused, for one token and for more, as every other operand
+    is; where no gradient is asked for it is a value."""
+    k = 64
+    layer = w8.W8Linear(k, 32).cuda()
+    layer.weight.random_(-127, 128)
+    layer.weight_scale.fill_(0.01)
+    x, r = torch.randn(m, k, device="cuda").half(), torch.randn(m, k, device="cuda").half()
+    plain = torch.rand(k, device="cuda").half() + 0.5
+    calls = (lambda w: norm.rms_norm_int8(x, w, 1e-6), lambda w: norm.fused_add_rms_norm_int8(x, r.clone(), w, 1e-6),
+             lambda w: layer.forward_norm(x, None, w, 1e-6), lambda w: layer.forward_norm(x, r.clone(), w, 1e-6))
+    weight = torch.nn.Parameter(plain.clone())
+    for call in calls:
+        want = call(plain)
+        with pytest.raises(RuntimeError, match="inference only"):
+            call(weight)
+        with pytest.raises(RuntimeError, match="inference only"):
+            call(plain.as_subclass(Own))
+        with forward_ad.dual_level(), pytest.raises(RuntimeError, match="inference only"):
+            call(forward_ad.make_dual(plain, torch.ones_like(plain)))
+        with pytest.raises(RuntimeError, match="inference only"):
+            torch.func.vmap(lambda w: call(w)[0])(plain[None])
+        with torch.no_grad():
+            got = call(weight)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert all(torch.equal(a, b) for a, b in zip(call(torch.nn.Parameter(plain, requires_grad=False)), want))
