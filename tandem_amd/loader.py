@@ -37,6 +37,8 @@ from typing import Any, Optional
 import torch
 from torch import nn
 
+from tandem_amd.layers.w8 import W8Linear
+
 logger = logging.getLogger(__name__)
 
 AWQ_TENSORS = ("qweight", "qzeros", "scales")
@@ -137,7 +139,8 @@ def fused_sources(target: str) -> Optional[tuple[list[str], int]]:
 def model_tensors(model: nn.Module) -> dict[str, torch.Tensor]:
     """What a checkpoint fills: every parameter, and the buffers W4Linear (AutoAWQ) and W8Linear register."""
     out = dict(model.named_parameters())
-    out.update((n, b) for n, b in model.named_buffers() if n.rsplit(".", 1)[-1] in AWQ_TENSORS + W8_TENSORS)
+    int8 = {f"{n}.{t}" if n else t for n, m in model.named_modules() if isinstance(m, W8Linear) for t in W8_TENSORS}
+    out.update((n, b) for n, b in model.named_buffers() if n.rsplit(".", 1)[-1] in AWQ_TENSORS or n in int8)
     return out
 
 
