@@ -19,7 +19,7 @@ comes from (``plan_sources``): a checkpoint tensor of the same name, or the list
 tensors that stacked along the output dimension make it up. The output dimension is dim 0 of a
 dense weight or bias and dim 1 of the AutoAWQ tensors (qweight [K, N/8], qzeros [K/G, N/8],
 scales [K/G, N]), so ``fused_sources`` records the axis with the names. Every plan is checked
-(sources present, stacked shape equal to the target's) before any data is copied. Loading is host
+(sources present, stacked shape equal to the target's, codes stored as int8) before any data is copied. Loading is host
 work on CPU tensors; the layers are moved to the GPU and repacked afterwards by
 ``finalize_quantized`` (see ``tandem_amd.model.prepare``).
 """
@@ -190,12 +190,13 @@ def load_weights(model: nn.Module, model_path: str) -> None:
             if got != tuple(targets[name].shape):
                 detail = ", ".join(f"{s} {shape_of[s]}" for s in srcs)
                 raise ValueError(f"shape mismatch for {name}: model {tuple(targets[name].shape)}, checkpoint {detail}")
+            types = [where[s].get_slice(s).get_dtype() for s in srcs] if targets[name].dtype == torch.int8 else []
+            if any(t != "I8" for t in types):
+                raise ValueError(f"{name}: int8 tensors expected, checkpoint {types}")
         with torch.no_grad():
             for name, (srcs, axis) in plans.items():
                 dst = targets[name]
                 parts = [where[s].get_tensor(s) for s in srcs]
-                if dst.dtype == torch.int8 and any(p.dtype != torch.int8 for p in parts):
-                    raise ValueError(f"{name}: int8 tensors expected, checkpoint {[str(p.dtype) for p in parts]}")
                 dst.copy_((parts[0] if len(parts) == 1 else torch.cat(parts, dim=axis)).to(dst.dtype))
         used = {s for srcs, _ in plans.values() for s in srcs}
         extra = sorted(n for n in where if n not in used and n != "lm_head.weight" and not n.endswith(_NOT_STATE))

@@ -43,3 +43,14 @@ def test_other_modules_buffers_are_left_alone(tmp_path):
 def test_a_layer_that_is_the_model(tmp_path):
     layer = w8.W8Linear(16, 3)
     assert set(loader.model_tensors(layer)) == {"weight", "weight_scale"}
+
+
+def test_types_are_checked_before_anything_is_copied(tmp_path):
+    model = nn.Module()
+    model.first, model.proj = nn.Linear(4, 2, bias=False), w8.W8Linear(32, 6)
+    _save(tmp_path, {"first.weight": torch.zeros(2, 4), "proj.weight": torch.zeros(6, 32, dtype=torch.uint8), "proj.weight_scale": torch.ones(6, 1)})
+    model.proj.weight.fill_(1)
+    before = {n: t.clone() for n, t in loader.model_tensors(model).items()}
+    with pytest.raises(ValueError, match="proj.weight: int8 tensors expected"):
+        loader.load_weights(model, str(tmp_path))
+    assert all(torch.equal(t.nan_to_num(), before[n].nan_to_num()) for n, t in loader.model_tensors(model).items())
