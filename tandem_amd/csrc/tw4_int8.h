@@ -1,4 +1,5 @@
-// What the operators on 8-bit integers share: the two 16-bit types activations come in, and the epilogue of the products.
+// What the operators on 8-bit integers share: the two 16-bit types activations come in, SwiGLU, the matrix instruction, the host's look at overlapping
+// memory, and the products' arguments and tiles.
 #pragma once
 
 #include "tw4_common.h"
@@ -74,21 +75,6 @@ __device__ __forceinline__ i4 mfma_i8(const u4& a, const u4& b, const i4& c) {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(bitcast<i4>(a), bitcast<i4>(b), c, 0, 0, 0);
 }
 
-// Output features n .. n + 3 of one token: sums times both scales, rounded once. wide: N % 4 == 0 and y 8-byte aligned, so that the
-// four lie in the row together.
-template <bool BF16>
-__device__ __forceinline__ void store_features(uint16_t* row, int n, int N, bool wide, const float (&v)[4]) {
-    if (wide) {
-        if (n < N)
-            *reinterpret_cast<u2*>(row + n) =
-                u2{value16<BF16>(v[0]) | value16<BF16>(v[1]) << 16, value16<BF16>(v[2]) | value16<BF16>(v[3]) << 16};
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (n + i < N) row[n + i] = static_cast<uint16_t>(value16<BF16>(v[i]));
-    }
-}
-
 // Whether so many bytes from a and from b on are apart (host).
 inline bool bytes_apart(const void* a, int64_t bytes_a, const void* b, int64_t bytes_b) {
     return static_cast<const char*>(a) + bytes_a <= b || static_cast<const char*>(b) + bytes_b <= a;
@@ -121,7 +107,10 @@ struct Gemm8Args {
 #define TW4_GEMM8_LDS(X)                                                                                             \
     X(1, 1, 2, 1, 2, 7) X(2, 1, 2, 1, 2, 3) X(3, 1, 2, 2, 2, 5) X(4, 2, 2, 2, 2, 5) X(5, 2, 2, 2, 4, 6) X(6, 4, 2, 2, 4, 3) \
     X(7, 6, 2, 2, 2, 3) X(8, 4, 6, 2, 2, 2) X(9, 6, 4, 2, 2, 2) X(10, 4, 4, 2, 4, 3) X(11, 4, 4, 4, 2, 3) X(12, 8, 4, 2, 4, 2)
-constexpr int kGemm8Kernels = 13;
+#define TW4_COUNT(...) +1
+constexpr int kGemm8Kernels = 1 TW4_GEMM8_LDS(TW4_COUNT);
+#undef TW4_COUNT
+static_assert(kGemm8Kernels == TW4_GEMM_INT8_KERNELS, "the header's count");
 
 int gemm8_stream(const Gemm8Args& a, int rows);             // tw4_gemm8.hip
 int gemm8_lds(const Gemm8Args& a, int kernel, int splits);  // tw4_gemm8_lds.hip
