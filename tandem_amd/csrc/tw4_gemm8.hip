@@ -249,7 +249,7 @@ int gemm8_stream(const Gemm8Args& a, int rows) {
 // Coefficients in microseconds on MI355X (256 CUs), a row for one tile of tokens (w read once, not kept) and one for more, from least
 // squares on relative errors over 520 sizes (20 K x N, M = 1 .. 8192, w streamed from HBM) x up to 60 kernels and splits each
 // (profiles/gemm_int8_rule_sweep.jsonl). The choice is 0.9 % slower than the fastest that was timed on average, 20 % at
-// most.
+// most. The times are those of the tiles listed in tw4_int8.h and their epilogue: what changes either makes them stale.
 struct Gemm8Cost {
     double start, round, stage, share, split, part, rate, step, cu;
 };

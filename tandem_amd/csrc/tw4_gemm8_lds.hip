@@ -18,8 +18,9 @@
 // M = 8192 keeps the cores busy 58 % of the cycles at 1.8 GHz, wavefronts wait 37 % of theirs (stages come from past L2: 1.2 GB of
 // it, and with every load a hit the loop runs 20 % faster), LDS is busy 25 %. 674-702 us, 2.35-2.45 POP/s, where the library's int8 product
 // without scales or SwiGLU takes 765; K 12288 x N 4096 304 (341), K 4096 x N 4096 113-119 (126); at M = 512 18 (22), K 12288 40 (45).
-// Middle sizes: a stage's chain of barrier, LDS reads and products, and how evenly the tiles divide over the CUs. Few tokens: reading w,
-// 5.0 TB/s of it (K 4096 x N 24576, M = 1 .. 16: 20-22 us).
+// Middle sizes: how fast stages come into LDS, 58-72 KB/us a CU with all CUs at work whatever the tile's shape (the fitted stages of tw4_gemm8.hip; the
+// products of a stage at 5 POP/s are 14 to 56 % of that time, and a second workgroup of the small tiles on the CU overlaps with nothing), and how evenly the
+// tiles divide over the CUs. Few tokens: reading w, 5.0 TB/s of it (K 4096 x N 24576, M = 1 .. 16: 20-22 us).
 // Measured steps, us, K 4096: results straight from the accumulators, 8 bytes a lane, and the scales read for each tile: M = 8192, N 4096 134,
 // through LDS 115; N 5001 (K 2064), M = 2048 45 -> 36. Non-temporal w: N 24576, M = 16 21.9 -> 19.8, N 34816 (K 5120) 41.8 -> 38.1.
 // v_mfma_i32_32x32x32_i8 instead, the same tiles: 5-30 % slower at every size. Stages of 64 k in 4 or 5 slots (a barrier

@@ -45,16 +45,16 @@ __device__ __forceinline__ u4 values_chunk(const float (&f)[8]) {
 // M = 512 57.3 -> 55.9 us, 2048 191 -> 185; level at 8192, which the card's power bounds.
 __device__ __forceinline__ float silu_rcp(float g) { return g * __builtin_amdgcn_rcpf(1.0f + __expf(-g)); }
 
-// Below kSiluFar exp(-g) comes to pass 2^126, whose reciprocal that instruction flushes to 0, and float32 later on. 1 + exp(-g) is exp(-g) there, and g exp(g)
-// = (g exp(g / 2)) exp(g / 2) rounds once more than it has to, and to subnormal numbers only in its last product.
+// Below kSiluFar exp(-g) comes to pass 2^126, whose reciprocal that instruction flushes to 0, and float32 later on. 1 + exp(-g) is exp(-g)
+// there, and g exp(g) = (g exp(g / 2)) exp(g / 2) meets subnormal numbers in its last product only.
 constexpr float kSiluFar = -87.0f;
 __device__ __forceinline__ float silu_far(float g) {
     const float e = __expf(0.5f * g);
     return g * e * e;
 }
 
-// g[i] becomes silu(g[i]). Gates that far out are few or none: a wavefront without one jumps over their form (K 2560 x N 19456, M = 200 18.1 -> 18.4 us
-// for the look; M = 5 and 8192 level).
+// g[i] becomes silu(g[i]). Gates that far out are few or none: a wavefront without one jumps over their form (the look costs K 2560 x N
+// 19456 at M = 200 0.3 us, 18.1 -> 18.4; M = 5 and 8192 are level).
 template <int N>
 __device__ __forceinline__ void silu_values(float (&g)[N]) {
     float least = g[0], s[N];

@@ -186,7 +186,8 @@ class W8Linear(nn.Module):
     def forward_norm(self, x: torch.Tensor, residual: torch.Tensor | None, norm_weight: torch.Tensor,
                      eps: float) -> tuple[torch.Tensor, torch.Tensor]:
         """self(rms_norm(x + residual) * norm_weight), the norm's output in 8 bits as it is written, and the new residual (x itself without
-        one). residual is consumed, as W4Linear's: one token gets the new one in fresh memory, more have it written in place."""
+        one). residual is consumed, as W4Linear's: one token gets the new one in fresh memory, more have it written in place. Rows [M, K] only. It
+        does not go through forward: hooks on the layer do not see it."""
         if x.dim() == 2 and self._one_token(x):
             y, total = _token_int8(x, residual, norm_weight, eps, self.weight, self.weight_scale, self.silu_mul)
             return y, x if residual is None else total
